@@ -229,6 +229,55 @@ NVFP4_API int nvfp4_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, v
                              void* sf_blocked, void* stream);
 
 /*
+ * Routing of tokens to experts.  Per row of logits [T, E] (dtype 0 float32,
+ * 1 float16, 2 bfloat16; row stride ld elements):
+ *   s_e = softmax(x)_e (score 0) or 1 / (1 + exp(-x_e)) (score 1);
+ *   c_e = s_e + bias_e (bias: float32 [E], or NULL; without it the experts
+ *         rank by x_e, which is the same order in exact arithmetic);
+ *   a group's score is the sum of its group_top (1 or 2) largest c; experts
+ *   outside the top_groups best of the `groups` equal groups are off;
+ *   ids[t, 0..k) = the k largest c in descending order, ties to the lowest
+ *   index (of groups, too); weights = s of those, divided by their sum when
+ *   renorm is non-zero, times scale.
+ * An expert whose logit or bias is -inf or NaN is off: it has score 0, and a
+ * slot that no expert fills gets id -1 and weight 0.  +inf counts as the
+ * largest float.  The ids are those of 64-bit arithmetic; weights are float32.
+ * 1 <= E <= 1024, k <= min(32, E), groups <= 32 and divides E; T may be 0.
+ * weights and ids are contiguous [T, k].  No counterpart in the reference.
+ */
+NVFP4_API int nvfp4_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, const float* bias,
+                                  int score, int64_t k, int64_t groups, int64_t top_groups, int group_top, int renorm,
+                                  float scale, float* weights, int32_t* ids, void* stream);
+
+/*
+ * The SiLU-gated MLP of the experts that each token chose, NVFP4 weights:
+ *   xq = nvfp4(x[t]);  h = silu(xq . Wg_e^T) * (xq . Wu_e^T);  hq = nvfp4(h);
+ *   out[t] = sum_j weights[t, j] * (hq . Wd_e^T),   e = ids[t, j]
+ * with nvfp4() the quantisation of nvfp4_quantize (h from its fp32 value),
+ * fp32 accumulation, and one rounding to fp16 at the end.  A slot whose id is
+ * not in [0, E) is skipped (nvfp4_route_experts fills empty slots with -1); a
+ * token without any gets zeros.  Finite inputs.
+ *   x [T, D] fp16 (row stride ldx elements), ids [T, k] int32, weights [T, k]
+ *   float32, both contiguous; out [T, D] fp16 (row stride ldo elements; out
+ *   may be x);
+ *   w_gate, w_up [E][F][D/2], w_down [E][D][F/2] codes with byte strides ld_*
+ *   (rows) and es_* (experts), multiples of 16; their scales in the blocked
+ *   layout per expert, sfe_* bytes from expert to expert (a multiple of 16).
+ *   Gate and up share their strides.
+ * D and F are multiples of 64; E <= 1024, k <= 32, T * k <= 2^24; T may be 0.
+ * The counts per expert stay on the GPU.  `workspace` is device memory of at
+ * least nvfp4_moe_workspace() bytes, 256-byte aligned, with undefined contents,
+ * in use until the call's work on `stream` ends.  No counterpart in the
+ * reference.
+ */
+NVFP4_API int nvfp4_moe_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F, int64_t* bytes);
+NVFP4_API int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, const float* weights, int64_t T, int64_t k,
+                            int64_t E, int64_t D, int64_t F, const void* w_gate, const void* w_up, const void* sf_gate,
+                            const void* sf_up, int64_t ld_in, int64_t es_in, int64_t sfe_in, const void* w_down,
+                            const void* sf_down, int64_t ld_down, int64_t es_down, int64_t sfe_down, void* out,
+                            int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Tensor-core peak probe: one CTA per SM issues `iters` dense 128x256x64
  * kind::mxf4nvf4 MMAs (4,194,304 FLOP each) from shared memory.  Time it with
  * events on `stream` to get the device's FP4 tensor throughput, the

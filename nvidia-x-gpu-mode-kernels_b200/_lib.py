@@ -39,6 +39,11 @@ SIGNATURES: dict[str, list] = {
     "nvfp4_mma_peak_pattern": [ctypes.c_int, ctypes.c_int, VP],
     "nvfp4_quantize": [VP, I64, I64, I64, VP, I64, VP, VP],
     "nvfp4_gemm_skinny": [VP, VP, VP, VP, VP, I64, I64, I64, I64, I64, I64, VP],
+    "nvfp4_route_experts": [VP, ctypes.c_int, I64, I64, I64, VP, ctypes.c_int, I64, I64, I64, ctypes.c_int,
+                            ctypes.c_int, ctypes.c_float, VP, VP, VP],
+    "nvfp4_moe_workspace": [I64, I64, I64, I64, I64, ctypes.POINTER(I64)],
+    "nvfp4_moe_mlp": [VP, I64, VP, VP, I64, I64, I64, I64, I64, VP, VP, VP, VP, I64, I64, I64, VP, VP, I64, I64, I64,
+                      VP, I64, VP, I64, VP],
     "nvfp4_gemv_grid": [I64, I64, I64, ctypes.POINTER(I64)],
     "nvfp4_set_peer_wait_ns": [ctypes.c_uint64],
     "nvfp4_gemv_allgather": [VP, VP, VP, VP, I64, I64, I64, I64, I64, I64, I64, I64, I64,

@@ -1,0 +1,389 @@
+// The experts' products on the tcgen05 tensor cores: for every row tile of the
+// plan (rows of one expert, ordered by expert) and every tile of the expert's
+// weight rows,
+//
+//   gate and up (DUAL):  h = silu(x . Wg^T) * (x . Wu^T), quantised to NVFP4 in the epilogue
+//   down:                y = weight[row] * (h . Wd^T), in fp32
+//
+// The walk over tiles reads the plan from device memory, so one launch serves
+// any split of the tokens over the experts, known to the host or not.  Weights
+// are [experts, rows, K/2] codes (3-D tensor map) with blocked scales
+// [experts][row tiles][K/64][512 bytes] (4-D map).
+//
+// TRANS 0: the tokens are the MMA's 128-row operand, BN weight rows its other
+// one; an epilogue thread holds one token's row.  TRANS 1, for few tokens per
+// expert: 128 weight rows are the MMA's first operand and BN tokens (16, 32 or
+// 64) the other, so the tensor cores' work shrinks with the tokens and the
+// weights stream; an epilogue lane holds one weight row of every token.
+//
+// Warp roles and the two-barrier stages are those of gemm_kernel: warp 0 TMA
+// producer, warp 1 MMA, warps 2-5 epilogue, warps 6-9 copy the scales into
+// tensor memory.  Every wait is bounded.
+#pragma once
+#include "plan.cuh"
+#include "quant.cuh"
+
+namespace nvfp4 {
+namespace {
+
+struct ExpertParams {
+  CUtensorMap tt, tst;              // tokens: codes [rows][K/2], scales [row tiles][K/64][128 x u32]
+  CUtensorMap tw[2], tsw[2];        // weights (gate and up, or down) and their scales
+  const PlanTile* tiles;
+  const int* ntiles;
+  int N, K;                         // weight rows of one matrix, inner dimension
+  int wtiles;                       // tiles of weight rows
+  uint8_t* codes;                   // DUAL: h [rows][N/2] and its blocked scales
+  uint8_t* sf;
+  float* y;                         // down: [rows][N]
+  const float* row_weight;
+  uint32_t* err;
+};
+
+template <bool TRANS_, bool DUAL_, int BN_, int KA_, int STAGES_>
+struct ExpertCfg {
+  static constexpr bool TRANS = TRANS_, DUAL = DUAL_;
+  static constexpr int BN = BN_, KA = KA_, STAGES = STAGES_;
+  static constexpr int KPS = 4 * KA;                       // 64-element K blocks per stage
+  static constexpr int NW = DUAL ? 2 : 1;                  // weight matrices
+  static constexpr int T_ROWS = TRANS ? BN : BM;           // tokens per tile
+  static constexpr int W_ROWS = TRANS ? BM : BN;           // weight rows per tile
+  static constexpr int NBW = W_ROWS / 128;                 // scale blocks of a weight tile
+  static_assert(W_ROWS % 128 == 0, "weight tiles are whole scale blocks");
+  static_assert(!TRANS || BN == 16 || BN == 32 || BN == 64, "token tiles");
+  static constexpr int T_ATOM = T_ROWS * KSTEP_BYTES, W_ATOM = W_ROWS * KSTEP_BYTES;
+  static constexpr int T_BYTES = KA * T_ATOM, W_BYTES = KA * W_ATOM;
+  static constexpr int OFF_W = T_BYTES;
+  static constexpr int SFT_BYTES = KPS * 512;
+  static constexpr int SFW_BYTES = NBW * KPS * 512;        // per weight matrix
+  static constexpr int OFF_SFT = OFF_W + NW * W_BYTES;
+  static constexpr int OFF_SFW = OFF_SFT + SFT_BYTES;
+  static constexpr int STAGE_BYTES = (OFF_SFW + NW * SFW_BYTES + 1023) / 1024 * 1024;
+  static constexpr int OFF_BAR = STAGES * STAGE_BYTES;
+  static constexpr int OFF_BUF = OFF_BAR + 512;            // TRANS && DUAL: a 16 x 36 float patch per epilogue warp
+  static constexpr int BUF_BYTES = TRANS && DUAL ? 4 * 16 * 36 * 4 : 0;
+  static constexpr int SMEM = OFF_BUF + BUF_BYTES;
+  static_assert((4 * STAGES + 2) * 8 + 4 <= 512, "barriers");
+  static constexpr uint32_t OP_BYTES = T_BYTES + NW * W_BYTES;
+  static constexpr uint32_t SF_BYTES = SFT_BYTES + NW * SFW_BYTES;
+  // tensor memory columns
+  static constexpr int SF_BASE = NW * BN;                  // the accumulators come first
+  static constexpr int SFT_COLS = 4 * KPS;
+  static constexpr int SFW_COLS = KPS * NBW * 4;           // per weight matrix
+  static constexpr int SF_STAGE_COLS = SFT_COLS + NW * SFW_COLS;
+  static constexpr int TMEM_COLS = 512;
+  static_assert(SF_BASE + STAGES * SF_STAGE_COLS <= TMEM_COLS, "tensor memory budget");
+  static_assert(SMEM <= 232448, "shared memory budget");
+  static_assert(SMEM < (1 << 18), "descriptor address field");
+  static constexpr int THREADS = 320;
+  static constexpr uint32_t IDESC = tc::idesc_mxf4nvf4(BM, BN);
+};
+
+template <class C>
+__device__ __forceinline__ void expert_mma(uint32_t tmem, uint64_t dt, uint64_t dw, uint32_t sft, uint32_t sfw,
+                                           int kk, uint32_t accum) {
+  const uint64_t ot = (uint64_t)((kk >> 2) * (C::T_ATOM >> 4) + 2 * (kk & 3));
+  const uint64_t ow = (uint64_t)((kk >> 2) * (C::W_ATOM >> 4) + 2 * (kk & 3));
+#pragma unroll
+  for (int m = 0; m < C::NW; ++m) {
+    const uint64_t w = dw + (uint64_t)(m * (C::W_BYTES >> 4)) + ow;
+    const uint32_t s = sfw + m * C::SFW_COLS + kk * C::NBW * 4;
+    if (C::TRANS) tc::mma_mxf4nvf4(tmem + m * C::BN, w, dt + ot, C::IDESC, s, sft + 4 * kk, accum);
+    else tc::mma_mxf4nvf4(tmem + m * C::BN, dt + ot, w, C::IDESC, sft + 4 * kk, s, accum);
+  }
+}
+
+// Byte of the blocked scale layout that belongs to (row, 16-element block).
+__device__ __forceinline__ int64_t blocked_at(int row, int block, int64_t nk64) {
+  return ((int64_t)(row >> 7) * nk64 + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
+}
+
+template <class C>
+__global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_constant__ ExpertParams P) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  const uint32_t sbase = smem_u32(smem_raw);
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  griddep_launch();
+  if (sbase & 1023u) {  // the swizzled tiles need a 1024-aligned base; the launch guarantees it
+    if (threadIdx.x == 0) atomicOr(P.err, kDevErrTimeoutMma);
+    griddep_wait();
+    return;
+  }
+  const uint32_t bar_full = sbase + C::OFF_BAR;             // operand boxes landed
+  const uint32_t bar_empty = bar_full + 8 * C::STAGES;      // stage consumed by the MMAs
+  const uint32_t bar_sfr = bar_empty + 8 * C::STAGES;       // scales staged in tensor memory
+  const uint32_t bar_sff = bar_sfr + 8 * C::STAGES;         // scale boxes landed
+  const uint32_t bar_accf = bar_sff + 8 * C::STAGES;
+  const uint32_t bar_acce = bar_accf + 8;
+  const uint32_t tmem_slot = bar_acce + 8;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_empty + 8 * s, 1);
+      mbar_init(bar_sfr + 8 * s, 4);
+      mbar_init(bar_sff + 8 * s, 1);
+    }
+    mbar_init(bar_accf, 1);
+    mbar_init(bar_acce, 4);
+    fence_mbar_init();
+    prefetch_tmap(&P.tt);
+    prefetch_tmap(&P.tst);
+#pragma unroll
+    for (int m = 0; m < C::NW; ++m) {
+      prefetch_tmap(&P.tw[m]);
+      prefetch_tmap(&P.tsw[m]);
+    }
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, C::TMEM_COLS);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - sbase));
+  griddep_wait();                                           // the plan and the operands are written
+  const int total = *P.ntiles * P.wtiles;
+  const int nk64 = P.K / 64;
+  const int nks = (nk64 + C::KPS - 1) / C::KPS;
+
+  if (warp == 0) {
+    // ---------------------------- producer ----------------------------
+    if (lane == 0) {
+      const uint64_t pol_t = policy_evict_last();    // token tiles are re-read by every weight tile
+      const uint64_t pol_w = policy_evict_first();
+      uint32_t it = 0;
+      for (int t = blockIdx.x; t < total; t += gridDim.x) {
+        const PlanTile q = P.tiles[t / P.wtiles];
+        const int local = t - q.first * P.wtiles;
+        const int row = q.row0 + local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
+        for (int ks = 0; ks < nks; ++ks, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(bar_empty + 8 * s, ((it / C::STAGES) & 1) ^ 1, P.err, kDevErrTimeoutEmpty)) goto done;
+          const uint32_t st = sbase + s * C::STAGE_BYTES;
+          // scales first, on their own barrier; boxes always count in full
+          // (what lies past the end of a matrix or of K reads as zeros)
+          const uint32_t sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
+          mbar_arrive_expect_tx(sb, C::SF_BYTES);
+          tma_load_3d(st + C::OFF_SFT, &P.tst, sb, 0, C::KPS * ks, row / 128, pol_t);
+#pragma unroll
+          for (int m = 0; m < C::NW; ++m)
+            tma_load_4d(st + C::OFF_SFW + m * C::SFW_BYTES, &P.tsw[m], sb, 0, C::KPS * ks, w0 / 128, q.index, pol_w);
+          mbar_arrive_expect_tx(fb, C::OP_BYTES);
+#pragma unroll
+          for (int a = 0; a < C::KA; ++a) {
+            const int x = (ks * C::KA + a) * KSTEP_BYTES;
+            tma_load_2d(st + a * C::T_ATOM, &P.tt, fb, x, row, pol_t);
+#pragma unroll
+            for (int m = 0; m < C::NW; ++m)
+              tma_load_3d(st + C::OFF_W + m * C::W_BYTES + a * C::W_ATOM, &P.tw[m], fb, x, w0, q.index, pol_w);
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------ MMA -------------------------------
+    if (lane == 0) {
+      const uint64_t dt0 = tc::desc_sw128(sbase), dw0 = tc::desc_sw128(sbase + C::OFF_W);
+      uint32_t it = 0, tile_it = 0;
+      for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
+        if (!mbar_wait(bar_acce, (tile_it & 1) ^ 1, P.err, kDevErrTimeoutMma)) goto done;
+        tc::fence_after_sync();
+        for (int ks = 0; ks < nks; ++ks, ++it) {
+          const int s = it % C::STAGES;
+          const uint32_t par = (it / C::STAGES) & 1;
+          if (!mbar_wait(bar_sfr + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
+          if (!mbar_wait(bar_full + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
+          tc::fence_after_sync();
+          const uint64_t soff = (uint64_t)((s * C::STAGE_BYTES) >> 4);
+          const uint32_t sf = tmem + C::SF_BASE + s * C::SF_STAGE_COLS;
+          const int nch = min(C::KPS, nk64 - C::KPS * ks);
+          if (nch == C::KPS) {   // a compile-time count: straight-line MMA issues
+#pragma unroll
+            for (int kk = 0; kk < C::KPS; ++kk)
+              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+          } else {
+            for (int kk = 0; kk < nch; ++kk)
+              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+          }
+          tc::commit(bar_empty + 8 * s);
+        }
+        tc::commit(bar_accf);
+      }
+    }
+  } else if (warp >= 6) {
+    // --------------------------- scale warps ---------------------------
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    uint32_t it = 0;
+    for (int t = blockIdx.x; t < total; t += gridDim.x) {
+      // A narrow token tile starts anywhere in its 128-row scale block, but the MMA reads a tile's scales from
+      // an aligned group of columns and from lane 0 on: they are moved there on the way to tensor memory.
+      // `from`: byte of this lane's first word in a 512-byte block.
+      int from = lane * 16;
+      if (C::TRANS) {
+        const PlanTile q = P.tiles[t / P.wtiles];
+        const int off = (q.row0 + (t - q.first * P.wtiles) % q.tiles * C::T_ROWS) % 128;
+        from = (lane + off) % 32 * 16 + off / 32 * 4;
+      }
+      for (int ks = 0; ks < nks; ++ks, ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(bar_sff + 8 * s, (it / C::STAGES) & 1, P.err, kDevErrTimeoutFull)) goto done;
+        const uint8_t* st = smem_raw + s * C::STAGE_BYTES;
+        const uint32_t sf = tmem + lane_base + C::SF_BASE + s * C::SF_STAGE_COLS;
+#pragma unroll
+        for (int kk = 0; kk < C::KPS; ++kk) {
+          uint4 v;
+          if constexpr (!C::TRANS) {
+            v = *reinterpret_cast<const uint4*>(st + C::OFF_SFT + kk * 512 + from);
+            tc::st_32x32b_x4(sf + 4 * kk, v.x, v.y, v.z, v.w);
+          } else if constexpr (C::BN == 64) {            // off is 0 or 64: two words, 8-byte aligned
+            const uint2 u = *reinterpret_cast<const uint2*>(st + C::OFF_SFT + kk * 512 + from);
+            tc::st_32x32b_x2(sf + 4 * kk, u.x, u.y);
+          } else {                                       // one column of up to 32 tokens
+            const uint32_t u = *reinterpret_cast<const uint32_t*>(st + C::OFF_SFT + kk * 512 + from);
+            tc::st_32x32b_x2(sf + 4 * kk, u, u);
+          }
+#pragma unroll
+          for (int m = 0; m < C::NW; ++m)
+#pragma unroll
+            for (int nb = 0; nb < C::NBW; ++nb) {
+              v = *reinterpret_cast<const uint4*>(st + C::OFF_SFW + m * C::SFW_BYTES + (nb * C::KPS + kk) * 512 + lane * 16);
+              tc::st_32x32b_x4(sf + C::SFT_COLS + m * C::SFW_COLS + (kk * C::NBW + nb) * 4, v.x, v.y, v.z, v.w);
+            }
+        }
+        tc::wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_sfr + 8 * s);
+      }
+    }
+  } else {
+    // ---------------------------- epilogue ----------------------------
+    const int sub = warp & 3;                 // tensor-memory lane quarter of this warp
+    const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16);
+    uint32_t tile_it = 0;
+    auto release = [&] {                      // the accumulators are read: the next tile's MMAs may start
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_acce);
+    };
+    for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
+      const PlanTile q = P.tiles[t / P.wtiles];
+      const int local = t - q.first * P.wtiles;
+      const int t0 = local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
+      if (!mbar_wait(bar_accf, tile_it & 1, P.err, kDevErrTimeoutMma)) break;
+      tc::fence_after_sync();
+      if constexpr (C::TRANS && C::DUAL) {
+        // lane = weight row, column = token: 16 tokens at a time through a patch of shared memory, so
+        // that a lane gets one token's block of 16 weight rows
+        float* buf = reinterpret_cast<float*>(smem_raw + C::OFF_BUF) + sub * 16 * 36;
+        const int blk = (w0 + sub * 32) / 16 + (lane & 1);
+#pragma unroll 1
+        for (int cb = 0; cb < C::BN / 16; ++cb) {
+          uint32_t g[32], u[32];
+          tc::ld_32x32b_x16(acc + cb * 16, g);
+          tc::ld_32x32b_x16(acc + C::BN + cb * 16, u);
+          tc::wait_ld();
+          if (cb == C::BN / 16 - 1) release();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) buf[j * 36 + lane] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
+          __syncwarp();
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float4 f = *reinterpret_cast<const float4*>(buf + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * j);
+            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+          }
+          __syncwarp();
+          const int tok = t0 + cb * 16 + (lane >> 1);
+          if (tok < q.rows && blk * 16 < P.N) {
+            const int row = q.row0 + tok;
+            uint32_t packed[2];
+            const uint32_t sbyte = quant_floats(v, packed);
+            *reinterpret_cast<uint2*>(P.codes + (int64_t)row * (P.N / 2) + blk * 8) = make_uint2(packed[0], packed[1]);
+            P.sf[blocked_at(row, blk, P.N / 64)] = (uint8_t)sbyte;
+          }
+        }
+      } else if constexpr (C::TRANS) {
+        constexpr int CHUNK = C::BN < 32 ? C::BN : 32;
+        const int col = w0 + sub * 32 + lane;
+#pragma unroll 1
+        for (int cb = 0; cb < C::BN / CHUNK; ++cb) {
+          uint32_t v[32];
+          if constexpr (CHUNK == 32) tc::ld_32x32b_x32(acc + cb * 32, v);
+          else tc::ld_32x32b_x16(acc + cb * CHUNK, v);
+          tc::wait_ld();
+          if (cb == C::BN / CHUNK - 1) release();
+          if (col < P.N) {
+#pragma unroll
+            for (int j = 0; j < CHUNK; ++j) {
+              const int tok = t0 + cb * CHUNK + j;
+              if (tok < q.rows)
+                P.y[(int64_t)(q.row0 + tok) * P.N + col] = P.row_weight[q.row0 + tok] * __uint_as_float(v[j]);
+            }
+          }
+        }
+      } else if constexpr (C::DUAL) {
+        // thread = token row: its blocks of 16 columns lie in its registers
+        const int tok = t0 + sub * 32 + lane, row = q.row0 + tok;
+#pragma unroll 1
+        for (int cb = 0; cb < C::BN / 64; ++cb) {
+          uint32_t codes[8], scales = 0;
+#pragma unroll
+          for (int b = 0; b < 4; ++b) {
+            uint32_t g[32], u[32];
+            tc::ld_32x32b_x16(acc + cb * 64 + b * 16, g);
+            tc::ld_32x32b_x16(acc + C::BN + cb * 64 + b * 16, u);
+            tc::wait_ld();
+            if (cb == C::BN / 64 - 1 && b == 3) release();
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
+            uint32_t packed[2];
+            scales |= quant_floats(v, packed) << (8 * b);
+            codes[2 * b] = packed[0];
+            codes[2 * b + 1] = packed[1];
+          }
+          const int col0 = w0 + cb * 64;             // N is a multiple of 64
+          if (tok < q.rows && col0 < P.N) {
+            uint4* dst = reinterpret_cast<uint4*>(P.codes + (int64_t)row * (P.N / 2) + col0 / 2);
+            dst[0] = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            dst[1] = make_uint4(codes[4], codes[5], codes[6], codes[7]);
+            *reinterpret_cast<uint32_t*>(P.sf + blocked_at(row, col0 / 16, P.N / 64)) = scales;
+          }
+        }
+      } else {
+        const int tok = t0 + sub * 32 + lane, row = q.row0 + tok;
+        const bool live = tok < q.rows;
+        const float weight = live ? P.row_weight[row] : 0.f;
+#pragma unroll 1
+        for (int cb = 0; cb < C::BN / 32; ++cb) {
+          uint32_t v[32];
+          tc::ld_32x32b_x32(acc + cb * 32, v);
+          tc::wait_ld();
+          if (cb == C::BN / 32 - 1) release();
+          const int col0 = w0 + cb * 32;             // N is a multiple of 64
+          if (live && col0 < P.N) {
+            float4* dst = reinterpret_cast<float4*>(P.y + (int64_t)row * P.N + col0);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(weight * __uint_as_float(v[4 * j]), weight * __uint_as_float(v[4 * j + 1]),
+                                   weight * __uint_as_float(v[4 * j + 2]), weight * __uint_as_float(v[4 * j + 3]));
+          }
+        }
+      }
+    }
+  }
+done:
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, C::TMEM_COLS);
+  }
+}
+
+}  // namespace
+}  // namespace nvfp4

@@ -1,0 +1,378 @@
+// Routing of tokens to experts: scores, limit to the best groups, top-k and
+// weights, one warp per token.
+//
+//   s_e = softmax(x)_e  or  1 / (1 + exp(-x_e))
+//   c_e = s_e + bias_e                      (the choice; without a bias the experts rank by x itself,
+//                                            the same order in exact arithmetic)
+//   group score = sum of the group's `group_top` largest c; experts outside the `top_groups` best groups are off
+//   ids = the k largest c, ties to the lowest index;  w_j = s_j / sum_j s_j * scale
+//
+// An expert whose logit or bias is -inf or NaN is off; +inf counts as the largest float.  Slots that no
+// expert fills get id -1 and weight 0.
+//
+// The ids are those of 64-bit arithmetic.  Scores are evaluated in 32 bits first; each comparison that
+// decides (the last group in against the first one out, and every neighbouring pair of the k + 1 best)
+// must differ by more than the 32-bit evaluation can be off, otherwise the warp repeats the row in 64
+// bits.  Comparisons of logits alone are exact and never repeat.
+//
+// Values are compared as unsigned keys that order like the numbers (0 = off), so a warp-wide maximum is one
+// redux instruction; the k best are taken one after the other, each with a maximum and a lowest index.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include "common.h"
+#include "ptx.cuh"
+
+namespace nvfp4 {
+namespace {
+
+constexpr int kMaxExperts = 1024, kMaxTopK = 32, kMaxGroups = 32;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  float* weights;
+  int32_t* ids;
+  int64_t T, ld;
+  int E, k, groups, top_groups, group_top, group_size;
+  int dtype;               // of the logits: 0 float, 1 half, 2 bfloat16
+  int renorm;
+  float scale;
+};
+
+// Order-preserving keys.  0 is below every number's key and means "off".
+template <typename R> struct KeyOf;
+template <> struct KeyOf<float> {
+  using U = uint32_t;
+  static __device__ __forceinline__ U key(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);   // -0 and +0 are one value
+    return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+  }
+  static __device__ __forceinline__ float value(U k) {
+    return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+  }
+  static __device__ __forceinline__ U warp_max(U v) { return __reduce_max_sync(kAll, v); }
+  static __device__ __forceinline__ float exponential(float v) { return expf(v); }
+  // for the screen alone: a sigmoid of these is within 1e-6 of the exact one
+  static __device__ __forceinline__ float rough_exponential(float v) { return __expf(v); }
+  static __device__ __forceinline__ float rough_quotient(float a, float b) { return __fdividef(a, b); }
+};
+template <> struct KeyOf<double> {
+  using U = unsigned long long;
+  static __device__ __forceinline__ U key(double v) {
+    const U b = (U)__double_as_longlong(v + 0.0);
+    return b ^ ((b >> 63) ? ~0ull : 0x8000000000000000ull);
+  }
+  static __device__ __forceinline__ double value(U k) {
+    return __longlong_as_double((long long)(k ^ ((k >> 63) ? 0x8000000000000000ull : ~0ull)));
+  }
+  static __device__ __forceinline__ U warp_max(U v) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      const U w = __shfl_xor_sync(kAll, v, o);
+      v = w > v ? w : v;
+    }
+    return v;
+  }
+  static __device__ __forceinline__ double exponential(double v) { return exp(v); }
+  static __device__ __forceinline__ double rough_exponential(double v) { return exp(v); }
+  static __device__ __forceinline__ double rough_quotient(double a, double b) { return a / b; }
+};
+
+template <typename R>
+__device__ __forceinline__ R warp_sum(R v) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+  return v;
+}
+
+// How far two 32-bit choices together may be off.  An approximate exponential of v is within
+// (2 + 1.5 |v|) * 2^-23 relative, an approximate quotient within 2^-22; a score of 1/(1 + e^-x) or e^(x-m)/z moves
+// by that times at most 1/4 (|v| s (1 - s) < 0.23) or 1 (|v| e^v < 0.37), a softmax's sum of up to 1024 terms by 16
+// roundings more, the bias rounds once: 1.5e-6 for one choice, 3e-6 for two, 4e-6 with room.  A group's
+// score is a sum of two.
+__device__ __forceinline__ bool too_near(float hi, float lo) {
+  return !(hi - lo > 4e-6f * fmaxf(1.0f, fmaxf(fabsf(hi), fabsf(lo))));
+}
+
+// One row in R arithmetic.  x: this lane's logits (expert i * 32 + lane), -inf where off.  Returns whether
+// a comparison was too near to be trusted (R = float only); lane j then holds slot j's id and weight.
+template <typename R, int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
+__device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float (&bias)[VPL],
+                          int lane, int& id, float& weight) {
+  using K = KeyOf<R>;
+  using U = typename K::U;
+  constexpr bool kScreen = sizeof(R) == 4;
+  bool near = false;
+  R m = 0, z = 0;
+  if (SOFTMAX) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, x[i]);
+    const uint32_t mk = __reduce_max_sync(kAll, KeyOf<float>::key(mx));
+    m = (R)KeyOf<float>::value(mk);
+    if (BIAS || GROUPS || !p.renorm) {
+      R part = 0;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (x[i] > -INFINITY) part += K::exponential((R)x[i] - m);
+      z = warp_sum(part);
+    }
+  }
+  auto score = [&](float v) -> R {      // of an expert that is on
+    if (SOFTMAX) return K::exponential((R)v - m) / z;
+    return (R)1 / ((R)1 + K::exponential(-(R)v));
+  };
+  auto rough_score = [&](float v) -> R {
+    if (SOFTMAX) return K::rough_quotient(K::rough_exponential((R)v - m), z);
+    return K::rough_quotient((R)1, (R)1 + K::rough_exponential(-(R)v));
+  };
+  U key[VPL];
+  if (BIAS || GROUPS) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      key[i] = 0;
+      if (x[i] > -INFINITY) {
+        const R c = BIAS ? rough_score(x[i]) + (R)bias[i] : rough_score(x[i]);
+        key[i] = K::key(c);
+      }
+    }
+  }
+  if (GROUPS) {
+    U mine = 0;                          // lane g: group g's score
+    // top, next: this lane's two largest of the group
+    auto group_score = [&](int g, U top, U next) {
+      const U first = K::warp_max(top);
+      R sum = K::value(first);
+      if (p.group_top == 2) {
+        // the second largest: the (lowest) lane that holds the largest offers its next
+        const unsigned holders = __ballot_sync(kAll, top == first);
+        if (lane == __ffs(holders) - 1) top = next;
+        const U second = K::warp_max(top);
+        if (second) sum += K::value(second);
+      }
+      if (lane == g && first) mine = K::key(sum);
+    };
+    if (p.group_size % 32 == 0) {        // groups are runs of registers: one pass over them
+      U top = 0, next = 0;
+      int g = 0, left = p.group_size;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        if (g < p.groups) {
+          next = key[i] > top ? top : (key[i] > next ? key[i] : next);
+          top = key[i] > top ? key[i] : top;
+          if ((left -= 32) == 0) {
+            group_score(g++, top, next);
+            top = next = 0;
+            left = p.group_size;
+          }
+        }
+      }
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        U top = 0, next = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const int e = i * 32 + lane - g * p.group_size;
+          if (e < 0 || e >= p.group_size) continue;
+          next = key[i] > top ? top : (key[i] > next ? key[i] : next);
+          top = key[i] > top ? key[i] : top;
+        }
+        group_score(g, top, next);
+      }
+    }
+    unsigned chosen = 0;
+    U last = 0;
+    for (int q = 0; q < p.top_groups; ++q) {
+      const U best = K::warp_max((chosen >> lane) & 1 ? 0 : mine);
+      if (best == 0) break;
+      const unsigned at = __ballot_sync(kAll, mine == best && !((chosen >> lane) & 1));
+      chosen |= at & (0u - at);
+      last = best;
+    }
+    if (kScreen && last) {
+      const U out = K::warp_max((chosen >> lane) & 1 ? 0 : mine);
+      if (out) near = near || too_near((float)K::value(last) * 0.5f, (float)K::value(out) * 0.5f);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i * 32 + lane < p.E && !((chosen >> ((i * 32 + lane) / p.group_size)) & 1)) key[i] = 0;
+  }
+  if (!BIAS) {                           // experts rank by their logits, exactly
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      key[i] = (x[i] > -INFINITY && (!GROUPS || key[i])) ? K::key((R)x[i]) : 0;
+  }
+  // Each lane keeps its DEPTH largest in order; a lane whose DEPTH have all been taken looks for the next
+  // ones below the last taken (rare: of 256 experts' 8 best, 3 share a lane in one row of twenty).
+  constexpr int DEPTH = VPL < 3 ? VPL : 3;
+  U top[DEPTH];
+  unsigned at[DEPTH];
+  auto refill = [&](U below, unsigned after) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) top[d] = 0, at[d] = ~0u;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const unsigned e = i * 32 + lane;
+      U v = key[i] < below || (key[i] == below && e > after) ? key[i] : 0;
+      unsigned w = e;
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {  // strictly larger goes first: equal ones stay in index order
+        const bool up = v > top[d];
+        const U tv = top[d];
+        const unsigned tw = at[d];
+        top[d] = up ? v : tv;
+        at[d] = up ? w : tw;
+        v = up ? tv : v;
+        w = up ? tw : w;
+      }
+    }
+  };
+  refill(~(U)0, ~0u);
+  int taken = 0;
+  id = -1;
+  U before = 0;
+  const int rounds = kScreen && BIAS ? p.k + 1 : p.k;   // the screen also looks at the first one left out
+  for (int j = 0; j < rounds; ++j) {
+    const U best = K::warp_max(top[0]);
+    if (best == 0) break;
+    if (kScreen && BIAS) {
+      if (j) near = near || too_near((float)K::value(before), (float)K::value(best));
+      before = best;
+    }
+    if (j == p.k) break;
+    const unsigned e = __reduce_min_sync(kAll, top[0] == best ? at[0] : ~0u);
+    if (lane == j) id = (int)e;
+    if (lane == (int)(e & 31)) {
+#pragma unroll
+      for (int d = 0; d + 1 < DEPTH; ++d) top[d] = top[d + 1], at[d] = at[d + 1];
+      top[DEPTH - 1] = 0;
+      if (VPL > DEPTH && ++taken == DEPTH) {
+        taken = 0;
+        refill(best, e);
+      }
+    }
+  }
+  if (kScreen && near) return true;
+  // weights: lane j fetches its expert's logit from the lane that holds it
+  float lx = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const float v = __shfl_sync(kAll, x[i], id & 31);
+    if (id >= 0 && (id >> 5) == i) lx = v;
+  }
+  R w = 0;
+  if (id >= 0) {
+    if (SOFTMAX) {
+      w = K::exponential((R)lx - m);
+      if (!p.renorm) w /= z;
+    } else {
+      w = score(lx);
+    }
+  }
+  if (p.renorm) {
+    const R total = warp_sum(w);
+    w = total > 0 ? w / total : (R)0;
+  }
+  weight = (float)(w * (R)p.scale);
+  return false;
+}
+
+template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
+__global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
+  float bias[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) bias[i] = BIAS && i * 32 + lane < p.E ? p.bias[i * 32 + lane] : 0.f;
+  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < p.T; t += warps) {
+    float x[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) x[i] = -INFINITY;
+    if (p.dtype == 0) {
+      const float* row = static_cast<const float*>(p.logits) + t * p.ld;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane < p.E) x[i] = row[i * 32 + lane];
+    } else if (p.dtype == 1) {
+      const __half* row = static_cast<const __half*>(p.logits) + t * p.ld;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane < p.E) x[i] = __half2float(row[i * 32 + lane]);
+    } else {
+      const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane < p.E) x[i] = __bfloat162float(row[i * 32 + lane]);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      x[i] = x[i] > -INFINITY ? fminf(x[i], FLT_MAX) : -INFINITY;       // NaN is off, +inf the largest float
+      if (BIAS && !(bias[i] > -INFINITY)) x[i] = -INFINITY;
+    }
+    int id;
+    float w;
+    if (route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w))
+      route_row<double, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w);
+    if (lane < p.k) {
+      p.ids[t * p.k + lane] = id;
+      p.weights[t * p.k + lane] = w;
+    }
+  }
+}
+
+template <int VPL>
+int launch_route(const RouteArgs& p, bool softmax, cudaStream_t stream) {
+  using Fn = void (*)(const RouteArgs);
+  const bool b = p.bias != nullptr, g = p.groups > 1;
+  static const Fn table[8] = {
+      route_kernel<VPL, false, false, false>, route_kernel<VPL, false, false, true>,
+      route_kernel<VPL, false, true, false>,  route_kernel<VPL, false, true, true>,
+      route_kernel<VPL, true, false, false>,  route_kernel<VPL, true, false, true>,
+      route_kernel<VPL, true, true, false>,   route_kernel<VPL, true, true, true>};
+  const int64_t ctas = std::min<int64_t>((p.T + 7) / 8, (int64_t)sm_count() * 8);
+  table[softmax * 4 + b * 2 + g]<<<(unsigned)ctas, 256, 0, stream>>>(p);
+  return check_launch("route_kernel");
+}
+
+}  // namespace
+}  // namespace nvfp4
+
+extern "C" int nvfp4_route_experts(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, const float* bias,
+                                   int score, int64_t k, int64_t groups, int64_t top_groups, int group_top,
+                                   int renorm, float scale, float* weights, int32_t* ids, void* stream) {
+  using namespace nvfp4;
+  if (T < 0 || E < 1 || E > kMaxExperts) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: need T >= 0 and 1..%d experts", kMaxExperts);
+  if (k < 1 || k > kMaxTopK || k > E) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: top_k must be 1..min(%d, experts)", kMaxTopK);
+  if (groups < 1 || groups > kMaxGroups || E % groups || top_groups < 1 || top_groups > groups)
+    return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: 1..%d groups that divide the experts, of which 1..groups may be used", kMaxGroups);
+  if (group_top < 1 || group_top > 2) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: a group's score sums its 1 or 2 best experts");
+  if (score < 0 || score > 1) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: unknown score function");
+  if (dtype < 0 || dtype > 2) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: logits must be float32, float16 or bfloat16");
+  if (ld < E && T > 1) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: row stride below the number of experts");
+  if (T == 0) return NVFP4_OK;
+  if (!logits || !weights || !ids) return fail(NVFP4_ERR_INVALID, "nvfp4_route_experts: null pointer");
+  const uintptr_t size = dtype == 0 ? 4 : 2;
+  if (reinterpret_cast<uintptr_t>(logits) % size || (reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(weights) |
+                                                     reinterpret_cast<uintptr_t>(ids)) % 4)
+    return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_route_experts: a pointer is not aligned to its element");
+  RouteArgs p;
+  p.logits = logits; p.bias = bias; p.weights = weights; p.ids = ids;
+  p.T = T; p.ld = ld;
+  p.E = (int)E; p.k = (int)k; p.groups = (int)groups; p.top_groups = (int)top_groups;
+  p.group_top = group_top; p.group_size = (int)(E / groups);
+  p.renorm = renorm; p.scale = scale;
+  p.dtype = dtype;
+  const bool softmax = score == 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int vpl = (p.E + 31) / 32;
+  if (vpl <= 1) return launch_route<1>(p, softmax, st);
+  if (vpl <= 2) return launch_route<2>(p, softmax, st);
+  if (vpl <= 4) return launch_route<4>(p, softmax, st);
+  if (vpl <= 8) return launch_route<8>(p, softmax, st);
+  if (vpl <= 16) return launch_route<16>(p, softmax, st);
+  return launch_route<32>(p, softmax, st);
+}

@@ -1,0 +1,97 @@
+"""The experts' SiLU-gated MLP on NVFP4 weights, for tokens that chose their experts.
+
+``moe_mlp(x, ids, weights, w_gate, w_up, w_down, scale_gate, scale_up, scale_down)`` returns fp16 ``[T, D]``:
+
+    out[t] = sum_j weights[t, j] * (nvfp4(silu(xq . w_gate[e]^T) * (xq . w_up[e]^T)) . w_down[e]^T),
+    e = ids[t, j],  xq = nvfp4(x[t])
+
+* ``x`` fp16 ``[T, D]``; ``ids`` int32 and ``weights`` float32 ``[T, k]``, as ``route_experts`` returns them.  A slot
+  with an id outside ``[0, E)`` is skipped; the same expert twice in a row counts twice.
+* codes ``[E, F, D/2]`` (gate, up: same strides, so halves of one merged tensor will do) and ``[E, D, F/2]`` (down);
+* scales per expert in the 128x4 blocked layout, ``[E, layout.blocked_numel(rows, K/16)]``, or plain ``[E, rows, K/16]``
+  (converted here, which costs extra launches).
+
+How many tokens an expert gets stays on the GPU: no synchronisation, and the call can be captured in a CUDA graph.  The
+workspace comes from torch's allocator, on the current stream.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .gemm import _FP4, _FP8
+from .layout import blocked_numel, to_blocked
+
+
+def _weights(name, w, E, N, K, dev):
+    if not isinstance(w, torch.Tensor) or w.dtype not in _FP4 or w.dim() != 3:
+        raise TypeError(f"{name} must be a 3-D uint8 / float4_e2m1fn_x2 tensor [E, rows, K/2]")
+    if tuple(w.shape) != (E, N, K // 2):
+        raise ValueError(f"{name} has shape {tuple(w.shape)}, expected {(E, N, K // 2)}")
+    if w.stride(2) != 1:
+        raise ValueError(f"{name} must be contiguous along K")
+    if w.device != dev:
+        raise ValueError(f"{name} must be on the device of x")
+    return w
+
+
+def _expert_scales(name, s, E, N, K, dev):
+    if not isinstance(s, torch.Tensor) or s.dtype not in _FP8:
+        raise TypeError(f"{name} must be a uint8 / float8_e4m3fn tensor")
+    if s.device != dev:
+        raise ValueError(f"{name} must be on the device of x")
+    if tuple(s.shape) == (E, N, K // 16):
+        return torch.stack([to_blocked(s[e]) for e in range(E)])
+    if tuple(s.shape) != (E, blocked_numel(N, K // 16)) or s.stride(1) != 1:
+        raise ValueError(f"{name}: expected plain [{E}, {N}, {K // 16}] or blocked [{E}, {blocked_numel(N, K // 16)}] "
+                         f"with contiguous bytes, got shape {tuple(s.shape)}")
+    return s
+
+
+def moe_mlp(x, ids, weights, w_gate, w_up, w_down, scale_gate, scale_up, scale_down, out=None):
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.float16 or x.dim() != 2:
+        raise TypeError("x must be a 2-D float16 tensor [T, D]")
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError("x must be a CUDA tensor")
+    T, D = x.shape
+    if x.stride(1) != 1:
+        raise ValueError("x must be contiguous along D")
+    if not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.dim() != 2:
+        raise TypeError("ids must be a 2-D int32 tensor [T, k]")
+    k = ids.shape[1]
+    if ids.shape[0] != T or not ids.is_contiguous() or ids.device != dev:
+        raise ValueError(f"ids must be contiguous [{T}, k] on the device of x, got {tuple(ids.shape)}")
+    if not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32:
+        raise TypeError("weights must be a float32 tensor [T, k]")
+    if weights.shape != ids.shape or not weights.is_contiguous() or weights.device != dev:
+        raise ValueError(f"weights must be contiguous {tuple(ids.shape)} on the device of x, got {tuple(weights.shape)}")
+    if not isinstance(w_gate, torch.Tensor) or w_gate.dim() != 3:
+        raise TypeError("w_gate must be a 3-D uint8 / float4_e2m1fn_x2 tensor [E, F, D/2]")
+    E, F = w_gate.shape[:2]
+    _weights("w_gate", w_gate, E, F, D, dev)
+    _weights("w_up", w_up, E, F, D, dev)
+    _weights("w_down", w_down, E, D, F, dev)
+    sg = _expert_scales("scale_gate", scale_gate, E, F, D, dev)
+    su = _expert_scales("scale_up", scale_up, E, F, D, dev)
+    sd = _expert_scales("scale_down", scale_down, E, D, F, dev)
+    if w_gate.stride() != w_up.stride() or sg.stride() != su.stride():
+        raise ValueError("w_gate and w_up, and their scales, must have the same strides")
+    if out is None:
+        out = torch.empty((T, D), dtype=torch.float16, device=dev)
+    elif not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or tuple(out.shape) != (T, D) \
+            or out.stride(1) != 1 or out.device != dev:
+        raise ValueError(f"out must be a float16 [{T}, {D}] tensor with unit column stride on the device of x")
+    l = _lib.lib()
+    need = ctypes.c_int64(0)
+    _lib.check(l.nvfp4_moe_workspace(T, k, E, D, F, ctypes.byref(need)))
+    with torch.cuda.device(dev):
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        _lib.check(l.nvfp4_moe_mlp(
+            x.data_ptr(), x.stride(0), ids.data_ptr(), weights.data_ptr(), T, k, E, D, F, w_gate.data_ptr(),
+            w_up.data_ptr(), sg.data_ptr(), su.data_ptr(), w_gate.stride(1), w_gate.stride(0), sg.stride(0),
+            w_down.data_ptr(), sd.data_ptr(), w_down.stride(1), w_down.stride(0), sd.stride(0), out.data_ptr(),
+            out.stride(0), ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    return out

@@ -1,0 +1,54 @@
+"""Routing of tokens to experts, for ``moe_mlp``.
+
+``route_experts(logits, top_k)`` returns ``(weights, ids)``: float32 and int32 ``[T, top_k]``, best first.  Per row x:
+
+* scores ``s = softmax(x)`` or, with ``score="sigmoid"``, ``1 / (1 + exp(-x))``;
+* choices ``c = s + bias`` (a bias that balances the experts' load changes who is chosen, not the weights);
+* with ``num_groups`` > 1 only the experts of the ``top_groups`` best groups stay, a group's score being the sum of its
+  ``group_top`` (1 or 2) largest choices;
+* the ``top_k`` largest choices, ties to the lowest index; weights are their s, divided by their sum
+  (``renormalize``), times ``scale``.
+
+An expert whose logit or bias is -inf or NaN is off; a slot that no expert fills gets id -1 and weight 0, and
+``moe_mlp`` skips it.  The ids are those of 64-bit arithmetic.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def route_experts(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = None, score: str = "softmax",
+                  num_groups: int = 1, top_groups: int = 1, group_top: int = 2, renormalize: bool = True,
+                  scale: float = 1.0, weights: torch.Tensor | None = None, ids: torch.Tensor | None = None):
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES or logits.dim() != 2:
+        raise TypeError("logits must be a 2-D float32, float16 or bfloat16 tensor [T, E]")
+    dev = logits.device
+    if dev.type != "cuda":
+        raise ValueError("logits must be a CUDA tensor")
+    T, E = logits.shape
+    if E > 1 and logits.stride(1) != 1:
+        raise ValueError("logits must be contiguous along the experts")
+    if score not in _SCORES:
+        raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
+    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape != (E,)
+                             or bias.device != dev or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 tensor [{E}] on the device of logits")
+    if weights is None:
+        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+    elif weights.dtype != torch.float32 or weights.shape != (T, top_k) or weights.device != dev or not weights.is_contiguous():
+        raise ValueError(f"weights must be a contiguous float32 tensor [{T}, {top_k}] on the device of logits")
+    if ids is None:
+        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+    elif ids.dtype != torch.int32 or ids.shape != (T, top_k) or ids.device != dev or not ids.is_contiguous():
+        raise ValueError(f"ids must be a contiguous int32 tensor [{T}, {top_k}] on the device of logits")
+    with torch.cuda.device(dev):
+        _lib.check(_lib.lib().nvfp4_route_experts(
+            logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), None if bias is None else bias.data_ptr(),
+            _SCORES[score], top_k, num_groups, top_groups, group_top, int(renormalize), scale, weights.data_ptr(),
+            ids.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+    return weights, ids

@@ -307,3 +307,148 @@ def quantize(x) -> tuple[np.ndarray, np.ndarray]:
     codes = np.where((s > 0)[:, :, None], codes, 0).astype(np.uint8).reshape(M, K)
     packed = (codes[:, 0::2] | (codes[:, 1::2] << 4)).astype(np.uint8)
     return packed, to_blocked_ref(sbyte)
+
+
+# ---------------------------------------------------------------------------
+# Routing of tokens to experts (no reference code; the contract is the formula).
+# ---------------------------------------------------------------------------
+
+def route(logits, k: int, bias=None, score: str = "softmax", groups: int = 1, top_groups: int = 1, group_top: int = 2,
+          renormalize: bool = True, scale: float = 1.0):
+    """Row by row in float64: (weights [T, k] float64, ids [T, k] int32).  An
+    expert with a logit or bias of -inf or NaN is off; +inf counts as the
+    largest float32; ties go to the lowest index; an empty slot is (0, -1)."""
+    x = logits.detach().float().cpu().numpy().astype(np.float64) if isinstance(logits, torch.Tensor) else np.asarray(logits, np.float64)
+    T, E = x.shape
+    b = np.zeros(E) if bias is None else (bias.detach().cpu().numpy() if isinstance(bias, torch.Tensor) else np.asarray(bias)).astype(np.float64)
+    weights, ids = np.zeros((T, k)), np.full((T, k), -1, np.int32)
+    size = E // groups
+    for t in range(T):
+        on = ~(np.isnan(x[t]) | np.isneginf(x[t]) | np.isnan(b) | np.isneginf(b))
+        if not on.any():
+            continue
+        v = np.where(on, np.minimum(np.where(on, x[t], 0.0), float(np.finfo(np.float32).max)), 0.0)
+        with np.errstate(over="ignore", under="ignore"):
+            if score == "softmax":
+                e = np.where(on, np.exp(v - v[on].max()), 0.0)
+                s = e / e.sum()
+            else:
+                s = np.where(on, 1.0 / (1.0 + np.exp(-v)), 0.0)
+        c = s + b
+        rank = c if bias is not None else v
+        if groups > 1:
+            gs = []
+            for g in range(groups):
+                members = sorted((c[i] for i in range(g * size, (g + 1) * size) if on[i]), reverse=True)[:group_top]
+                gs.append((-(sum(members)), g) if members else (np.inf, g))
+            best = {g for gscore, g in sorted(gs)[:top_groups]}
+            on = on & np.array([i // size in best for i in range(E)])
+        order = sorted((i for i in range(E) if on[i]), key=lambda i: (-rank[i], i))[:k]
+        w = s[order]
+        if renormalize:
+            w = w / w.sum() if w.sum() > 0 else np.zeros_like(w)
+        weights[t, :len(order)] = w * scale
+        ids[t, :len(order)] = order
+    return weights, ids
+
+
+# ---------------------------------------------------------------------------
+# The routed experts' MLP (no reference code; the contract is the formula).
+# ---------------------------------------------------------------------------
+
+def quantize_values(v):
+    """float64 [..., K] -> the values its NVFP4 quantisation stands for.  The
+    scale is e4m3(amax / 6); codes are e2m1(v * fl32(1/s)) with an f32 product."""
+    v = np.asarray(v, np.float64)
+    b = v.reshape(-1, 16)
+    with np.errstate(divide="ignore", over="ignore"):
+        sbyte = e4m3_rne_satfinite(np.abs(b).max(axis=1) / 6.0).astype(np.uint8)
+        s = E4M3_LUT[sbyte].astype(np.float64)[:, None]
+        inv = np.where(s > 0, (np.float32(1.0) / s.astype(np.float32)).astype(np.float64), 0.0)
+        q = (b.astype(np.float32) * inv.astype(np.float32)).astype(np.float64)
+    return (E2M1_LUT[e2m1_rne_satfinite(q)].astype(np.float64) * s).reshape(v.shape)
+
+
+def moe_mlp(x, ids, weights, w_gate, w_up, w_down, s_gate, s_up, s_down):
+    """float64 [T, D] from fp16 x [T, D], ids / weights [T, k], and per-expert
+    lists (or stacked arrays) of codes and blocked scales."""
+    x = x.detach().cpu().double().numpy()
+    ids = ids.detach().cpu().numpy()
+    weights = weights.detach().cpu().double().numpy()
+    T, D = x.shape
+    xq = quantize_values(x)
+    out = np.zeros((T, D))
+    for e in range(len(w_gate)):
+        F = w_gate[e].shape[0]
+        t, j = np.nonzero(ids == e)
+        if len(t) == 0:
+            continue
+        wg, wu = (dequant_matrix(w[e], s[e], F, D).astype(np.float64) for w, s in ((w_gate, s_gate), (w_up, s_up)))
+        wd = dequant_matrix(w_down[e], s_down[e], D, F).astype(np.float64)
+        g, u = xq[t] @ wg.T, xq[t] @ wu.T
+        with np.errstate(over="ignore"):
+            h = quantize_values(g / (1 + np.exp(-g)) * u)
+        np.add.at(out, t, (h @ wd.T) * weights[t, j][:, None])
+    return out
+
+
+def _quantize_within(v, dv):
+    """(values of v's quantisation, how far each may move when every element
+    of v is off by at most dv): the scale is that of a block whose largest
+    magnitude lies between max(|v| - dv) and max(|v| + dv), at most two
+    neighbouring e4m3 values, and rounding is monotone, so the extremes of each
+    element under each scale bound it."""
+    b, d = v.reshape(-1, 16), dv.reshape(-1, 16)
+
+    def under(s, w):
+        inv = np.where(s > 0, (np.float32(1.0) / np.where(s > 0, s, 1).astype(np.float32)).astype(np.float64), 0.0)
+        return E2M1_LUT[e2m1_rne_satfinite(w * inv)].astype(np.float64) * s
+
+    def scale(a):
+        return E4M3_LUT[e4m3_rne_satfinite(a / 6.0)].astype(np.float64)[:, None]
+
+    a = np.abs(b)
+    base = under(scale(a.max(axis=1)), b)
+    far = np.zeros_like(base)
+    lo, hi = scale(np.maximum(a - d, 0).max(axis=1)), scale((a + d).max(axis=1))
+    for s in (lo, hi, scale(a.max(axis=1))):
+        for w in (b - d, b + d):
+            far = np.maximum(far, np.abs(under(s, w) - base))
+    return base.reshape(v.shape), far.reshape(v.shape)
+
+
+def moe_mlp_bounds(x, ids, weights, w_gate, w_up, w_down, s_gate, s_up, s_down):
+    """(out, tolerance) of ``moe_mlp`` for an implementation that accumulates in
+    fp32.  A sum over K products made of K/64 partial sums is off by at most
+    2 (K/64 + 8) units of 2^-24 of the sum of magnitudes (each addition rounds
+    or truncates once; 8 for the sum inside a 64-element step); silu(g) * u by
+    2^-18 relative (exponential (2 + 1.2 |g|) 2^-23, quotient and product 2^-22,
+    |g| < 20).  What that lets h's codes move, times |Wd|, is carried through;
+    the sum over slots adds k roundings, the result one to fp16."""
+    x = x.detach().cpu().double().numpy()
+    ids = ids.detach().cpu().numpy()
+    weights = weights.detach().cpu().double().numpy()
+    T, D = x.shape
+    k = ids.shape[1]
+    xq = quantize_values(x)
+    out, tol, mag = np.zeros((T, D)), np.zeros((T, D)), np.zeros((T, D))
+    for e in range(len(w_gate)):
+        F = w_gate[e].shape[0]
+        t, j = np.nonzero(ids == e)
+        if len(t) == 0:
+            continue
+        wg, wu = (dequant_matrix(w[e], s[e], F, D).astype(np.float64) for w, s in ((w_gate, s_gate), (w_up, s_up)))
+        wd = dequant_matrix(w_down[e], s_down[e], D, F).astype(np.float64)
+        g, u = xq[t] @ wg.T, xq[t] @ wu.T
+        unit = 2 * (D / 64 + 8) * 2.0 ** -24
+        eg, eu = unit * (np.abs(xq[t]) @ np.abs(wg).T), unit * (np.abs(xq[t]) @ np.abs(wu).T)
+        sg = g / (1 + np.exp(-g))
+        h = sg * u
+        dh = 1.1 * eg * (np.abs(u) + eu) + np.abs(sg) * eu + 2.0 ** -18 * np.abs(h) + 2.0 ** -126
+        hq, far = _quantize_within(h, dh)
+        w = weights[t, j][:, None]
+        m = np.abs(hq) @ np.abs(wd).T
+        np.add.at(out, t, (hq @ wd.T) * w)
+        np.add.at(tol, t, (far @ np.abs(wd).T + 2 * (F / 64 + 8) * 2.0 ** -24 * (m + far @ np.abs(wd).T)) * np.abs(w))
+        np.add.at(mag, t, m * np.abs(w))
+    return out, tol + (k + 1) * 2.0 ** -24 * mag + (np.abs(out) + tol) * 2.0 ** -11 + 2.0 ** -24

@@ -1,0 +1,179 @@
+"""Routing of tokens to experts: refusals on the CPU, and the GPU kernel against
+the float64 oracle (ids equal, weights within 32-bit rounding).
+
+Weights tolerance: with logits within 32 of the row's maximum an exponential is
+off by at most (32 + 2) * 2^-24 (argument rounding and the function itself), a
+sum of up to 1024 terms adds at most 37 roundings, the quotients and the scale
+four more on each side: (34 + 37 + 8) * 2^-24 < 6e-6."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+RTOL, ATOL = 6e-6, 1e-37
+
+
+def _check(pkg, oracle, logits, k, bias=None, **kw):
+    w, ids = pkg.route_experts(logits, k, bias=bias, **{"num_groups": kw.get("groups", 1), **{a: b for a, b in kw.items() if a != "groups"}})
+    torch.cuda.synchronize()
+    rw, ri = oracle.route(logits, k, bias, **kw)
+    np.testing.assert_array_equal(ids.cpu().numpy(), ri)
+    np.testing.assert_allclose(w.cpu().numpy().astype(np.float64), rw, rtol=RTOL, atol=ATOL)
+    return w, ids
+
+
+# ------------------------------------------------------------------- CPU
+
+def test_oracle_route_by_hand(oracle):
+    x = np.array([[0.0, math.log(3.0), -np.inf, math.log(2.0)]])
+    w, ids = oracle.route(x, 2)
+    assert ids.tolist() == [[1, 3]]
+    np.testing.assert_allclose(w, [[0.6, 0.4]])
+    w, ids = oracle.route(x, 4, renormalize=False, scale=2.0)
+    assert ids.tolist() == [[1, 3, 0, -1]]
+    np.testing.assert_allclose(w, [[1.0, 2 / 3, 1 / 3, 0.0]])
+    # groups {0,1} and {2,3}: sums 1/2 + 3/4 against 2/3 + nothing
+    w, ids = oracle.route(x, 2, score="sigmoid", groups=2, top_groups=1)
+    assert ids.tolist() == [[1, 0]]
+    np.testing.assert_allclose(w, [[0.6, 0.4]])
+
+
+def test_route_refuses_without_gpu(pkg):
+    l, p = pkg._lib.lib(), 4096
+    call = lambda T=4, E=8, ld=8, score=0, k=2, g=1, tg=1, gt=2, dt=0, x=p, w=p: l.nvfp4_route_experts(
+        x, dt, T, E, ld, None, score, k, g, tg, gt, 1, 1.0, w, p, None)
+    assert call(E=0) == 1 and call(E=1025, ld=1025) == 1
+    assert call(k=0) == 1 and call(k=9) == 1 and call(E=64, ld=64, k=33) == 1
+    assert call(g=3) == 1 and call(tg=2) == 1 and call(tg=0) == 1 and call(E=64, ld=64, g=64) == 1
+    assert call(gt=3) == 1 and call(gt=0) == 1 and call(score=2) == 1 and call(dt=3) == 1 and call(ld=7) == 1
+    assert call(x=None) == 1 and b"null" in l.nvfp4_last_error()
+    assert call(x=p + 2) == 2 and call(w=p + 2) == 2
+    assert call(T=0, x=None) == 0
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.route_experts(torch.zeros(2, 8), 2)
+    with pytest.raises(TypeError):
+        pkg.route_experts(torch.zeros(2, 8, dtype=torch.float64), 2)
+
+
+# ------------------------------------------------------------------- GPU
+
+CASES = [
+    (1, 8, 2, {}), (3, 1, 1, {}), (5, 2, 2, {}), (257, 7, 3, {}), (33, 32, 32, {}), (64, 60, 4, {}),
+    (40, 128, 8, dict(renormalize=False, scale=1.7)), (20, 1000, 8, {}), (9, 1024, 32, dict(renormalize=False)),
+    (64, 256, 8, dict(groups=8, top_groups=4)), (31, 256, 8, dict(groups=8, top_groups=4, group_top=1)),
+    (50, 60, 4, dict(groups=4, top_groups=2)), (50, 96, 6, dict(groups=32, top_groups=5)),
+    (50, 64, 8, dict(groups=32, top_groups=4)), (17, 512, 9, dict(groups=2, top_groups=2)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,kw", CASES)
+def test_route(pkg, oracle, cuda, T, E, k, kw, dtype, with_bias, score):
+    g = torch.Generator().manual_seed(T * 1000 + E)
+    x = (torch.randn((T, E), generator=g) * 2).to(dtype).to(cuda)
+    bias = (torch.randn(E, generator=g) * 0.1).to(cuda) if with_bias else None
+    _check(pkg, oracle, x, k, bias, score=score, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_route_masked_and_special_values(pkg, oracle, cuda, groups, with_bias, score):
+    """Rows whose mask leaves nothing or fewer than k, NaN, infinities, the
+    type's lowest value, signed zeros, rows of equal logits."""
+    E, k = 16, 5
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn((12, E), generator=g)
+    low = torch.finfo(torch.float32).min
+    x[0] = -math.inf
+    x[1] = math.nan
+    x[2] = low
+    x[3, 3:] = -math.inf
+    x[4, ::2] = math.nan
+    x[5, 7] = math.inf
+    x[5, 2] = math.inf
+    x[6] = 0.0
+    x[6, 1::2] = -0.0
+    x[7] = 1.25
+    x[8, 4:] = low
+    x[9, :8] = -math.inf
+    x[10, :13] = -math.inf
+    x[11] = x[11] * 30
+    bias = None
+    if with_bias:
+        bias = torch.randn(E, generator=g) * 0.1
+        bias[1], bias[6], bias[9], bias[12] = -math.inf, math.nan, 0.5, 0.5
+        bias = bias.to(cuda)
+    _check(pkg, oracle, x.to(cuda), k, bias, score=score, groups=groups, top_groups=max(1, groups // 2))
+
+
+@pytest.mark.gpu
+def test_route_infinite_bias_ranks_first(pkg, oracle, cuda):
+    x = torch.randn((6, 8), generator=torch.Generator().manual_seed(4)).to(cuda)
+    bias = torch.zeros(8)
+    bias[3] = bias[5] = math.inf
+    w, ids = _check(pkg, oracle, x, 3, bias.to(cuda), score="sigmoid")
+    assert (ids[:, 0] == 3).all() and (ids[:, 1] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("gap", [0.0, 1e-8, 1e-6, 1e-5])
+def test_route_near_ties_are_ranked_in_64_bits(pkg, oracle, cuda, gap, score):
+    """Choices that differ by less than 32-bit arithmetic can tell: the bias
+    makes every expert's choice the same up to `gap` and the bias's rounding."""
+    E, T = 64, 50
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(E, generator=g)
+    s = torch.softmax(x.double(), 0) if score == "softmax" else torch.sigmoid(x.double())
+    bias = (0.75 - s + gap * torch.rand(E, generator=g)).float()
+    _check(pkg, oracle, x.repeat(T, 1).to(cuda), 8, bias.to(cuda), score=score, groups=4, top_groups=2)
+    _check(pkg, oracle, x.repeat(T, 1).to(cuda), 8, bias.to(cuda), score=score)
+
+
+@pytest.mark.gpu
+def test_route_strided_rows_other_stream_and_outputs(pkg, oracle, cuda):
+    g = torch.Generator().manual_seed(6)
+    big = torch.randn((40, 77), generator=g).to(cuda)
+    x = big[:, 3:67]
+    w = torch.full((42, 4), 7.0, device=cuda)
+    ids = torch.full((42, 4), 7, dtype=torch.int32, device=cuda)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        pkg.route_experts(x, 4, weights=w[1:41], ids=ids[1:41])
+    torch.cuda.synchronize()
+    rw, ri = oracle.route(x, 4)
+    np.testing.assert_array_equal(ids[1:41].cpu().numpy(), ri)
+    np.testing.assert_allclose(w[1:41].cpu().numpy(), rw, rtol=RTOL, atol=ATOL)
+    assert (w[[0, 41]] == 7).all() and (ids[[0, 41]] == 7).all()     # rows around stay as they were
+
+
+@pytest.mark.gpu
+def test_route_no_tokens_and_many(pkg, oracle, cuda):
+    w, ids = pkg.route_experts(torch.empty((0, 8), device=cuda), 2)
+    assert w.shape == (0, 2) and ids.shape == (0, 2)
+    x = torch.randn((20000, 16), generator=torch.Generator().manual_seed(7)).to(cuda)
+    _check(pkg, oracle, x, 2)
+
+
+@pytest.mark.gpu
+def test_route_refusals(pkg, cuda):
+    x = torch.zeros((4, 8), device=cuda)
+    with pytest.raises(RuntimeError, match="top_k"):
+        pkg.route_experts(x, 9)
+    with pytest.raises(RuntimeError, match="groups"):
+        pkg.route_experts(x, 2, num_groups=3)
+    with pytest.raises(ValueError, match="score"):
+        pkg.route_experts(x, 2, score="relu")
+    with pytest.raises(ValueError, match="bias"):
+        pkg.route_experts(x, 2, bias=torch.zeros(7, device=cuda))
+    with pytest.raises(ValueError, match="contiguous"):
+        pkg.route_experts(torch.zeros((8, 4), device=cuda).t(), 2)
+    with pytest.raises(ValueError, match="ids"):
+        pkg.route_experts(x, 2, ids=torch.zeros((4, 2), dtype=torch.int64, device=cuda))
