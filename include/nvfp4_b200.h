@@ -278,6 +278,30 @@ NVFP4_API int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, cons
                             int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * Low-rank adapters of many requests, added to a shared projection's output:
+ *   out[t] = fp16( base[t] + scales[i] * ((x[t] . A_i^T) . B_i^T) ),  i = adapters[t]
+ * in fp32 (the inner product enters the outer one with at least 22 bits), one
+ * rounding at the end.  A token whose index is not in [0, n) keeps base.
+ *   base, out [T, N] fp16 (row strides ld_base, ldo elements; out may be base
+ *   (in place); otherwise it overlaps neither base nor x);
+ *   x [T, K] fp16; a: n matrices [r, K], b: n matrices [N, r], fp16, with row
+ *   strides lda, ldb and matrix strides a_stride, b_stride in elements, all
+ *   multiples of 8, and 16-byte aligned pointers; adapters int32 [T];
+ *   scales float32 [n] or NULL (1); ranks int32 [n] or NULL: adapter i uses its
+ *   first ranks[i] rows of A and columns of B (clamped to 0..r), the others may
+ *   hold anything.
+ * r is a multiple of 16 up to 128, K of 8; N is any; n <= 1023; T may be 0.
+ * `workspace`: device memory of at least nvfp4_lora_workspace() bytes (0 for few
+ * tokens), 256-byte aligned, in use until the call's work on `stream` ends.
+ * No counterpart in the reference.
+ */
+NVFP4_API int nvfp4_lora_workspace(int64_t T, int64_t r, int64_t n, int64_t* bytes);
+NVFP4_API int nvfp4_lora_add(const void* base, int64_t ld_base, const void* x, int64_t ldx, const void* a, int64_t lda,
+                             int64_t a_stride, const void* b, int64_t ldb, int64_t b_stride, const int32_t* adapters,
+                             const float* scales, const int32_t* ranks, int64_t T, int64_t K, int64_t N, int64_t r,
+                             int64_t n, void* out, int64_t ldo, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Tensor-core peak probe: one CTA per SM issues `iters` dense 128x256x64
  * kind::mxf4nvf4 MMAs (4,194,304 FLOP each) from shared memory.  Time it with
  * events on `stream` to get the device's FP4 tensor throughput, the

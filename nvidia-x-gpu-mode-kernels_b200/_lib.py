@@ -44,6 +44,9 @@ SIGNATURES: dict[str, list] = {
     "nvfp4_moe_workspace": [I64, I64, I64, I64, I64, ctypes.POINTER(I64)],
     "nvfp4_moe_mlp": [VP, I64, VP, VP, I64, I64, I64, I64, I64, VP, VP, VP, VP, I64, I64, I64, VP, VP, I64, I64, I64,
                       VP, I64, VP, I64, VP],
+    "nvfp4_lora_workspace": [I64, I64, I64, ctypes.POINTER(I64)],
+    "nvfp4_lora_add": [VP, I64, VP, I64, VP, I64, I64, VP, I64, I64, VP, VP, VP, I64, I64, I64, I64, I64, VP, I64,
+                       VP, I64, VP],
     "nvfp4_gemv_grid": [I64, I64, I64, ctypes.POINTER(I64)],
     "nvfp4_set_peer_wait_ns": [ctypes.c_uint64],
     "nvfp4_gemv_allgather": [VP, VP, VP, VP, I64, I64, I64, I64, I64, I64, I64, I64, I64,

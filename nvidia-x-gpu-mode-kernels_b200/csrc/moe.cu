@@ -166,25 +166,6 @@ int token_maps(ExpertParams& P, const void* codes, const void* sf, int64_t rows,
   return encode_tmap(&P.tst, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, sf, sdims, sstr, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
-// Launches a kernel that may start while its predecessor in the stream drains
-// (it waits with griddep_wait before touching the predecessor's memory).
-template <typename... Args>
-int launch_after(void (*kern)(Args...), const char* name, unsigned grid, unsigned block, size_t smem,
-                 cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(block);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
-  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, name);
-}
-
 struct MoeCall {
   const void *wg, *wu, *wd, *sg, *su, *sd;
   int64_t E, D, F;
@@ -287,7 +268,7 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
   int* const rows = reinterpret_cast<int*>(c.ws + m.row);
   const Plan plan = {reinterpret_cast<int*>(c.ws), reinterpret_cast<PlanTile*>(c.ws + m.tiles), rows, nullptr};
-  if ((rc = launch_plan(ids, T * k, E, m.tile, m.tile, plan, c.stream))) return rc;
+  if ((rc = launch_plan(ids, T * k, E, -1, m.tile, m.tile, plan, c.stream))) return rc;
   const int threads = (int)std::min<int64_t>(256, (D / 16 + 31) / 32 * 32);
   if ((rc = launch_after(scatter_quantize_kernel, "scatter_quantize_kernel",
                          (unsigned)std::min<int64_t>(T, (int64_t)sm_count() * 8), threads, 0, c.stream,

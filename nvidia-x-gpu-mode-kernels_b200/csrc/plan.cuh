@@ -3,6 +3,9 @@
 // index's rows starting at a multiple of `align`, and the row tiles to walk
 // are listed.  Everything stays on the GPU: the host never learns the counts.
 //
+// A slot whose index is not in [0, indexes) goes to the index `other`, or is
+// left out where `other` is negative.
+//
 // One cluster of C CTAs: each counts its share of the slots in shared memory
 // (an atomic gives a slot its place among its share's equals), the counts are
 // exchanged through distributed shared memory, every CTA scans them, and the
@@ -57,7 +60,7 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
 
 template <int C>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __restrict__ ids, int n, int indexes,
-                                                            int align, int tile, Plan p) {
+                                                            int other, int align, int tile, Plan p) {
   __shared__ uint32_t hist[kPlanMaxIndexes];
   __shared__ int start[kPlanMaxIndexes];
   __shared__ int warp_rows[32], warp_tiles[32];
@@ -69,8 +72,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   const int share = (n + C - 1) / C;
   const int lo = me * share, hi = min(n, lo + share);
   for (int s = lo + tid; s < hi; s += kPlanThreads) {
-    const int e = ids[s];
-    p.row[s] = (unsigned)e < (unsigned)indexes ? (int)atomicAdd(&hist[e], 1u) : -1;
+    int e = ids[s];
+    if ((unsigned)e >= (unsigned)indexes) e = other;
+    p.row[s] = e >= 0 ? (int)atomicAdd(&hist[e], 1u) : -1;
   }
   if (C > 1) cluster_sync();
   else __syncthreads();
@@ -123,17 +127,18 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const int32_t* __res
   __syncthreads();
   for (int s = lo + tid; s < hi; s += kPlanThreads) {
     if (p.row[s] < 0) continue;                  // written by this thread above
-    const int at = p.row[s] + start[ids[s]];
+    const int e = ids[s];
+    const int at = p.row[s] + start[(unsigned)e < (unsigned)indexes ? e : other];
     p.row[s] = at;
     if (p.slot) p.slot[at] = s;
   }
   if (C > 1) cluster_sync();                     // the others have read this CTA's counts
 }
 
-inline int launch_plan(const int32_t* ids, int64_t n, int64_t indexes, int align, int tile, const Plan& p,
+inline int launch_plan(const int32_t* ids, int64_t n, int64_t indexes, int other, int align, int tile, const Plan& p,
                        cudaStream_t stream) {
   if (n <= 4096) {
-    plan_kernel<1><<<1, kPlanThreads, 0, stream>>>(ids, (int)n, (int)indexes, align, tile, p);
+    plan_kernel<1><<<1, kPlanThreads, 0, stream>>>(ids, (int)n, (int)indexes, other, align, tile, p);
     return check_launch("plan_kernel");
   }
   cudaLaunchConfig_t cfg = {};
@@ -147,8 +152,27 @@ inline int launch_plan(const int32_t* ids, int64_t n, int64_t indexes, int align
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, plan_kernel<8>, ids, (int)n, (int)indexes, align, tile, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, plan_kernel<8>, ids, (int)n, (int)indexes, other, align, tile, p);
   return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaLaunchKernelEx(plan)");
+}
+
+// Launches a kernel that may start while its predecessor in the stream drains
+// (it waits with griddep_wait before touching the predecessor's memory).
+template <typename... Args>
+int launch_after(void (*kern)(Args...), const char* name, unsigned grid, unsigned block, size_t smem,
+                 cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, name);
 }
 
 }  // namespace

@@ -1,0 +1,73 @@
+"""Low-rank adapters of many requests beside a shared projection.
+
+``lora_add(base, x, a, b, adapters)`` adds to ``base``, what ``skinny_gemm`` / ``grouped_gemm`` wrote for the shared
+weights, each token's own low-rank term, from the activations before their quantisation:
+
+    out[t] = base[t] + scales[i] * ((x[t] . a[i]^T) . b[i]^T),   i = adapters[t]
+
+* ``base`` fp16 ``[T, N]``, ``x`` fp16 ``[T, K]``, ``a`` fp16 ``[n, r, K]``, ``b`` fp16 ``[n, N, r]``: ``r`` is the
+  largest rank, padded to a multiple of 16 (up to 128); ``ranks`` int32 ``[n]`` says how much of it each adapter uses,
+  what lies beyond may hold anything;
+* ``adapters`` int32 ``[T]`` on the GPU: an index outside ``[0, n)``, such as -1, is a token without an adapter;
+* ``out`` is ``base`` (in place) unless given; it may not overlap ``x``.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+
+def _half(name, t, dim, dev):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float16 or t.dim() != dim:
+        raise TypeError(f"{name} must be a {dim}-D float16 tensor")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on the device of base")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name} must be contiguous along its last dimension")
+
+
+def _vector(name, t, n, dtype, dev):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != (n,):
+        raise ValueError(f"{name} must be a {dtype} tensor [{n}]")
+    if t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous on the device of base")
+    return t.data_ptr()
+
+
+def lora_add(base, x, a, b, adapters, scales=None, ranks=None, out=None):
+    if not isinstance(base, torch.Tensor):
+        raise TypeError("base must be a 2-D float16 tensor")
+    dev = base.device
+    if dev.type != "cuda":
+        raise ValueError("base must be a CUDA tensor")
+    _half("base", base, 2, dev)
+    _half("x", x, 2, dev)
+    _half("a", a, 3, dev)
+    _half("b", b, 3, dev)
+    (T, N), K, (n, r) = base.shape, x.shape[1], a.shape[:2]
+    if x.shape[0] != T:
+        raise ValueError(f"x has {x.shape[0]} rows, expected {T}")
+    if a.shape[2] != K or tuple(b.shape) != (n, N, r):
+        raise ValueError(f"a {tuple(a.shape)} and b {tuple(b.shape)} do not fit [n, r, {K}] and [n, {N}, r]")
+    if out is None:
+        out = base
+    else:
+        _half("out", out, 2, dev)
+        if out.shape != base.shape:
+            raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(base.shape)}")
+    ad = _vector("adapters", adapters, T, torch.int32, dev)
+    sc = None if scales is None else _vector("scales", scales, n, torch.float32, dev)
+    rk = None if ranks is None else _vector("ranks", ranks, n, torch.int32, dev)
+    l = _lib.lib()
+    need = ctypes.c_int64(0)
+    _lib.check(l.nvfp4_lora_workspace(T, r, n, ctypes.byref(need)))
+    with torch.cuda.device(dev):
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        _lib.check(l.nvfp4_lora_add(
+            base.data_ptr(), base.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), a.stride(1), a.stride(0),
+            b.data_ptr(), b.stride(1), b.stride(0), ad, sc, rk, T, K, N, r, n, out.data_ptr(), out.stride(0),
+            None if ws is None else ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    return out

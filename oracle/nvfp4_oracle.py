@@ -452,3 +452,32 @@ def moe_mlp_bounds(x, ids, weights, w_gate, w_up, w_down, s_gate, s_up, s_down):
         np.add.at(tol, t, (far @ np.abs(wd).T + 2 * (F / 64 + 8) * 2.0 ** -24 * (m + far @ np.abs(wd).T)) * np.abs(w))
         np.add.at(mag, t, m * np.abs(w))
     return out, tol + (k + 1) * 2.0 ** -24 * mag + (np.abs(out) + tol) * 2.0 ** -11 + 2.0 ** -24
+
+
+# ---------------------------------------------------------------------------
+# Low-rank adapters (no reference code; the contract is the formula).
+# ---------------------------------------------------------------------------
+
+def lora_add(base, x, a, b, adapters, scales=None, ranks=None):
+    """(out, tolerance) in float64.  Tolerance of an implementation in fp32: u's
+    sum over K and the sum over r are off by at most their number of terms (in
+    mma steps of 16, each adding 16 products and rounding or truncating at most
+    twice, plus 24 joined partial sums) times 2^-23 of their magnitudes, u's two
+    halves by 2^-21, and the result is rounded to fp16 once."""
+    base, x, a, b = (t.detach().cpu().double().numpy() for t in (base, x, a, b))
+    ids = adapters.detach().cpu().numpy()
+    n, r, K = a.shape
+    out, tol = base.copy(), np.zeros_like(base)
+    for t in range(len(ids)):
+        i = ids[t]
+        if not 0 <= i < n:
+            continue
+        rank = r if ranks is None else max(0, min(r, int(ranks[i])))
+        s = 1.0 if scales is None else float(scales[i])
+        u = a[i, :rank] @ x[t]
+        ua = np.abs(a[i, :rank]) @ np.abs(x[t])
+        bi = b[i, :, :rank]
+        out[t] += s * (bi @ u)
+        eu = (K / 16 + 24) * 2.0 ** -23 * ua + 2.0 ** -21 * (np.abs(u).max() if rank else 0.0)
+        tol[t] = abs(s) * (np.abs(bi) @ (eu + (2 * r / 16 + 8) * 2.0 ** -23 * np.abs(u)))
+    return out, tol + (np.abs(out) + tol) * 2.0 ** -11 + 2.0 ** -24

@@ -1,0 +1,228 @@
+"""Low-rank adapters: refusals on the CPU, the GPU kernels against the float64
+oracle with its derived element-wise tolerance (fp32 sums, one rounding)."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+
+class Problem:
+    def __init__(self, T, K, N, r, n, run=1, mixed=True, seed=0):
+        g = torch.Generator().manual_seed(seed + T + K + N + r)
+        h = lambda *s: torch.randn(s, generator=g).to(torch.float16)
+        self.x, self.base = h(T, K), h(T, N)
+        self.a = (h(n, r, K).float() / K ** 0.5).to(torch.float16)
+        self.b = (h(n, N, r).float() / r ** 0.5).to(torch.float16)
+        owner = torch.randint(-1, n, (-(-max(T, 1) // run),), generator=g)
+        self.adapters = owner.repeat_interleave(run)[:T].to(torch.int32).contiguous()
+        self.scales = torch.rand(n, generator=g) + 0.5 if mixed else None
+        self.ranks = torch.randint(0, r + 1, (n,), generator=g).to(torch.int32) if mixed else None
+        if mixed:
+            self.ranks[0] = r
+            for i in range(n):      # what lies beyond a rank may hold anything
+                self.a[i, self.ranks[i]:] = float("nan")
+                self.b[i, :, self.ranks[i]:] = float("inf")
+
+    def args(self, dev="cuda"):
+        mv = lambda t: None if t is None else t.to(dev)
+        return [mv(t) for t in (self.base, self.x, self.a, self.b, self.adapters, self.scales, self.ranks)]
+
+    def check(self, oracle, got):
+        want, tol = oracle.lora_add(self.base, self.x, self.a, self.b, self.adapters, self.scales, self.ranks)
+        err = np.abs(got.cpu().double().numpy() - want)
+        assert (err <= tol).all(), f"off by {err.max()}, {(~(err <= tol)).sum()} elements"
+
+
+# ------------------------------------------------------------------- CPU
+
+def test_oracle_lora_by_hand(oracle):
+    t = lambda *v: torch.tensor(v, dtype=torch.float64)
+    a = t(1, 2, 3, 4).view(1, 2, 2)
+    b = t(1, 0, 0, 1, 1, 1).view(1, 3, 2)
+    out, _ = oracle.lora_add(t(1, 1, 1).view(1, 3), t(1, -1).view(1, 2), a, b, torch.tensor([0]), t(2))
+    assert out.tolist() == [[1 - 2, 1 - 2, 1 - 4]]
+    out, _ = oracle.lora_add(t(1, 1, 1).view(1, 3), t(1, -1).view(1, 2), a, b, torch.tensor([0]), None, torch.tensor([1]))
+    assert out.tolist() == [[0, 1, 0]]
+
+
+def test_lora_refuses_without_gpu(pkg):
+    l, p = pkg._lib.lib(), 4096
+    need = ctypes.c_int64(-1)
+    ws = lambda *a: l.nvfp4_lora_workspace(*a, ctypes.byref(need))
+    assert ws(1, 16, 4) == 0 and need.value == 0
+    assert ws(5000, 64, 4) == 0 and need.value > 0
+    assert ws(-1, 16, 4) == 1 and ws(4, 8, 4) == 1 and ws(4, 24, 4) == 1 and ws(4, 144, 4) == 1
+    assert ws(4, 16, 0) == 1 and ws(4, 16, 1024) == 1 and b"adapters" in l.nvfp4_last_error()
+
+    def call(base=p, ldb=16, x=p, ldx=64, lda=64, sa=1024, T=4, K=64, r=16, n=2, out=p, ldo=100, N=100, ldbase=100,
+             w=None, wb=0, ad=p):
+        return l.nvfp4_lora_add(base, ldbase, x, ldx, p, lda, sa, p, ldb, 1600, ad, None, None, T, K, N, r, n, out, ldo,
+                                w, wb, None)
+    assert call(base=None) == 1 and call(x=None) == 1 and call(out=None) == 1
+    assert call(K=60) == 1 and call(N=0) == 1 and call(K=0) == 1
+    assert call(ldx=56) == 1 and call(ldo=99, out=p + 2) == 1 and call(ldbase=99, out=p + 2) == 1 and call(lda=32) == 1
+    assert call(sa=-8) == 1 and call(ldb=8) == 1
+    assert call(x=p + 8) == 2 and call(ldx=68) == 2 and call(sa=1028) == 2 and call(base=p + 1, out=p) == 2
+    assert call(ad=p + 2) == 2
+    assert call(ldo=104) == 1 and b"stride" in l.nvfp4_last_error()          # in place with another row stride
+    assert call(T=5000) == 1 and b"workspace" in l.nvfp4_last_error()
+    assert call(T=5000, w=p, wb=64) == 1
+    assert call(T=0, base=None) == 0
+
+
+# ------------------------------------------------------------------- GPU
+
+SHAPES = [
+    (1, 64, 64, 16, 1, 1), (1, 4096, 1000, 16, 3, 1), (2, 8, 1, 16, 2, 1), (7, 72, 33, 32, 3, 1), (64, 512, 768, 64, 9, 1),
+    (40, 256, 520, 128, 2, 1), (128, 1000, 333, 48, 40, 3), (100, 136, 64, 96, 1, 100),
+    (129, 64, 64, 16, 2, 10), (200, 72, 1, 16, 3, 1), (777, 1000, 203, 48, 9, 37), (300, 520, 264, 128, 5, 20),
+    (500, 128, 520, 64, 1, 500), (1000, 8, 96, 32, 300, 1), (5000, 64, 40, 112, 7, 90),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("T,K,N,r,n,run", SHAPES)
+def test_lora(pkg, oracle, cuda, T, K, N, r, n, run, in_place):
+    p = Problem(T, K, N, r, n, run)
+    a = p.args()
+    out = None if in_place else torch.full((T, N), float("nan"), dtype=torch.float16, device=cuda)
+    got = pkg.lora_add(*a, out=out)
+    torch.cuda.synchronize()
+    assert got is (a[0] if in_place else out)
+    p.check(oracle, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 300])
+def test_lora_without_scales_and_ranks(pkg, oracle, cuda, T):
+    p = Problem(T, 128, 96, 32, 4, mixed=False)
+    p.check(oracle, pkg.lora_add(*p.args()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [0, 6, 400])
+def test_lora_no_tokens_or_no_adapters(pkg, cuda, T):
+    p = Problem(T, 64, 72, 16, 2)
+    p.adapters[:] = -1
+    p.adapters[1::2] = 2          # outside [0, n) as well
+    a = p.args()
+    out = torch.full_like(a[0], float("nan"))
+    pkg.lora_add(*a, out=out)
+    assert torch.equal(out, a[0])
+    pkg.lora_add(*a)
+    assert torch.equal(a[0].cpu(), p.base)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [24, 400])
+def test_lora_strides_and_what_lies_around(pkg, oracle, cuda, T):
+    """Row and matrix strides, odd output rows, negative ranks (none used),
+    ranks beyond r, dirty memory from the allocator."""
+    K, N, r, n = 200, 136, 32, 3
+    p = Problem(T, K, N, r, n, run=5)
+    p.ranks = torch.tensor([32, -3, 99], dtype=torch.int32)
+    g = torch.Generator().manual_seed(2)
+    p.a = torch.randn((n, r, K), generator=g).div(14).to(torch.float16)
+    p.b = torch.randn((n, N, r), generator=g).div(6).to(torch.float16)
+    nan = lambda *s: torch.full(s, float("nan"), dtype=torch.float16, device=cuda)
+    base, x, a, b, ad, sc, rk = p.args()
+    bigx, biga, bigb, bigo = nan(T, K + 24), nan(n + 1, r + 2, K + 8), nan(n, N + 1, r + 16), nan(T + 2, N + 3)
+    bigx[:, 8:8 + K], biga[:n, :r, :K], bigb[:, :N, 8:8 + r], bigo[1:T + 1, 1:1 + N] = x, a, b, base
+    bigo[[0, T + 1]] = 5
+    need = ctypes.c_int64(0)
+    pkg._lib.lib().nvfp4_lora_workspace(T, r, n, ctypes.byref(need))
+    torch.full((max(need.value, 1),), 0xFF, dtype=torch.uint8, device=cuda)
+    got = pkg.lora_add(bigo[1:T + 1, 1:1 + N], bigx[:, 8:8 + K], biga[:n, :r, :K], bigb[:, :N, 8:8 + r], ad, sc, rk)
+    p.check(oracle, got)
+    assert (bigo[[0, T + 1]] == 5).all() and torch.isnan(bigo[1:T + 1, 0]).all() and torch.isnan(bigo[1:T + 1, N + 1:]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 200])
+@pytest.mark.parametrize("size", [1e-6, 2e3])
+def test_lora_far_ranges(pkg, oracle, cuda, T, size):
+    """Inner products far below and above fp16's range, brought back by B: u must not be rounded to fp16."""
+    K, N, r, n = 512, 64, 16, 2
+    p = Problem(T, K, N, r, n, mixed=False)
+    g = torch.Generator().manual_seed(3)
+    p.x = (torch.randn((T, K), generator=g) * max(size, 1)).to(torch.float16)
+    p.a = (torch.randn((n, r, K), generator=g) * size).to(torch.float16)
+    p.b = (torch.randn((n, N, r), generator=g) * (1e-6 if size > 1 else 1e4)).to(torch.float16)
+    p.scales = torch.full((n,), 1e-2 if size > 1 else 1.0)      # u * scale is about 1e6, or 2e-5
+    p.check(oracle, pkg.lora_add(*p.args()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [16, 300])
+def test_lora_graphs_and_streams(pkg, oracle, cuda, T):
+    ps = [Problem(T, 128, 200, 32, 4, seed=s) for s in (1, 2)]
+    live = [p.args() for p in ps]
+    outs = [torch.empty_like(a[0]) for a in live]
+    want = [pkg.lora_add(*a).clone() for a in [p.args() for p in ps]]
+    torch.cuda.synchronize()
+    graphs = []
+    for a, o in zip(live, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            pkg.lora_add(*a, out=o)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for o in outs:
+            o.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
+    live[0][4].copy_(live[1][4])          # other requests through the same graph
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    ps[0].adapters = ps[1].adapters
+    ps[0].check(oracle, outs[0])
+
+
+@pytest.mark.gpu
+def test_lora_beside_the_skinny_gemm(pkg, oracle, cuda):
+    """The projection as it is used: quantise, shared NVFP4 weights, adapters."""
+    T, K, N, r, n = 20, 512, 640, 32, 3
+    p = Problem(T, K, N, r, n)
+    w = pkg.inputs.operand(N, K, torch.Generator().manual_seed(4), device=cuda)
+    base, x, a, b, ad, sc, rk = p.args()
+    codes, sf = pkg.quantize(x)
+    pkg.skinny_gemm(codes, w.codes, sf, w.sf_blocked, base)
+    torch.cuda.synchronize()
+    p.base = base.cpu()
+    shared = oracle.gemm(codes.cpu(), w.codes.cpu(), sf.cpu(), w.sf_blocked.cpu(), T, N, K)
+    np.testing.assert_allclose(p.base.numpy().astype(np.float32), shared, rtol=1e-2, atol=1e-2)
+    p.check(oracle, pkg.lora_add(base, x, a, b, ad, sc, rk))
+
+
+@pytest.mark.gpu
+def test_lora_refusals(pkg, cuda):
+    p = Problem(4, 64, 72, 16, 2)
+    a = p.args()
+
+    def bad(i, t, err, match):
+        c = list(a)
+        c[i] = t
+        with pytest.raises(err, match=match):
+            pkg.lora_add(*c)
+    bad(0, a[0].cpu(), ValueError, "CUDA")
+    bad(0, a[0].float(), TypeError, "float16")
+    bad(1, a[1][:3], ValueError, "rows")
+    bad(1, a[1].bfloat16(), TypeError, "float16")
+    bad(2, a[2][:, :, :32], ValueError, "fit")
+    bad(3, a[3][:, :, :8], ValueError, "fit")
+    bad(4, a[4].long(), ValueError, "adapters")
+    bad(4, a[4][:3], ValueError, "adapters")
+    bad(5, a[5].double(), ValueError, "scales")
+    bad(6, a[6][:1], ValueError, "ranks")
+    with pytest.raises(RuntimeError, match="rank"):
+        pkg.lora_add(a[0], a[1], a[2][:, :8].contiguous(), a[3][:, :, :8].contiguous(), a[4])
+    with pytest.raises(ValueError, match="out"):
+        pkg.lora_add(*a, out=a[0][:3])
