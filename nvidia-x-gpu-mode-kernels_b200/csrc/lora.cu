@@ -12,12 +12,12 @@
 // u survive, whatever its range, and the sum stays in fp32.
 //
 // The k index of an mma is summed over, so its 16 slots may stand for any 16 elements as long as both operands
-// agree.  Slots {2q, 2q+1, 2q+8, 2q+9} of lane quarter q stand for 4 consecutive elements: fragments are loaded
-// from memory as they lie there, 8 or 16 bytes a lane, without shared memory.
+// agree.  Two mma's take 32 elements, slots {2q, 2q+1, 2q+8, 2q+9} of lane q of 4 standing for elements 8q..8q+3 in
+// the first and 8q+4..8q+7 in the second: fragments are loaded as they lie in memory, 16 bytes a lane.
 //
-// Few tokens (decode_kernel): one launch.  A cluster of 8 CTAs takes up to 8 tokens of one adapter: each
-// CTA sums an eighth of K for all ranks, the partial u's are exchanged through distributed shared memory and each
-// CTA writes an eighth of N.  B is prefetched into L2 at the start, so both matrices stream at once.
+// Few tokens (decode_kernel): one launch.  A cluster of CTAs takes up to 8 tokens of one adapter: each CTA
+// sums its share of K for all ranks, the partial u's are exchanged through distributed shared memory and each CTA
+// writes its share of N.  B is prefetched into L2 at the start, so both matrices stream at once.
 //
 // Many tokens: the plan (plan.cuh) orders them by adapter; shrink_kernel computes u, expand_kernel adds u . B^T.
 #include <cuda_fp16.h>
@@ -50,7 +50,7 @@ struct LoraArgs {
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                           uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -74,297 +74,402 @@ __device__ __forceinline__ void split_halves(float v, __half& hi, __half& lo) {
   lo = __float2half_rn(v - __half2float(hi));
 }
 
-// Four consecutive halves of a row of B from element k on, zeros from element `rank` on (which may hold anything).
-__device__ __forceinline__ uint2 load_b(const __half* row, int k, int rank) {
-  uint2 v = *reinterpret_cast<const uint2*>(row + k);
-  if (k + 4 > rank) {
-    if (k + 3 >= rank) v.y &= 0x0000ffffu;
-    if (k + 2 >= rank) v.y = 0;
-    if (k + 1 >= rank) v.x &= 0x0000ffffu;
-    if (k >= rank) v.x = 0;
+// Zeros from element `rank` on (the row may hold anything there) in eight consecutive halves from element k on.
+__device__ __forceinline__ uint4 below_rank(uint4 v, int k, int rank) {
+  if (k + 8 > rank) {
+    uint32_t* w = &v.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (k + 2 * j + 1 >= rank) w[j] &= 0x0000ffffu;
+      if (k + 2 * j >= rank) w[j] = 0;
+    }
   }
   return v;
 }
 
-// out[8 columns] = base + d, vectorised where the rows allow it.
-__device__ __forceinline__ void add_eight(const LoraArgs& p, int64_t t, int col, const float (&d)[8]) {
-  const __half* src = p.base + t * p.ld_base + col;
+// out[8 columns] = base + scale * d; `v` holds base where all 8 columns exist and the rows are 16-byte aligned.
+__device__ __forceinline__ void add_eight(const LoraArgs& p, int64_t t, int col, const float (&d)[8], float scale, uint4 v) {
   __half* dst = p.out + t * p.ldo + col;
   if (p.vec && col + 8 <= p.N) {
-    const uint4 v = *reinterpret_cast<const uint4*>(src);
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-      const __half2 h = __floats2half2_rn(f.x + d[2 * j], f.y + d[2 * j + 1]);
+      const __half2 h = __floats2half2_rn(fmaf(d[2 * j], scale, f.x), fmaf(d[2 * j + 1], scale, f.y));
       o[j] = *reinterpret_cast<const uint32_t*>(&h);
     }
     *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
   } else {
+    const __half* src = p.base + t * p.ld_base + col;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (col + j < p.N) dst[j] = __float2half_rn(__half2float(src[j]) + d[j]);
+      if (col + j < p.N) dst[j] = __float2half_rn(fmaf(d[j], scale, __half2float(src[j])));
   }
 }
 
+__device__ __forceinline__ void cp_async_16(void* dst, const void* src, bool copy) {   // zeros if not `copy`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"(smem_u32(dst)), "l"(src), "r"(copy ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" :: "n"(N) : "memory"); }
+
 // ------------------------------------------------------------------ few tokens
 
-constexpr int kCluster = 8;
 constexpr int kDecodeWarps = 8;
 
-// RT: 16-row tiles of the largest rank.
+__device__ __forceinline__ int cluster_nctas() {
+  uint32_t v;
+  asm volatile("mov.u32 %0, %cluster_nctaid.x;" : "=r"(v));
+  return (int)v;
+}
+
+constexpr int kDecodeTokens = 128;       // most tokens of one call
+static_assert(kDecodeTokens <= kDecodeWarps * 32, "a thread per token");
+
+// RT: 16-row tiles of the largest rank, even.
 template <int RT>
-__global__ void __cluster_dims__(kCluster, 1, 1) __launch_bounds__(kDecodeWarps * 32) decode_kernel(const LoraArgs p) {
-  constexpr int R = RT * 16;
-  __shared__ float part[kDecodeWarps][R][8];             // each warp's share of K; later the warps' output patches
+__global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_kernel(const __grid_constant__ LoraArgs p) {
+  constexpr int R = RT * 16, RS = RT / 2;                // RS: 32 ranks a step
+  constexpr bool kAhead = RT <= 4;                       // registers for the next step's B
+  // each warp's share of K, then u, in the end the warps' output patches
+  __shared__ __align__(16) float pool[kDecodeWarps * (R > 36 ? R : 36) * 8];
+  float(*const part)[R][8] = reinterpret_cast<float(*)[R][8]>(pool);
   __shared__ float mine[R][8];                           // this CTA's share of K
   __shared__ __align__(16) __half hi[8][R + 8], lo[8][R + 8];
   __shared__ float down[8];
-  __shared__ int tok[8];
-  __shared__ int ntok;
-  static_assert(sizeof(part) >= kDecodeWarps * 8 * 68 * 4 || RT < 8, "patch");
-  __shared__ float patch_small[RT < 8 ? kDecodeWarps * 8 * 68 : 1];
+  __shared__ int key[kDecodeTokens], items[kDecodeTokens], tok[8], warp_items[kDecodeTokens / 32];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int rank_in_cluster = (int)cluster_ctarank();
-  const int t0 = (int)(blockIdx.x / kCluster);
-  int i = p.adapters[t0];
-  if ((unsigned)i >= (unsigned)p.n) i = -1;
-  const int groups = (p.N + 63) / 64;                    // 64 columns per warp and step
-  const int glo = groups * rank_in_cluster / kCluster, ghi = groups * (rank_in_cluster + 1) / kCluster;
-  if (i < 0) {                                           // the whole cluster leaves together
-    if (!p.in_place)
-      for (int c = glo * 64 + tid; c < min(p.N, ghi * 64); c += blockDim.x)
-        p.out[t0 * p.ldo + c] = p.base[t0 * p.ld_base + c];
-    return;
-  }
-  // Tokens of one adapter go in eights, in token order; the first of an eight takes it.
-  int before = 0;
-  for (int s0 = 0; s0 < t0; s0 += blockDim.x) before += __syncthreads_count(s0 + tid < t0 && p.adapters[s0 + tid] == i);
-  if (before % 8) return;
-  if (warp == 0) {
-    if (lane < 8) tok[lane] = -1;
-    __syncwarp();
-    int found = 0;
-    for (int s0 = t0; s0 < p.T && found < 8; s0 += 32) {
-      const bool hit = s0 + lane < p.T && p.adapters[s0 + lane] == i;
-      const unsigned hits = __ballot_sync(0xffffffffu, hit);
-      const int at = found + __popc(hits & ((1u << lane) - 1));
-      if (hit && at < 8) tok[at] = s0 + lane;
-      found += __popc(hits);
-    }
-    if (lane == 0) ntok = min(found, 8);
-  }
-  const int rank = lora_rank(p, i);
-  const int steps_r = (rank + 15) / 16;
-  const __half* A = p.a + i * p.a_stride;
-  const __half* B = p.b + i * p.b_stride;
-  {
-    // B's rows of this CTA, on their way into L2 while A streams
-    const int n0 = glo * 64, n1 = min(p.N, ghi * 64);
-    const char* lo_b = reinterpret_cast<const char*>(B + n0 * p.ldb);
-    const int64_t bytes = n1 > n0 ? ((int64_t)(n1 - 1 - n0) * p.ldb + rank) * 2 : 0;
-    for (int64_t o = (int64_t)tid * 128; o < bytes; o += (int64_t)blockDim.x * 128)
-      asm volatile("prefetch.global.L2 [%0];" :: "l"(lo_b + o));
+  const int me = (int)cluster_ctarank(), ncta = cluster_nctas();
+  // ---- the work list, the same in every CTA: tokens of one adapter go in eights, in token order, and an item is
+  // the first token of an eight
+  if (tid < p.T) {
+    const int i = p.adapters[tid];
+    key[tid] = (unsigned)i < (unsigned)p.n ? i : -1;
   }
   __syncthreads();
-  // ---- u = x . A^T over this CTA's share of K: ranks are the mma's rows, tokens its columns
-  {
-    float acc[RT][4] = {};
-    const int ksteps = (p.K + 31) / 32;
-    const int klo = ksteps * rank_in_cluster / kCluster, khi = ksteps * (rank_in_cluster + 1) / kCluster;
-    const __half* xr = g < ntok ? p.x + (int64_t)tok[g] * p.ldx : nullptr;
-    for (int ks = klo + warp; ks < khi; ks += kDecodeWarps) {
-      const int k = ks * 32 + q * 8;
-      const bool in = k < p.K;                           // K is a multiple of 8
-      uint4 xv = make_uint4(0, 0, 0, 0);
-      if (xr && in) xv = *reinterpret_cast<const uint4*>(xr + k);
-      uint4 av[RT][2];
+  bool leads = false;
+  if (tid < p.T) {
+    int before = 0;
+    for (int s = 0; s < tid; ++s) before += key[s] == key[tid];
+    leads = before % 8 == 0 && (key[tid] >= 0 || !p.in_place);
+  }
+  const unsigned leaders = __ballot_sync(0xffffffffu, leads);
+  if (warp < kDecodeTokens / 32 && lane == 0) warp_items[warp] = __popc(leaders);
+  __syncthreads();
+  int nitems = 0, at = 0;
 #pragma unroll
-      for (int m = 0; m < RT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = m * 16 + h * 8 + g;
-          av[m][h] = make_uint4(0, 0, 0, 0);
-          if (row < rank && in) av[m][h] = *reinterpret_cast<const uint4*>(A + row * p.lda + k);
-        }
-#pragma unroll
-      for (int m = 0; m < RT; ++m) {
-        mma_16816(acc[m], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv.x, xv.y);
-        mma_16816(acc[m], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv.z, xv.w);
+  for (int w = 0; w < kDecodeTokens / 32; ++w) {
+    if (w == warp) at = nitems;
+    nitems += warp_items[w];
+  }
+  if (leads) items[at + __popc(leaders & ((1u << lane) - 1))] = tid;
+  __syncthreads();
+  const int groups = (p.N + 31) / 32;                    // 32 columns per warp and step
+  const int glo = groups * me / ncta, ghi = groups * (me + 1) / ncta;
+
+  for (int item = (int)(blockIdx.x / ncta); item < nitems; item += (int)(gridDim.x / ncta)) {
+    const int t0 = items[item], i = key[t0];
+    if (warp == 0) {                                     // the eight's tokens; the previous item's readers have left
+      if (lane < 8) tok[lane] = -1;
+      __syncwarp();
+      int found = 0;
+      for (int s0 = t0; s0 < p.T && found < 8; s0 += 32) {
+        const bool hit = s0 + lane < p.T && key[s0 + lane] == i;
+        const unsigned hits = __ballot_sync(0xffffffffu, hit);
+        const int to = found + __popc(hits & ((1u << lane) - 1));
+        if (hit && to < 8) tok[to] = s0 + lane;
+        found += __popc(hits);
       }
-    }
-#pragma unroll
-    for (int m = 0; m < RT; ++m) {
-      *reinterpret_cast<float2*>(&part[warp][m * 16 + g][2 * q]) = make_float2(acc[m][0], acc[m][1]);
-      *reinterpret_cast<float2*>(&part[warp][m * 16 + g + 8][2 * q]) = make_float2(acc[m][2], acc[m][3]);
-    }
-  }
-  __syncthreads();
-  for (int e = tid; e < R * 8; e += blockDim.x) {
-    float s = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDecodeWarps; ++w) s += part[w][e >> 3][e & 7];
-    mine[e >> 3][e & 7] = s;
-  }
-  cluster_sync();
-  // every CTA adds all shares in the same order: the same u everywhere
-  {
-    const float scale = p.scales ? p.scales[i] : 1.f;
-    float* u = &part[0][0][0];
-    for (int e = tid; e < R * 8; e += blockDim.x) {
-      const uint32_t here = smem_u32(&mine[e >> 3][e & 7]);
-      float s = 0.f;
-#pragma unroll
-      for (int c = 0; c < kCluster; ++c) s += __uint_as_float(ld_cluster_u32(mapa(here, c)));
-      u[e] = s * scale;
     }
     __syncthreads();
-    // warp w: token w
-    float m = 0.f;
+    if (i < 0) {                                         // no adapter: the rows stay what base says
+      for (int j = 0; j < 8 && tok[j] >= 0; ++j)
+        for (int c = glo * 32 + tid; c < min(p.N, ghi * 32); c += blockDim.x)
+          p.out[tok[j] * p.ldo + c] = p.base[tok[j] * p.ld_base + c];
+      __syncthreads();
+      continue;
+    }
+    const int rank = lora_rank(p, i);
+    const __half* A = p.a + i * p.a_stride;
+    const __half* B = p.b + i * p.b_stride;
+    {
+      // B's rows of this CTA, on their way into L2 while A streams
+      const int n0 = glo * 32, n1 = min(p.N, ghi * 32);
+      const char* lo_b = reinterpret_cast<const char*>(B + n0 * p.ldb);
+      const int64_t bytes = n1 > n0 ? ((int64_t)(n1 - 1 - n0) * p.ldb + rank) * 2 : 0;
+      for (int64_t o = (int64_t)tid * 128; o < bytes; o += (int64_t)blockDim.x * 128)
+        asm volatile("prefetch.global.L2 [%0];" :: "l"(lo_b + o));
+    }
+    // ---- u = x . A^T over this CTA's share of K: ranks are the mma's rows, tokens its columns
+    {
+      float acc[RT][4] = {};
+      const int ksteps = (p.K + 31) / 32;
+      const int klo = ksteps * me / ncta, khi = ksteps * (me + 1) / ncta;
+      const __half* xr = tok[g] >= 0 ? p.x + (int64_t)tok[g] * p.ldx : nullptr;
+#pragma unroll(kAhead ? 2 : 1)
+      for (int ks = klo + warp; ks < khi; ks += kDecodeWarps) {
+        const int k = ks * 32 + q * 8;
+        const bool in = k < p.K;                         // K is a multiple of 8
+        uint4 xv = make_uint4(0, 0, 0, 0);
+        if (xr && in) xv = *reinterpret_cast<const uint4*>(xr + k);
+        uint4 av[RT][2];
 #pragma unroll
-    for (int e = 0; e < R; e += 32)
-      if (e + lane < R) m = fmaxf(m, fabsf(u[(e + lane) * 8 + warp]));
+        for (int m = 0; m < RT; ++m)
 #pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float up, dn;
-    half_scale(m, up, dn);
+          for (int h = 0; h < 2; ++h) {
+            const int row = m * 16 + h * 8 + g;
+            av[m][h] = make_uint4(0, 0, 0, 0);
+            if (row < rank && in) av[m][h] = *reinterpret_cast<const uint4*>(A + row * p.lda + k);
+          }
 #pragma unroll
-    for (int e = 0; e < R; e += 32)
-      if (e + lane < R) split_halves(u[(e + lane) * 8 + warp] * up, hi[warp][e + lane], lo[warp][e + lane]);
-    if (lane == 0) down[warp] = dn;
-  }
-  cluster_sync();      // also: nobody leaves while its share is being read
-  // ---- out += u . B^T over this CTA's share of N: columns are the mma's rows, tokens its columns
-  uint32_t uh[RT][2], ul[RT][2];
+        for (int m = 0; m < RT; ++m) {
+          mma_16816(acc[m], av[m][0].x, av[m][1].x, av[m][0].y, av[m][1].y, xv.x, xv.y);
+          mma_16816(acc[m], av[m][0].z, av[m][1].z, av[m][0].w, av[m][1].w, xv.z, xv.w);
+        }
+      }
 #pragma unroll
-  for (int s = 0; s < RT; ++s) {
-    const uint2 h = *reinterpret_cast<const uint2*>(&hi[g][s * 16 + 4 * q]);
-    const uint2 l = *reinterpret_cast<const uint2*>(&lo[g][s * 16 + 4 * q]);
-    uh[s][0] = h.x; uh[s][1] = h.y;
-    ul[s][0] = l.x; ul[s][1] = l.y;
-  }
-  float* patch = (RT < 8 ? patch_small : &part[0][0][0]) + warp * 8 * 68;
-  for (int gr = glo + warp; gr < ghi; gr += kDecodeWarps) {
-    const int n0 = gr * 64;
-    float acc[4][4] = {};
-#pragma unroll
-    for (int s = 0; s < RT; ++s) {
-      if (s >= steps_r) break;
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        const int r0 = n0 + m * 16 + g, r1 = r0 + 8;
-        uint2 b0 = make_uint2(0, 0), b1 = make_uint2(0, 0);
-        if (r0 < p.N) b0 = load_b(B + r0 * p.ldb, s * 16 + 4 * q, rank);
-        if (r1 < p.N) b1 = load_b(B + r1 * p.ldb, s * 16 + 4 * q, rank);
-        mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, uh[s][0], uh[s][1]);
-        mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, ul[s][0], ul[s][1]);
+      for (int m = 0; m < RT; ++m) {
+        *reinterpret_cast<float2*>(&part[warp][m * 16 + g][2 * q]) = make_float2(acc[m][0], acc[m][1]);
+        *reinterpret_cast<float2*>(&part[warp][m * 16 + g + 8][2 * q]) = make_float2(acc[m][2], acc[m][3]);
       }
     }
-    // [token][column] patch, so that lanes write runs of a token's columns
+    __syncthreads();
+    for (int e = tid; e < R * 8; e += blockDim.x) {
+      float s = 0.f;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      patch[(2 * q) * 68 + m * 16 + g] = acc[m][0];
-      patch[(2 * q + 1) * 68 + m * 16 + g] = acc[m][1];
-      patch[(2 * q) * 68 + m * 16 + g + 8] = acc[m][2];
-      patch[(2 * q + 1) * 68 + m * 16 + g + 8] = acc[m][3];
+      for (int w = 0; w < kDecodeWarps; ++w) s += part[w][e >> 3][e & 7];
+      mine[e >> 3][e & 7] = s;
     }
-    __syncwarp();
+    cluster_sync();
+    // every CTA adds all shares in the same order: the same u everywhere
+    {
+      const float scale = p.scales ? p.scales[i] : 1.f;
+      float* const u = pool;
+      for (int e = tid; e < R * 8; e += blockDim.x) {
+        const uint32_t here = smem_u32(&mine[e >> 3][e & 7]);
+        float s = 0.f;
+#pragma unroll 8
+        for (int c = 0; c < ncta; ++c) s += __uint_as_float(ld_cluster_u32(mapa(here, c)));
+        u[e] = s * scale;
+      }
+      __syncthreads();
+      // warp w: token w
+      float m = 0.f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = h * 4 + (lane >> 3), c = (lane & 7) * 8;
-      if (j < ntok && n0 + c < p.N) {
+      for (int e = 0; e < R; e += 32)
+        if (e + lane < R) m = fmaxf(m, fabsf(u[(e + lane) * 8 + warp]));
+#pragma unroll
+      for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      float up, dn;
+      half_scale(m, up, dn);
+#pragma unroll
+      for (int e = 0; e < R; e += 32)
+        if (e + lane < R) split_halves(u[(e + lane) * 8 + warp] * up, hi[warp][e + lane], lo[warp][e + lane]);
+      if (lane == 0) down[warp] = dn;
+    }
+    cluster_sync();    // also: the shares have been read everywhere, and pool is free
+    // ---- out += u . B^T over this CTA's share of N: columns are the mma's rows, tokens its columns
+    uint4 uh[RS], ul[RS];
+#pragma unroll
+    for (int s = 0; s < RS; ++s) {
+      uh[s] = *reinterpret_cast<const uint4*>(&hi[g][s * 32 + 8 * q]);
+      ul[s] = *reinterpret_cast<const uint4*>(&lo[g][s * 32 + 8 * q]);
+    }
+    float(*const patch)[36] = reinterpret_cast<float(*)[36]>(pool + warp * 8 * 36);
+    const int j = lane >> 2, mytok = tok[j];             // this lane's token and columns in the end
+    const float mydown = down[j];
+    uint4 bv[RS][4], bn[RS][4], basev, basen;
+    auto ask = [&](int gr, uint4 (&v)[RS][4], uint4& base) {   // all that a step reads
+      const int n0 = gr * 32;
+#pragma unroll
+      for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int col = n0 + m * 8 + g;
+          v[s][m] = make_uint4(0, 0, 0, 0);
+          if (gr < ghi && s * 32 + 8 * q < rank && col < p.N)
+            v[s][m] = *reinterpret_cast<const uint4*>(B + col * p.ldb + s * 32 + 8 * q);
+        }
+      const int c = n0 + (lane & 3) * 8;
+      base = make_uint4(0, 0, 0, 0);
+      if (gr < ghi && p.vec && mytok >= 0 && c + 8 <= p.N)
+        base = *reinterpret_cast<const uint4*>(p.base + mytok * p.ld_base + c);
+    };
+    if (kAhead) ask(glo + warp, bn, basen);
+    for (int gr = glo + warp; gr < ghi; gr += kDecodeWarps) {
+      const int c = gr * 32 + (lane & 3) * 8;
+      if (kAhead) {
+#pragma unroll
+        for (int s = 0; s < RS; ++s)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) bv[s][m] = bn[s][m];
+        basev = basen;
+        ask(gr + kDecodeWarps, bn, basen);
+      } else {
+        ask(gr, bv, basev);
+      }
+      float acc[2][4] = {};
+#pragma unroll
+      for (int s = 0; s < RS; ++s) {
+        if (s * 32 >= rank) break;
+        if (rank & 7) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) bv[s][m] = below_rank(bv[s][m], s * 32 + 8 * q, rank);
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint4 b0 = bv[s][2 * m], b1 = bv[s][2 * m + 1];
+          mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, uh[s].x, uh[s].y);
+          mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, ul[s].x, ul[s].y);
+          mma_16816(acc[m], b0.z, b1.z, b0.w, b1.w, uh[s].z, uh[s].w);
+          mma_16816(acc[m], b0.z, b1.z, b0.w, b1.w, ul[s].z, ul[s].w);
+        }
+      }
+      // [token][column] patch, so that a lane gets a run of one token's columns
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        patch[2 * q][m * 16 + g] = acc[m][0];
+        patch[2 * q + 1][m * 16 + g] = acc[m][1];
+        patch[2 * q][m * 16 + g + 8] = acc[m][2];
+        patch[2 * q + 1][m * 16 + g + 8] = acc[m][3];
+      }
+      __syncwarp();
+      if (mytok >= 0 && c < p.N) {
         float d[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = patch[j * 68 + c + e] * down[j];
-        add_eight(p, tok[j], n0 + c, d);
+        for (int e = 0; e < 8; ++e) d[e] = patch[j][(lane & 3) * 8 + e];
+        add_eight(p, mytok, c, d, mydown, basev);
       }
+      __syncwarp();
     }
-    __syncwarp();
+    __syncthreads();                                     // pool, tok and down are reused
   }
 }
 
 // ------------------------------------------------------------------ many tokens
 
-constexpr int kTile = 64;                // tokens per tile of the plan
-constexpr int kShrinkTokens = 32;        // tokens per CTA of the first product
-constexpr int kShrinkWarps = 8;
-constexpr int kExpandWarps = 8;
+constexpr int kTile = 128;               // tokens per tile of the plan
+constexpr int kShrinkTokens = 64;        // tokens per CTA of the first product
+constexpr int kShrinkK = 128;            // elements of K per stage
+constexpr int kShrinkStages = 3;
+constexpr int kExpandCols = 64;          // columns per step of the second product
+constexpr int kExpandStages = 3;
+constexpr int kLoraThreads = 256;
 
 struct LoraRows {
   const int* ntiles;
   const PlanTile* tiles;
   const int* slot;                       // token of each row, -1 for padding
-  __half* hi;                            // [rows][R], R = r rounded up to 16, 32, 64, 128
+  __half* hi;                            // [rows][R], R = r rounded up to 32, 64 or 128
   __half* lo;
   float* down;                           // [rows]
 };
 
-// u of 32 tokens of one adapter: tokens are the mma's rows, ranks its columns; the warps share K.
+// Row length in halves of a tile in shared memory that is read 16 bytes a lane, two neighbouring rows of 4 lanes
+// at a time: rows 16 words apart modulo the 32 banks.
+constexpr int padded_row(int halves) { return halves % 64 ? halves : halves + 32; }
+
 template <int RT>
-__global__ void __launch_bounds__(kShrinkWarps * 32) shrink_kernel(const LoraArgs p, const LoraRows w) {
-  constexpr int R = RT * 16, NT = RT * 2;
-  extern __shared__ __align__(16) float part[];          // [warps][32 tokens][R]
+struct LoraCfg {
+  static constexpr int R = RT * 16;
+  static constexpr int LDK = padded_row(kShrinkK), LDR = padded_row(R);
+  static constexpr int SHRINK_STAGE = (kShrinkTokens + R) * LDK * 2;
+  static constexpr int SHRINK_SMEM = kShrinkStages * SHRINK_STAGE;
+  static_assert(SHRINK_SMEM >= 2 * kShrinkTokens * R * 4, "the two halves of u");
+  static constexpr int EXPAND_B = kExpandCols * LDR * 2;
+  static constexpr int EXPAND_BASE = 8 * 4 * 512;        // a warp's 16 tokens x 64 columns, 4 pieces a lane
+  static constexpr int EXPAND_SMEM = kExpandStages * (EXPAND_B + EXPAND_BASE);
+};
+
+// u of 64 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
+// of 128-element stages; four warps take 16 tokens each over the first half of a stage, four over the second.
+template <int RT>
+__global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
+  using C = LoraCfg<RT>;
+  constexpr int R = C::R, NT = RT * 2, PER = kTile / kShrinkTokens, LD = C::LDK, CHUNKS = kShrinkK / 8;
+  extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int m0 = (warp & 3) * 16, khalf = (warp >> 2) * (kShrinkK / 2);
   griddep_launch();
   griddep_wait();
-  const int total = *w.ntiles * (kTile / kShrinkTokens);
+  const int total = *w.ntiles * PER;
+  const int nk = (p.K + kShrinkK - 1) / kShrinkK;
   for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const PlanTile tile = w.tiles[item / 2];
-    const int tr = (item / 2 - tile.first) * kTile + (item & 1) * kShrinkTokens;   // first token within the adapter
+    const PlanTile tile = w.tiles[item / PER];
+    const int tr = (item / PER - tile.first) * kTile + item % PER * kShrinkTokens;   // first token within the adapter
     if (tile.index >= p.n || tr >= tile.rows) continue;
     const int row0 = tile.row0 + tr;
     const int rank = lora_rank(p, tile.index);
     const __half* A = p.a + tile.index * p.a_stride;
-    const __half* xr[4];
+    // this thread's pieces of a stage: 16 threads a row, 16 rows a pass
+    const int pc = tid % CHUNKS * 8, pr = tid / CHUNKS;
+    constexpr int XP = kShrinkTokens / (kLoraThreads / CHUNKS), AP = (R + kLoraThreads / CHUNKS - 1) / (kLoraThreads / CHUNKS);
+    const __half* xp[XP];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int s = w.slot[row0 + m * 8 + g];
-      xr[m] = s >= 0 ? p.x + (int64_t)s * p.ldx : nullptr;
+    for (int e = 0; e < XP; ++e) {
+      const int s = w.slot[row0 + e * (kLoraThreads / CHUNKS) + pr];
+      xp[e] = s >= 0 ? p.x + (int64_t)s * p.ldx : nullptr;
     }
-    float acc[2][NT][4] = {};
-    for (int k0 = warp * 32; k0 < p.K; k0 += kShrinkWarps * 32) {
-      const int k = k0 + q * 8;
-      const bool in = k < p.K;
-      uint4 xv[4];
+    auto ask = [&](int ks) {
+      if (ks < nk) {
+        __half* const st = reinterpret_cast<__half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
+        const int k = ks * kShrinkK + pc;
 #pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        xv[m] = make_uint4(0, 0, 0, 0);
-        if (xr[m] && in) xv[m] = *reinterpret_cast<const uint4*>(xr[m] + k);
+        for (int e = 0; e < XP; ++e) {
+          const bool in = xp[e] && k < p.K;
+          cp_async_16(st + (e * (kLoraThreads / CHUNKS) + pr) * LD + pc, in ? xp[e] + k : p.x, in);
+        }
+#pragma unroll
+        for (int e = 0; e < AP; ++e) {
+          const int row = e * (kLoraThreads / CHUNKS) + pr;
+          const bool in = row < rank && k < p.K;
+          if (row < R) cp_async_16(st + (kShrinkTokens + row) * LD + pc, in ? A + row * p.lda + k : p.a, in);
+        }
       }
+      cp_async_commit();
+    };
+    __syncthreads();                                     // the previous item's shared memory is read
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        uint4 av = make_uint4(0, 0, 0, 0);
-        if (nt * 8 + g < rank && in) av = *reinterpret_cast<const uint4*>(A + (nt * 8 + g) * p.lda + k);
+    for (int s = 0; s < kShrinkStages - 1; ++s) ask(s);
+    float acc[NT][4] = {};
+    for (int ks = 0; ks < nk; ++ks) {
+      cp_async_wait<kShrinkStages - 2>();
+      __syncthreads();                                   // stage ks is here, stage ks - 1 free
+      ask(ks + kShrinkStages - 1);
+      const __half* const st = reinterpret_cast<const __half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
+      const __half* const xs = st + (m0 + g) * LD + khalf + 8 * q;
+      const __half* const as = st + (kShrinkTokens + g) * LD + khalf + 8 * q;
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          mma_16816(acc[m][nt], xv[2 * m].x, xv[2 * m + 1].x, xv[2 * m].y, xv[2 * m + 1].y, av.x, av.y);
-          mma_16816(acc[m][nt], xv[2 * m].z, xv[2 * m + 1].z, xv[2 * m].w, xv[2 * m + 1].w, av.z, av.w);
+      for (int s = 0; s < kShrinkK / 64; ++s) {
+        const uint4 x0 = *reinterpret_cast<const uint4*>(xs + s * 32), x1 = *reinterpret_cast<const uint4*>(xs + 8 * LD + s * 32);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          if (nt * 8 >= rank) break;
+          const uint4 a = *reinterpret_cast<const uint4*>(as + nt * 8 * LD + s * 32);
+          mma_16816(acc[nt], x0.x, x1.x, x0.y, x1.y, a.x, a.y);
+          mma_16816(acc[nt], x0.z, x1.z, x0.w, x1.w, a.z, a.w);
         }
       }
     }
-    __syncthreads();                                     // the previous item's sums are read
+    cp_async_wait<0>();
+    __syncthreads();
+    float* const part = reinterpret_cast<float*>(smem);  // [half of K][64 tokens][R]
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float* at = part + (warp * kShrinkTokens + m * 16 + g) * R + nt * 8 + 2 * q;
-        *reinterpret_cast<float2*>(at) = make_float2(acc[m][nt][0], acc[m][nt][1]);
-        *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[m][nt][2], acc[m][nt][3]);
-      }
+    for (int nt = 0; nt < NT; ++nt) {
+      float* at = part + ((warp >> 2) * kShrinkTokens + m0 + g) * R + nt * 8 + 2 * q;
+      *reinterpret_cast<float2*>(at) = make_float2(acc[nt][0], acc[nt][1]);
+      *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[nt][2], acc[nt][3]);
+    }
     __syncthreads();
     const float scale = p.scales ? p.scales[tile.index] : 1.f;
-    for (int t = warp; t < kShrinkTokens; t += kShrinkWarps) {
-      float u[(R + 31) / 32];
+    for (int t = warp; t < kShrinkTokens; t += kLoraThreads / 32) {
+      float u[R / 32];
       float m = 0.f;
 #pragma unroll
-      for (int e = 0; e < (R + 31) / 32; ++e) {
-        u[e] = 0.f;
-        if (e * 32 + lane < R) {
-#pragma unroll
-          for (int v = 0; v < kShrinkWarps; ++v) u[e] += part[(v * kShrinkTokens + t) * R + e * 32 + lane];
-        }
-        u[e] *= scale;
+      for (int e = 0; e < R / 32; ++e) {
+        const float* at = part + t * R + e * 32 + lane;
+        u[e] = (at[0] + at[kShrinkTokens * R]) * scale;
         m = fmaxf(m, fabsf(u[e]));
       }
 #pragma unroll
@@ -373,96 +478,128 @@ __global__ void __launch_bounds__(kShrinkWarps * 32) shrink_kernel(const LoraArg
       half_scale(m, up, dn);
       const int64_t row = row0 + t;
 #pragma unroll
-      for (int e = 0; e < (R + 31) / 32; ++e)
-        if (e * 32 + lane < R) {
-          __half h, l;
-          split_halves(u[e] * up, h, l);
-          w.hi[row * R + e * 32 + lane] = h;
-          w.lo[row * R + e * 32 + lane] = l;
-        }
+      for (int e = 0; e < R / 32; ++e) {
+        __half h, l;
+        split_halves(u[e] * up, h, l);
+        w.hi[row * R + e * 32 + lane] = h;
+        w.lo[row * R + e * 32 + lane] = l;
+      }
       if (lane == 0) w.down[row] = dn;
     }
   }
 }
 
-// out += u . B^T for 64 tokens of one adapter and a run of columns: a warp takes 64 tokens x 32 columns at a time.
-// The 8 columns of mma tile j stand for columns 8 (c / 2) + 2 j + c % 2 of the 32, so that the four tiles give
-// a lane 8 consecutive columns of a token.
+// out += u . B^T for 128 tokens of one adapter and a run of columns, 64 at a time: a warp takes 16 tokens, whose u
+// stays in its registers.  B comes through a ring in shared memory that all warps read; base through a ring of
+// which each lane reads back just what it asked for itself.
+// The 8 columns of mma tile j of four stand for columns 8 (c / 2) + 2 j + c % 2 of 32, so that the four tiles
+// give a lane 8 consecutive columns of a token.
 template <int RT>
-__global__ void __launch_bounds__(kExpandWarps * 32) expand_kernel(const LoraArgs p, const LoraRows w, int nsplit) {
-  constexpr int R = RT * 16, LD = R + 8;
-  extern __shared__ __align__(16) __half us[];           // hi [64][LD], lo [64][LD]
-  __shared__ int tok[kTile];
-  __shared__ float down[kTile];
+__global__ void __launch_bounds__(kLoraThreads, 2)
+    expand_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
+  using C = LoraCfg<RT>;
+  constexpr int R = C::R, LD = C::LDR, RS = RT / 2, CHUNKS = R / 8;
+  extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  uint8_t* const bases = smem + kExpandStages * C::EXPAND_B + warp * 2048 + lane * 16;
   griddep_launch();
   griddep_wait();
-  const int total = *w.ntiles * nsplit;
-  const int groups = (p.N + 31) / 32;
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
-    const PlanTile tile = w.tiles[item / nsplit];
-    const int part = item % nsplit;
-    const int row0 = tile.row0 + (item / nsplit - tile.first) * kTile;
-    const bool none = tile.index >= p.n;
+  // all steps of all tiles in one row, an equal run of them for each CTA
+  const int steps = (p.N + kExpandCols - 1) / kExpandCols;
+  const int64_t total = (int64_t)*w.ntiles * steps;
+  const int64_t end = total * (blockIdx.x + 1) / gridDim.x;
+  for (int64_t at = total * blockIdx.x / gridDim.x; at < end;) {
+    const int index = (int)(at / steps);
+    const int lo = (int)(at - (int64_t)index * steps), hi = (int)min((int64_t)steps, lo + (end - at));
+    at += hi - lo;
+    const PlanTile tile = w.tiles[index];
+    const int tr = (index - tile.first) * kTile;
+    const int row0 = tile.row0 + tr + warp * 16;
+    const bool none = tile.index >= p.n, live = tr + warp * 16 < tile.rows;
     const int rank = none ? 0 : lora_rank(p, tile.index);
-    const int steps = (rank + 15) / 16;
-    __syncthreads();
-    if (tid < kTile) {
-      tok[tid] = w.slot[row0 + tid];
-      down[tid] = tok[tid] >= 0 && !none ? w.down[row0 + tid] : 0.f;
-    }
-    if (!none)
-      for (int e = tid; e < kTile * R / 8; e += blockDim.x) {
-        const int t = e / (R / 8), c = e % (R / 8) * 8;
-        *reinterpret_cast<uint4*>(us + t * LD + c) = *reinterpret_cast<const uint4*>(w.hi + (int64_t)(row0 + t) * R + c);
-        *reinterpret_cast<uint4*>(us + (kTile + t) * LD + c) = *reinterpret_cast<const uint4*>(w.lo + (int64_t)(row0 + t) * R + c);
-      }
-    __syncthreads();
-    const __half* B = none ? nullptr : p.b + tile.index * p.b_stride;
-    const int glo = groups * part / nsplit, ghi = groups * (part + 1) / nsplit;
-    for (int gr = glo + warp; gr < ghi; gr += kExpandWarps) {
-      const int n0 = gr * 32;
-      float acc[4][4][4] = {};                           // [16 tokens][column tile]
+    const __half* const B = none ? p.b : p.b + tile.index * p.b_stride;
+    int tok[2];
+    float down[2];
+    uint4 u[2][2][RS];                                   // [hi, lo][row g, g + 8][step]
 #pragma unroll
-      for (int s = 0; s < RT; ++s) {
-        if (s >= steps) break;
-        uint2 b[4];
+    for (int h = 0; h < 2; ++h) {
+      tok[h] = live ? w.slot[row0 + h * 8 + g] : -1;
+      down[h] = tok[h] >= 0 && !none ? w.down[row0 + h * 8 + g] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int col = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-          b[j] = make_uint2(0, 0);
-          if (col < p.N) b[j] = load_b(B + col * p.ldb, s * 16 + 4 * q, rank);
+      for (int s = 0; s < RS; ++s) {
+        u[0][h][s] = u[1][h][s] = make_uint4(0, 0, 0, 0);
+        if (s * 32 < rank && live) {
+          const int64_t from = (int64_t)(row0 + h * 8 + g) * R + s * 32 + 8 * q;
+          u[0][h][s] = *reinterpret_cast<const uint4*>(w.hi + from);
+          u[1][h][s] = *reinterpret_cast<const uint4*>(w.lo + from);
         }
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const __half* at = us + (h * kTile + m * 16 + g) * LD + s * 16 + 4 * q;
-            const uint2 u0 = *reinterpret_cast<const uint2*>(at), u1 = *reinterpret_cast<const uint2*>(at + 8 * LD);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) mma_16816(acc[m][j], u0.x, u1.x, u0.y, u1.y, b[j].x, b[j].y);
-          }
       }
+    }
+    auto ask = [&](int st) {
+      if (st < hi) {
+        const int ring = (st - lo) % kExpandStages;
+        __half* const bs = reinterpret_cast<__half*>(smem + ring * C::EXPAND_B);
+        const int n0 = st * kExpandCols;
+        if (rank > 0) {
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+          for (int e = tid; e < kExpandCols * CHUNKS; e += kLoraThreads) {
+            const int c = e / CHUNKS, k = e % CHUNKS * 8;
+            const bool in = n0 + c < p.N && k < rank;
+            cp_async_16(bs + c * LD + k, in ? B + (n0 + c) * p.ldb + k : p.b, in);
+          }
+        }
+        if (p.vec) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int t = m * 16 + h * 8 + g;
-          if (tok[t] < 0) continue;
-          float d[8];
+          for (int e = 0; e < 4; ++e) {                  // [column half][row half]
+            const int col = n0 + (e >> 1) * 32 + 8 * q;
+            if (tok[e & 1] >= 0 && col + 8 <= p.N)
+              cp_async_16(bases + ring * C::EXPAND_BASE + e * 512, p.base + tok[e & 1] * p.ld_base + col, true);
+          }
+        }
+      }
+      cp_async_commit();
+    };
+    __syncthreads();                                     // the previous item's ring is read
+#pragma unroll
+    for (int s = 0; s < kExpandStages - 1; ++s) ask(lo + s);
+    for (int st = lo; st < hi; ++st) {
+      cp_async_wait<kExpandStages - 2>();
+      __syncthreads();                                   // step st is here, step st - 1's ring free
+      ask(st + kExpandStages - 1);
+      const int ring = (st - lo) % kExpandStages;
+      const __half* const bs = reinterpret_cast<const __half*>(smem + ring * C::EXPAND_B) + (8 * (g >> 1) + (g & 1)) * LD + 8 * q;
+      if (!live) continue;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        float acc[4][4] = {};
+#pragma unroll
+        for (int s = 0; s < RS; ++s) {
+          if (s * 32 >= rank) break;
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            d[2 * j] = acc[m][j][2 * h] * down[t];
-            d[2 * j + 1] = acc[m][j][2 * h + 1] * down[t];
+            uint4 b = *reinterpret_cast<const uint4*>(bs + (half * 32 + 2 * j) * LD + s * 32);
+            if (rank & 7) b = below_rank(b, s * 32 + 8 * q, rank);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              mma_16816(acc[j], u[h][0][s].x, u[h][1][s].x, u[h][0][s].y, u[h][1][s].y, b.x, b.y);
+              mma_16816(acc[j], u[h][0][s].z, u[h][1][s].z, u[h][0][s].w, u[h][1][s].w, b.z, b.w);
+            }
           }
-          if (n0 + 8 * q < p.N) add_eight(p, tok[t], n0 + 8 * q, d);
         }
+        const int col = st * kExpandCols + half * 32 + 8 * q;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (tok[h] < 0 || col >= p.N) continue;
+          float d[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d[2 * j] = acc[j][2 * h], d[2 * j + 1] = acc[j][2 * h + 1];
+          add_eight(p, tok[h], col, d, down[h], *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512));
+        }
+      }
     }
+    cp_async_wait<0>();
   }
 }
-
-// Up to this many tokens take decode_kernel.
-constexpr int kDecodeTokens = 128;
 
 struct LoraLayout {
   int R;                                 // rank the kernels are built for
@@ -473,7 +610,7 @@ struct LoraLayout {
 LoraLayout lora_layout(int64_t T, int64_t r, int64_t n) {
   LoraLayout m;
   std::memset(&m, 0, sizeof(m));
-  m.R = r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : 128;
+  m.R = r <= 32 ? 32 : r <= 64 ? 64 : 128;
   if (T <= kDecodeTokens) return m;
   m.rows = plan_max_rows(T, n + 1, kTile);
   m.max_tiles = plan_max_tiles(T, n + 1, kTile);
@@ -503,9 +640,42 @@ int lora_check(int64_t T, int64_t r, int64_t n) {
 
 template <int RT>
 int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t stream) {
+  using C = LoraCfg<RT>;
+  static bool attr_set[64] = {};
+  static bool wide[64] = {};             // clusters of 16 fit
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.blockDim = dim3(kDecodeWarps * 32);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (!attr_set[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) {
+      int fit = 0;
+      cfg.gridDim = dim3(16);
+      wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT>, &cfg) == cudaSuccess && fit > 0;
+      cudaGetLastError();
+      e = cudaFuncSetAttribute(shrink_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHRINK_SMEM);
+    }
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(expand_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(low-rank products)");
+    attr_set[dev] = true;
+  }
   if (p.T <= kDecodeTokens) {
-    decode_kernel<RT><<<p.T * kCluster, kDecodeWarps * 32, 0, stream>>>(p);
-    return check_launch("decode_kernel");
+    const int ncta = p.T <= 4 && wide[dev] ? 16 : 8;
+    attr[0].val.clusterDim.x = (unsigned)ncta;
+    cfg.gridDim = dim3((unsigned)(std::min(p.T, std::max(1, sm_count() * 2 / ncta)) * ncta));
+    cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<RT>, p);
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaLaunchKernelEx(decode)");
   }
   const Plan plan = {reinterpret_cast<int*>(ws), reinterpret_cast<PlanTile*>(ws + m.tiles),
                      reinterpret_cast<int*>(ws + m.row), reinterpret_cast<int*>(ws + m.slot)};
@@ -514,26 +684,14 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   if (rc) return rc;
   const LoraRows rows = {plan.head, plan.tiles, plan.slot, reinterpret_cast<__half*>(ws + m.hi),
                          reinterpret_cast<__half*>(ws + m.lo), reinterpret_cast<float*>(ws + m.down)};
-  constexpr int kShrinkSmem = kShrinkWarps * kShrinkTokens * RT * 16 * 4;
-  constexpr int kExpandSmem = 2 * kTile * (RT * 16 + 8) * 2;
-  static bool attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
-  if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(shrink_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kShrinkSmem);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(shrink)");
-    attr_set[dev] = true;
-  }
-  const int64_t most = m.max_tiles;
   if ((rc = launch_after(shrink_kernel<RT>, "shrink_kernel",
-                         (unsigned)std::min<int64_t>(most * (kTile / kShrinkTokens), (int64_t)sm_count() * 2),
-                         kShrinkWarps * 32, kShrinkSmem, stream, p, rows)))
+                         (unsigned)std::min<int64_t>(m.max_tiles * (kTile / kShrinkTokens), (int64_t)sm_count() * 2),
+                         kLoraThreads, C::SHRINK_SMEM, stream, p, rows)))
     return rc;
-  // enough items for four rounds over the SMs, at least eight column groups (one per warp) each
-  const int nsplit = (int)std::max<int64_t>(1, std::min<int64_t>((p.N + 255) / 256, (int64_t)sm_count() * 8 * kTile / p.T));
-  return launch_after(expand_kernel<RT>, "expand_kernel", (unsigned)std::min<int64_t>(most * nsplit, (int64_t)sm_count() * 2),
-                      kExpandWarps * 32, kExpandSmem, stream, p, rows, nsplit);
+  const int64_t steps = (p.N + kExpandCols - 1) / kExpandCols;
+  return launch_after(expand_kernel<RT>, "expand_kernel",
+                      (unsigned)std::min<int64_t>(m.max_tiles * ((steps + 3) / 4), (int64_t)sm_count() * 2), kLoraThreads,
+                      C::EXPAND_SMEM, stream, p, rows);
 }
 
 }  // namespace
@@ -587,7 +745,6 @@ extern "C" int nvfp4_lora_add(const void* base, int64_t ld_base, const void* x, 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (m.R) {
-    case 16: return lora_run<1>(p, m, ws, st);
     case 32: return lora_run<2>(p, m, ws, st);
     case 64: return lora_run<4>(p, m, ws, st);
     default: return lora_run<8>(p, m, ws, st);

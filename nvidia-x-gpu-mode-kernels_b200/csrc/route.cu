@@ -22,6 +22,7 @@
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
+#include <type_traits>
 #include "common.h"
 #include "ptx.cuh"
 
@@ -156,21 +157,27 @@ __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float
       }
       if (lane == g && first) mine = K::key(sum);
     };
-    if (p.group_size % 32 == 0) {        // groups are runs of registers: one pass over them
-      U top = 0, next = 0;
-      int g = 0, left = p.group_size;
+    // groups of 32, 64 or 128 experts are 1, 2 or 4 whole registers: compile-time loops, whose warp-wide
+    // maxima overlap
+    auto by_registers = [&](auto regs) {
+      constexpr int RPG = decltype(regs)::value;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        if (g < p.groups) {
+      for (int g = 0; g * RPG < VPL; ++g) {
+        U top = 0, next = 0;
+#pragma unroll
+        for (int i = g * RPG; i < (g + 1) * RPG && i < VPL; ++i) {
           next = key[i] > top ? top : (key[i] > next ? key[i] : next);
           top = key[i] > top ? key[i] : top;
-          if ((left -= 32) == 0) {
-            group_score(g++, top, next);
-            top = next = 0;
-            left = p.group_size;
-          }
         }
+        group_score(g, top, next);
       }
+    };
+    if (kScreen && p.group_size == 32) {
+      by_registers(std::integral_constant<int, 1>());
+    } else if (kScreen && p.group_size == 64) {
+      by_registers(std::integral_constant<int, 2>());
+    } else if (kScreen && p.group_size == 128) {
+      by_registers(std::integral_constant<int, 4>());
     } else {
       for (int g = 0; g < p.groups; ++g) {
         U top = 0, next = 0;
@@ -281,46 +288,268 @@ __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float
   return false;
 }
 
+// Row t's logits (expert i * 32 + lane): -inf where the expert is off, at most the largest float.
+template <int VPL, bool BIAS>
+__device__ __forceinline__ void load_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
+                                         float (&x)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) x[i] = -INFINITY;
+  if (p.dtype == 0) {
+    const float* row = static_cast<const float*>(p.logits) + t * p.ld;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i * 32 + lane < p.E) x[i] = row[i * 32 + lane];
+  } else if (p.dtype == 1) {
+    const __half* row = static_cast<const __half*>(p.logits) + t * p.ld;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i * 32 + lane < p.E) x[i] = __half2float(row[i * 32 + lane]);
+  } else {
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (i * 32 + lane < p.E) x[i] = __bfloat162float(row[i * 32 + lane]);
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    x[i] = x[i] > -INFINITY ? fminf(x[i], FLT_MAX) : -INFINITY;       // NaN is off
+    if (BIAS && !(bias[i] > -INFINITY)) x[i] = -INFINITY;
+  }
+}
+
+template <int VPL, bool BIAS>
+__device__ __forceinline__ void load_bias(const RouteArgs& p, int lane, float (&bias)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    bias[i] = BIAS && i * 32 + lane < p.E ? p.bias[i * 32 + lane] : 0.f;
+    if (!(bias[i] > -INFINITY)) bias[i] = -INFINITY;     // NaN: off, too
+  }
+}
+
+__device__ __forceinline__ void store_row(const RouteArgs& p, int64_t t, int lane, int id, float w) {
+  if (lane < p.k) {
+    p.ids[t * p.k + lane] = id;
+    p.weights[t * p.k + lane] = w;
+  }
+}
+
+// A row that 32 bits could not decide, from the start: a function of its own, so that the common path keeps
+// none of it in registers.
 template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
-__global__ void __launch_bounds__(256) route_kernel(const RouteArgs p) {
+__device__ __noinline__ void route_row_in_64_bits(const RouteArgs& p, int64_t t, int lane) {
+  float bias[VPL], x[VPL];
+  load_bias<VPL, BIAS>(p, lane, bias);
+  load_row<VPL, BIAS>(p, t, lane, bias, x);
+  int id;
+  float w;
+  route_row<double, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w);
+  store_row(p, t, lane, id, w);
+}
+
+__device__ __forceinline__ float warp_max_float(float v) {      // no NaN among the values
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float reciprocal_approx(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The 32-bit pass over a row with a bias, where every choice is approximate anyway: floats instead of keys
+// (-inf: off), and the lowest bits of a choice replaced by its place in the lane, so that a lane's choices
+// differ and carry their index.  That moves a choice by less than VPL units of 2^-23 relative.  grp: each
+// expert's group.  Returns true where a comparison is too near: the row then needs the 64-bit pass.
+template <int VPL, bool SOFTMAX, bool GROUPS>
+__device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
+                                         const int (&grp)[VPL], int& id, float& weight) {
+  constexpr float kLog2e = 1.4426950408889634f;
+  constexpr uint32_t kPlace = VPL - 1;
+  constexpr float kTol = 4e-6f + 2 * VPL * 1.2e-7f;
+  float c[VPL];
+  load_row<VPL, true>(p, t, lane, bias, c);
+  float m = 0.f;
+  if (SOFTMAX) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, c[i]);
+    m = warp_max_float(mx);
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {      // a row that is off as a whole has NaN here, and no expert that is on
+      const float e = exp2_approx((c[i] - m) * kLog2e);
+      z += c[i] > -INFINITY ? e : 0.f;
+      c[i] = c[i] > -INFINITY ? e : -INFINITY;
+    }
+    z = reciprocal_approx(warp_sum(z));
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] *= z;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const float s = reciprocal_approx(1.f + exp2_approx(-c[i] * kLog2e));
+      c[i] = c[i] > -INFINITY ? s : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const float v = fminf(c[i] + bias[i], FLT_MAX);      // where the expert is off: whatever, its logit says so
+    c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
+  }
+  auto near = [&](float hi, float lo) { return !(hi - lo > kTol * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo)))); };
+  if (GROUPS) {
+    float mine = -INFINITY;              // lane g: group g's score
+    auto group_score = [&](int g, float top, float next) {
+      const float first = warp_max_float(top);
+      float sum = first;
+      if (p.group_top == 2) {
+        const unsigned holders = __ballot_sync(kAll, top == first);
+        if (lane == __ffs(holders) - 1) top = next;
+        const float second = warp_max_float(top);
+        if (second > -INFINITY) sum += second;
+      }
+      if (lane == g) mine = sum;
+    };
+    auto by_registers = [&](auto regs) {
+      constexpr int RPG = decltype(regs)::value;
+#pragma unroll
+      for (int g = 0; g * RPG < VPL; ++g) {
+        float top = -INFINITY, next = -INFINITY;
+#pragma unroll
+        for (int i = g * RPG; i < (g + 1) * RPG && i < VPL; ++i) {
+          next = fmaxf(next, fminf(top, c[i]));
+          top = fmaxf(top, c[i]);
+        }
+        group_score(g, top, next);
+      }
+    };
+    // groups of 32, 64 or 128 experts are whole registers: compile-time loops, whose warp-wide maxima overlap
+    if (p.group_size == 32) {
+      by_registers(std::integral_constant<int, 1>());
+    } else if (p.group_size == 64) {
+      by_registers(std::integral_constant<int, 2>());
+    } else if (p.group_size == 128) {
+      by_registers(std::integral_constant<int, 4>());
+    } else {
+      for (int g = 0; g < p.groups; ++g) {
+        float top = -INFINITY, next = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+          const float v = grp[i] == g ? c[i] : -INFINITY;
+          next = fmaxf(next, fminf(top, v));
+          top = fmaxf(top, v);
+        }
+        group_score(g, top, next);
+      }
+    }
+    unsigned chosen = 0;
+    float last = -INFINITY;
+    for (int q = 0; q < p.top_groups; ++q) {
+      const bool open = !((chosen >> lane) & 1);
+      const float best = warp_max_float(open ? mine : -INFINITY);
+      if (best == -INFINITY) break;
+      const unsigned at = __ballot_sync(kAll, open && mine == best);
+      chosen |= at & (0u - at);
+      last = best;
+    }
+    const float out = warp_max_float((chosen >> lane) & 1 ? -INFINITY : mine);
+    if (out > -INFINITY && near(0.5f * last, 0.5f * out)) return true;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] = (chosen >> grp[i]) & 1 ? c[i] : -INFINITY;
+  }
+  // Each lane keeps its DEPTH largest in order; a lane whose DEPTH have all been taken looks for the next ones
+  // below the last taken (rare: of 256 experts' 8 best, 3 share a lane in one row of twenty).
+  constexpr int DEPTH = VPL < 3 ? VPL : 3;
+  float top[DEPTH];
+  auto refill = [&](float below) {
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d) top[d] = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      float v = c[i] < below ? c[i] : -INFINITY;
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        const float lower = fminf(top[d], v);
+        top[d] = fmaxf(top[d], v);
+        v = lower;
+      }
+    }
+  };
+  refill(INFINITY);
+  int taken = 0;
+  float mine = -INFINITY, left_out = -INFINITY;          // lane j: the j-th choice
+  unsigned holder = 0;
+  for (int j = 0; j <= p.k; ++j) {
+    const float best = warp_max_float(top[0]);
+    if (best == -INFINITY) break;
+    if (j == p.k) {
+      left_out = best;
+      break;
+    }
+    const bool hold = top[0] == best;
+    const unsigned who = __ballot_sync(kAll, hold);
+    if (lane == j) mine = best, holder = who;
+    if (hold) {
+#pragma unroll
+      for (int d = 0; d + 1 < DEPTH; ++d) top[d] = top[d + 1];
+      top[DEPTH - 1] = -INFINITY;
+      if (VPL > DEPTH && ++taken == DEPTH) {
+        taken = 0;
+        refill(best);
+      }
+    }
+  }
+  const float up = __shfl_up_sync(kAll, mine, 1);
+  const bool on = mine > -INFINITY;
+  bool bad = on && ((holder & (holder - 1)) != 0 || (lane > 0 && near(up, mine)));
+  if (lane == p.k - 1 && left_out > -INFINITY) bad = bad || near(mine, left_out);
+  if (__any_sync(kAll, bad)) return true;
+  id = on ? (int)(kPlace - (__float_as_uint(mine) & kPlace)) * 32 + __ffs(holder) - 1 : -1;
+  float w = 0.f;
+  if (on) {
+    const int64_t from = t * p.ld + id;
+    float x = p.dtype == 0   ? static_cast<const float*>(p.logits)[from]
+              : p.dtype == 1 ? __half2float(static_cast<const __half*>(p.logits)[from])
+                             : __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[from]);
+    x = fminf(x, FLT_MAX);
+    w = SOFTMAX ? expf(x - m) : 1.f / (1.f + expf(-x));
+  }
+  if (p.renorm) {
+    const float total = warp_sum(w);
+    w = total > 0.f ? w / total : 0.f;
+  }
+  weight = w * p.scale;
+  return false;
+}
+
+template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
+__global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouteArgs p) {
   const int lane = threadIdx.x & 31;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   float bias[VPL];
+  int grp[VPL];
+  load_bias<VPL, BIAS>(p, lane, bias);
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) bias[i] = BIAS && i * 32 + lane < p.E ? p.bias[i * 32 + lane] : 0.f;
+  for (int i = 0; i < VPL; ++i) grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
   for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < p.T; t += warps) {
-    float x[VPL];
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) x[i] = -INFINITY;
-    if (p.dtype == 0) {
-      const float* row = static_cast<const float*>(p.logits) + t * p.ld;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane < p.E) x[i] = row[i * 32 + lane];
-    } else if (p.dtype == 1) {
-      const __half* row = static_cast<const __half*>(p.logits) + t * p.ld;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane < p.E) x[i] = __half2float(row[i * 32 + lane]);
-    } else {
-      const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (i * 32 + lane < p.E) x[i] = __bfloat162float(row[i * 32 + lane]);
-    }
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      x[i] = x[i] > -INFINITY ? fminf(x[i], FLT_MAX) : -INFINITY;       // NaN is off, +inf the largest float
-      if (BIAS && !(bias[i] > -INFINITY)) x[i] = -INFINITY;
-    }
     int id;
     float w;
-    if (route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w))
-      route_row<double, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w);
-    if (lane < p.k) {
-      p.ids[t * p.k + lane] = id;
-      p.weights[t * p.k + lane] = w;
+    bool again;
+    if (BIAS && (!SOFTMAX || p.renorm)) {   // softmax weights as they are want an accurate sum: the other pass
+      again = fast_row<VPL, SOFTMAX, GROUPS>(p, t, lane, bias, grp, id, w);
+    } else {
+      float x[VPL];
+      load_row<VPL, BIAS>(p, t, lane, bias, x);
+      again = route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w);
     }
+    if (again) route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
+    else store_row(p, t, lane, id, w);
   }
 }
 

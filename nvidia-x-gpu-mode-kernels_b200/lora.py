@@ -61,13 +61,10 @@ def lora_add(base, x, a, b, adapters, scales=None, ranks=None, out=None):
     ad = _vector("adapters", adapters, T, torch.int32, dev)
     sc = None if scales is None else _vector("scales", scales, n, torch.float32, dev)
     rk = None if ranks is None else _vector("ranks", ranks, n, torch.int32, dev)
-    l = _lib.lib()
     need = ctypes.c_int64(0)
-    _lib.check(l.nvfp4_lora_workspace(T, r, n, ctypes.byref(need)))
-    with torch.cuda.device(dev):
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        _lib.check(l.nvfp4_lora_add(
-            base.data_ptr(), base.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(), a.stride(1), a.stride(0),
-            b.data_ptr(), b.stride(1), b.stride(0), ad, sc, rk, T, K, N, r, n, out.data_ptr(), out.stride(0),
-            None if ws is None else ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    _lib.check(_lib.lib().nvfp4_lora_workspace(T, r, n, ctypes.byref(need)))
+    ws = base.new_empty(need.value, dtype=torch.uint8) if need.value else None
+    _lib.call("nvfp4_lora_add", dev, base.data_ptr(), base.stride(0), x.data_ptr(), x.stride(0), a.data_ptr(),
+              a.stride(1), a.stride(0), b.data_ptr(), b.stride(1), b.stride(0), ad, sc, rk, T, K, N, r, n,
+              out.data_ptr(), out.stride(0), None if ws is None else ws.data_ptr(), need.value)
     return out

@@ -77,21 +77,19 @@ def moe_mlp(x, ids, weights, w_gate, w_up, w_down, scale_gate, scale_up, scale_d
     sg = _expert_scales("scale_gate", scale_gate, E, F, D, dev)
     su = _expert_scales("scale_up", scale_up, E, F, D, dev)
     sd = _expert_scales("scale_down", scale_down, E, D, F, dev)
-    if w_gate.stride() != w_up.stride() or sg.stride() != su.stride():
+    in_strides = w_gate.stride()
+    if in_strides != w_up.stride() or sg.stride() != su.stride():
         raise ValueError("w_gate and w_up, and their scales, must have the same strides")
     if out is None:
         out = torch.empty((T, D), dtype=torch.float16, device=dev)
     elif not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or tuple(out.shape) != (T, D) \
             or out.stride(1) != 1 or out.device != dev:
         raise ValueError(f"out must be a float16 [{T}, {D}] tensor with unit column stride on the device of x")
-    l = _lib.lib()
     need = ctypes.c_int64(0)
-    _lib.check(l.nvfp4_moe_workspace(T, k, E, D, F, ctypes.byref(need)))
-    with torch.cuda.device(dev):
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev)
-        _lib.check(l.nvfp4_moe_mlp(
-            x.data_ptr(), x.stride(0), ids.data_ptr(), weights.data_ptr(), T, k, E, D, F, w_gate.data_ptr(),
-            w_up.data_ptr(), sg.data_ptr(), su.data_ptr(), w_gate.stride(1), w_gate.stride(0), sg.stride(0),
-            w_down.data_ptr(), sd.data_ptr(), w_down.stride(1), w_down.stride(0), sd.stride(0), out.data_ptr(),
-            out.stride(0), ws.data_ptr(), need.value, torch.cuda.current_stream(dev).cuda_stream))
+    _lib.check(_lib.lib().nvfp4_moe_workspace(T, k, E, D, F, ctypes.byref(need)))
+    ws = x.new_empty(need.value, dtype=torch.uint8)
+    _lib.call("nvfp4_moe_mlp", dev, x.data_ptr(), x.stride(0), ids.data_ptr(), weights.data_ptr(), T, k, E, D, F,
+              w_gate.data_ptr(), w_up.data_ptr(), sg.data_ptr(), su.data_ptr(), in_strides[1], in_strides[0],
+              sg.stride(0), w_down.data_ptr(), sd.data_ptr(), w_down.stride(1), w_down.stride(0), sd.stride(0),
+              out.data_ptr(), out.stride(0), ws.data_ptr(), need.value)
     return out

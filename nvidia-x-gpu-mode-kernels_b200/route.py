@@ -39,16 +39,14 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = 
                              or bias.device != dev or not bias.is_contiguous()):
         raise ValueError(f"bias must be a contiguous float32 tensor [{E}] on the device of logits")
     if weights is None:
-        weights = torch.empty((T, top_k), dtype=torch.float32, device=dev)
+        weights = logits.new_empty((T, top_k), dtype=torch.float32)
     elif weights.dtype != torch.float32 or weights.shape != (T, top_k) or weights.device != dev or not weights.is_contiguous():
         raise ValueError(f"weights must be a contiguous float32 tensor [{T}, {top_k}] on the device of logits")
     if ids is None:
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
+        ids = logits.new_empty((T, top_k), dtype=torch.int32)
     elif ids.dtype != torch.int32 or ids.shape != (T, top_k) or ids.device != dev or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 tensor [{T}, {top_k}] on the device of logits")
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().nvfp4_route_experts(
-            logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0), None if bias is None else bias.data_ptr(),
-            _SCORES[score], top_k, num_groups, top_groups, group_top, int(renormalize), scale, weights.data_ptr(),
-            ids.data_ptr(), torch.cuda.current_stream(dev).cuda_stream))
+    _lib.call("nvfp4_route_experts", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0),
+              None if bias is None else bias.data_ptr(), _SCORES[score], top_k, num_groups, top_groups, group_top,
+              renormalize, scale, weights.data_ptr(), ids.data_ptr())
     return weights, ids
