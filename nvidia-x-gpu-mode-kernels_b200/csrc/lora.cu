@@ -87,10 +87,10 @@ __device__ __forceinline__ uint4 below_rank(uint4 v, int k, int rank) {
   return v;
 }
 
-// out[8 columns] = base + scale * d; `v` holds base where all 8 columns exist and the rows are 16-byte aligned.
+// out[8 columns] = base + scale * d in 16-byte aligned rows; `v` holds base where all 8 columns exist.
 __device__ __forceinline__ void add_eight(const LoraArgs& p, int64_t t, int col, const float (&d)[8], float scale, uint4 v) {
   __half* dst = p.out + t * p.ldo + col;
-  if (p.vec && col + 8 <= p.N) {
+  if (col + 8 <= p.N) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[4];
 #pragma unroll
@@ -127,15 +127,30 @@ __device__ __forceinline__ int cluster_nctas() {
 constexpr int kDecodeTokens = 128;       // most tokens of one call
 static_assert(kDecodeTokens <= kDecodeWarps * 32, "a thread per token");
 
-// RT: 16-row tiles of the largest rank, even.
 template <int RT>
+struct DecodeCfg {
+  static constexpr int R = RT * 16;
+  static constexpr int POOL = kDecodeWarps * (R > 36 ? R : 36) * 8;   // floats
+  static constexpr int smem(int ncta) { return (POOL + ncta * R * 8) * 4; }
+};
+
+// The two halves of a cluster barrier.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(addr), "f"(v) : "memory");
+}
+
+// RT: 16-row tiles of the largest rank, even.  VEC: base and out have 16-byte aligned rows.
+template <int RT, bool VEC>
 __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_kernel(const __grid_constant__ LoraArgs p) {
   constexpr int R = RT * 16, RS = RT / 2;                // RS: 32 ranks a step
   constexpr bool kAhead = RT <= 4;                       // registers for the next step's B
+  extern __shared__ __align__(16) float dynamic[];
   // each warp's share of K, then u, in the end the warps' output patches
-  __shared__ __align__(16) float pool[kDecodeWarps * (R > 36 ? R : 36) * 8];
+  float* const pool = dynamic;
   float(*const part)[R][8] = reinterpret_cast<float(*)[R][8]>(pool);
-  __shared__ float mine[R][8];                           // this CTA's share of K
+  float* const shares = dynamic + DecodeCfg<RT>::POOL;   // every CTA's share of K, [ncta][R][8]
   __shared__ __align__(16) __half hi[8][R + 8], lo[8][R + 8];
   __shared__ float down[8];
   __shared__ int key[kDecodeTokens], items[kDecodeTokens], tok[8], warp_items[kDecodeTokens / 32];
@@ -184,12 +199,27 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
     }
     __syncthreads();
     if (i < 0) {                                         // no adapter: the rows stay what base says
-      for (int j = 0; j < 8 && tok[j] >= 0; ++j)
-        for (int c = glo * 32 + tid; c < min(p.N, ghi * 32); c += blockDim.x)
-          p.out[tok[j] * p.ldo + c] = p.base[tok[j] * p.ld_base + c];
+      const int c0 = glo * 32, cols = min(p.N, ghi * 32) - c0;
+      if (VEC) {
+        const int chunks = (cols + 7) / 8;
+#pragma unroll 4
+        for (int e = tid; e < 8 * chunks; e += blockDim.x) {
+          const int t = tok[e / chunks], c = c0 + e % chunks * 8;
+          if (t < 0) continue;
+          const float zero[8] = {};
+          add_eight(p, t, c, zero, 0.f, c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.base + t * p.ld_base + c) : make_uint4(0, 0, 0, 0));
+        }
+      } else {
+#pragma unroll 8
+        for (int e = tid; e < 8 * cols; e += blockDim.x) {
+          const int t = tok[e / cols], c = c0 + e % cols;
+          if (t >= 0) p.out[t * p.ldo + c] = p.base[t * p.ld_base + c];
+        }
+      }
       __syncthreads();
       continue;
     }
+    cluster_arrive();                                    // this CTA runs, and has read the previous item's shares
     const int rank = lora_rank(p, i);
     const __half* A = p.a + i * p.a_stride;
     const __half* B = p.b + i * p.b_stride;
@@ -201,13 +231,39 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
       for (int64_t o = (int64_t)tid * 128; o < bytes; o += (int64_t)blockDim.x * 128)
         asm volatile("prefetch.global.L2 [%0];" :: "l"(lo_b + o));
     }
+    const int j = lane >> 2, mytok = tok[j];             // this lane's token and columns in the end
+    struct Step {
+      uint4 b[RS][4], base;
+      __half plain[8];                                   // unaligned rows: this lane's column of each token's base
+    };
+    auto ask = [&](int gr, Step& v) {                    // all that a step reads, before any of it is used
+      if (gr >= ghi) return;
+      const int n0 = gr * 32, c = n0 + (lane & 3) * 8;
+      const __half* const from = B + (n0 + g) * p.ldb + 8 * q;
+#pragma unroll
+      for (int s = 0; s < RS; ++s)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          v.b[s][m] = make_uint4(0, 0, 0, 0);
+          if (s * 32 + 8 * q < rank && n0 + m * 8 + g < p.N)
+            v.b[s][m] = *reinterpret_cast<const uint4*>(from + m * 8 * p.ldb + s * 32);
+        }
+      if (VEC) {
+        if (mytok >= 0 && c + 8 <= p.N) v.base = *reinterpret_cast<const uint4*>(p.base + mytok * p.ld_base + c);
+      } else {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+          if (tok[t] >= 0 && n0 + lane < p.N) v.plain[t] = p.base[tok[t] * p.ld_base + n0 + lane];
+      }
+    };
+    Step one, two;
     // ---- u = x . A^T over this CTA's share of K: ranks are the mma's rows, tokens its columns
     {
       float acc[RT][4] = {};
       const int ksteps = (p.K + 31) / 32;
       const int klo = ksteps * me / ncta, khi = ksteps * (me + 1) / ncta;
       const __half* xr = tok[g] >= 0 ? p.x + (int64_t)tok[g] * p.ldx : nullptr;
-#pragma unroll(kAhead ? 2 : 1)
+#pragma unroll(RT <= 2 ? 2 : 1)
       for (int ks = klo + warp; ks < khi; ks += kDecodeWarps) {
         const int k = ks * 32 + q * 8;
         const bool in = k < p.K;                         // K is a multiple of 8
@@ -235,22 +291,25 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
       }
     }
     __syncthreads();
+    // this CTA's share goes to every CTA of the cluster, its own included, once all of them have arrived
+    cluster_wait();
     for (int e = tid; e < R * 8; e += blockDim.x) {
       float s = 0.f;
 #pragma unroll
       for (int w = 0; w < kDecodeWarps; ++w) s += part[w][e >> 3][e & 7];
-      mine[e >> 3][e & 7] = s;
+      const uint32_t there = smem_u32(shares + me * R * 8 + e);
+      for (int c = 0; c < ncta; ++c) st_cluster_f32(mapa(there, c), s);
     }
+    if (kAhead) ask(glo + warp, one);                    // in flight over the exchange
     cluster_sync();
     // every CTA adds all shares in the same order: the same u everywhere
     {
       const float scale = p.scales ? p.scales[i] : 1.f;
       float* const u = pool;
       for (int e = tid; e < R * 8; e += blockDim.x) {
-        const uint32_t here = smem_u32(&mine[e >> 3][e & 7]);
         float s = 0.f;
 #pragma unroll 8
-        for (int c = 0; c < ncta; ++c) s += __uint_as_float(ld_cluster_u32(mapa(here, c)));
+        for (int c = 0; c < ncta; ++c) s += shares[c * R * 8 + e];
         u[e] = s * scale;
       }
       __syncthreads();
@@ -268,7 +327,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
         if (e + lane < R) split_halves(u[(e + lane) * 8 + warp] * up, hi[warp][e + lane], lo[warp][e + lane]);
       if (lane == 0) down[warp] = dn;
     }
-    cluster_sync();    // also: the shares have been read everywhere, and pool is free
+    __syncthreads();
     // ---- out += u . B^T over this CTA's share of N: columns are the mma's rows, tokens its columns
     uint4 uh[RS], ul[RS];
 #pragma unroll
@@ -277,49 +336,21 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
       ul[s] = *reinterpret_cast<const uint4*>(&lo[g][s * 32 + 8 * q]);
     }
     float(*const patch)[36] = reinterpret_cast<float(*)[36]>(pool + warp * 8 * 36);
-    const int j = lane >> 2, mytok = tok[j];             // this lane's token and columns in the end
     const float mydown = down[j];
-    uint4 bv[RS][4], bn[RS][4], basev, basen;
-    auto ask = [&](int gr, uint4 (&v)[RS][4], uint4& base) {   // all that a step reads
-      const int n0 = gr * 32;
-#pragma unroll
-      for (int s = 0; s < RS; ++s)
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          const int col = n0 + m * 8 + g;
-          v[s][m] = make_uint4(0, 0, 0, 0);
-          if (gr < ghi && s * 32 + 8 * q < rank && col < p.N)
-            v[s][m] = *reinterpret_cast<const uint4*>(B + col * p.ldb + s * 32 + 8 * q);
-        }
-      const int c = n0 + (lane & 3) * 8;
-      base = make_uint4(0, 0, 0, 0);
-      if (gr < ghi && p.vec && mytok >= 0 && c + 8 <= p.N)
-        base = *reinterpret_cast<const uint4*>(p.base + mytok * p.ld_base + c);
-    };
-    if (kAhead) ask(glo + warp, bn, basen);
-    for (int gr = glo + warp; gr < ghi; gr += kDecodeWarps) {
-      const int c = gr * 32 + (lane & 3) * 8;
-      if (kAhead) {
-#pragma unroll
-        for (int s = 0; s < RS; ++s)
-#pragma unroll
-          for (int m = 0; m < 4; ++m) bv[s][m] = bn[s][m];
-        basev = basen;
-        ask(gr + kDecodeWarps, bn, basen);
-      } else {
-        ask(gr, bv, basev);
-      }
+    auto add = [&](int gr, Step& v) {
+      if (gr >= ghi) return;
+      const int n0 = gr * 32, c = n0 + (lane & 3) * 8;
       float acc[2][4] = {};
 #pragma unroll
       for (int s = 0; s < RS; ++s) {
         if (s * 32 >= rank) break;
         if (rank & 7) {
 #pragma unroll
-          for (int m = 0; m < 4; ++m) bv[s][m] = below_rank(bv[s][m], s * 32 + 8 * q, rank);
+          for (int m = 0; m < 4; ++m) v.b[s][m] = below_rank(v.b[s][m], s * 32 + 8 * q, rank);
         }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const uint4 b0 = bv[s][2 * m], b1 = bv[s][2 * m + 1];
+          const uint4 b0 = v.b[s][2 * m], b1 = v.b[s][2 * m + 1];
           mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, uh[s].x, uh[s].y);
           mma_16816(acc[m], b0.x, b1.x, b0.y, b1.y, ul[s].x, ul[s].y);
           mma_16816(acc[m], b0.z, b1.z, b0.w, b1.w, uh[s].z, uh[s].w);
@@ -335,13 +366,33 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
         patch[2 * q + 1][m * 16 + g + 8] = acc[m][3];
       }
       __syncwarp();
-      if (mytok >= 0 && c < p.N) {
-        float d[8];
+      if (VEC) {
+        if (mytok >= 0 && c < p.N) {
+          const float4 d0 = *reinterpret_cast<const float4*>(&patch[j][(lane & 3) * 8]);
+          const float4 d1 = *reinterpret_cast<const float4*>(&patch[j][(lane & 3) * 8 + 4]);
+          const float d[8] = {d0.x, d0.y, d0.z, d0.w, d1.x, d1.y, d1.z, d1.w};
+          add_eight(p, mytok, c, d, mydown, v.base);
+        }
+      } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = patch[j][(lane & 3) * 8 + e];
-        add_eight(p, mytok, c, d, mydown, basev);
+        for (int t = 0; t < 8; ++t)
+          if (tok[t] >= 0 && n0 + lane < p.N)
+            p.out[tok[t] * p.ldo + n0 + lane] = __float2half_rn(fmaf(patch[t][lane], down[t], __half2float(v.plain[t])));
       }
       __syncwarp();
+    };
+    if (kAhead) {
+      for (int gr = glo + warp; gr < ghi; gr += 2 * kDecodeWarps) {
+        ask(gr + kDecodeWarps, two);
+        add(gr, one);
+        ask(gr + 2 * kDecodeWarps, one);
+        add(gr + kDecodeWarps, two);
+      }
+    } else {
+      for (int gr = glo + warp; gr < ghi; gr += kDecodeWarps) {
+        ask(gr, one);
+        add(gr, one);
+      }
     }
     __syncthreads();                                     // pool, tok and down are reused
   }
@@ -350,7 +401,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
 // ------------------------------------------------------------------ many tokens
 
 constexpr int kTile = 128;               // tokens per tile of the plan
-constexpr int kShrinkTokens = 64;        // tokens per CTA of the first product
+constexpr int kShrinkTokens = 32;        // tokens per CTA of the first product
 constexpr int kShrinkK = 128;            // elements of K per stage
 constexpr int kShrinkStages = 3;
 constexpr int kExpandCols = 64;          // columns per step of the second product
@@ -376,21 +427,21 @@ struct LoraCfg {
   static constexpr int LDK = padded_row(kShrinkK), LDR = padded_row(R);
   static constexpr int SHRINK_STAGE = (kShrinkTokens + R) * LDK * 2;
   static constexpr int SHRINK_SMEM = kShrinkStages * SHRINK_STAGE;
-  static_assert(SHRINK_SMEM >= 2 * kShrinkTokens * R * 4, "the two halves of u");
+  static_assert(SHRINK_SMEM >= 4 * kShrinkTokens * R * 4, "the four shares of u");
   static constexpr int EXPAND_B = kExpandCols * LDR * 2;
   static constexpr int EXPAND_BASE = 8 * 4 * 512;        // a warp's 16 tokens x 64 columns, 4 pieces a lane
   static constexpr int EXPAND_SMEM = kExpandStages * (EXPAND_B + EXPAND_BASE);
 };
 
-// u of 64 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
-// of 128-element stages; four warps take 16 tokens each over the first half of a stage, four over the second.
+// u of 32 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
+// of 128-element stages; two warps take 16 tokens each over each quarter of a stage.
 template <int RT>
 __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
   using C = LoraCfg<RT>;
   constexpr int R = C::R, NT = RT * 2, PER = kTile / kShrinkTokens, LD = C::LDK, CHUNKS = kShrinkK / 8;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int m0 = (warp & 3) * 16, khalf = (warp >> 2) * (kShrinkK / 2);
+  const int m0 = (warp & 1) * 16, share = warp >> 1;     // of kShrinkK: 32 elements, two mma's
   griddep_launch();
   griddep_wait();
   const int total = *w.ntiles * PER;
@@ -438,26 +489,25 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
       __syncthreads();                                   // stage ks is here, stage ks - 1 free
       ask(ks + kShrinkStages - 1);
       const __half* const st = reinterpret_cast<const __half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
-      const __half* const xs = st + (m0 + g) * LD + khalf + 8 * q;
-      const __half* const as = st + (kShrinkTokens + g) * LD + khalf + 8 * q;
+      const __half* const xs = st + (m0 + g) * LD + share * 32 + 8 * q;
+      const __half* const as = st + (kShrinkTokens + g) * LD + share * 32 + 8 * q;
+      const uint4 x0 = *reinterpret_cast<const uint4*>(xs), x1 = *reinterpret_cast<const uint4*>(xs + 8 * LD);
 #pragma unroll
-      for (int s = 0; s < kShrinkK / 64; ++s) {
-        const uint4 x0 = *reinterpret_cast<const uint4*>(xs + s * 32), x1 = *reinterpret_cast<const uint4*>(xs + 8 * LD + s * 32);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          if (nt * 8 >= rank) break;
-          const uint4 a = *reinterpret_cast<const uint4*>(as + nt * 8 * LD + s * 32);
-          mma_16816(acc[nt], x0.x, x1.x, x0.y, x1.y, a.x, a.y);
-          mma_16816(acc[nt], x0.z, x1.z, x0.w, x1.w, a.z, a.w);
-        }
+      for (int nt = 0; nt < NT; nt += 2) {
+        if (nt * 8 >= rank) break;
+        const uint4 a0 = *reinterpret_cast<const uint4*>(as + nt * 8 * LD), a1 = *reinterpret_cast<const uint4*>(as + (nt + 1) * 8 * LD);
+        mma_16816(acc[nt], x0.x, x1.x, x0.y, x1.y, a0.x, a0.y);
+        mma_16816(acc[nt + 1], x0.x, x1.x, x0.y, x1.y, a1.x, a1.y);
+        mma_16816(acc[nt], x0.z, x1.z, x0.w, x1.w, a0.z, a0.w);
+        mma_16816(acc[nt + 1], x0.z, x1.z, x0.w, x1.w, a1.z, a1.w);
       }
     }
     cp_async_wait<0>();
     __syncthreads();
-    float* const part = reinterpret_cast<float*>(smem);  // [half of K][64 tokens][R]
+    float* const part = reinterpret_cast<float*>(smem);  // [quarter of K][32 tokens][R]
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float* at = part + ((warp >> 2) * kShrinkTokens + m0 + g) * R + nt * 8 + 2 * q;
+      float* at = part + (share * kShrinkTokens + m0 + g) * R + nt * 8 + 2 * q;
       *reinterpret_cast<float2*>(at) = make_float2(acc[nt][0], acc[nt][1]);
       *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[nt][2], acc[nt][3]);
     }
@@ -469,7 +519,7 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
 #pragma unroll
       for (int e = 0; e < R / 32; ++e) {
         const float* at = part + t * R + e * 32 + lane;
-        u[e] = (at[0] + at[kShrinkTokens * R]) * scale;
+        u[e] = (at[0] + at[kShrinkTokens * R] + at[2 * kShrinkTokens * R] + at[3 * kShrinkTokens * R]) * scale;
         m = fmaxf(m, fabsf(u[e]));
       }
 #pragma unroll
@@ -494,14 +544,19 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
 // which each lane reads back just what it asked for itself.
 // The 8 columns of mma tile j of four stand for columns 8 (c / 2) + 2 j + c % 2 of 32, so that the four tiles
 // give a lane 8 consecutive columns of a token.
-template <int RT>
+template <int RT, bool VEC>
 __global__ void __launch_bounds__(kLoraThreads, 2)
     expand_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
   using C = LoraCfg<RT>;
   constexpr int R = C::R, LD = C::LDR, RS = RT / 2, CHUNKS = R / 8;
+  constexpr int BROWS = kLoraThreads / CHUNKS;           // rows of B that the CTA copies in one go
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   uint8_t* const bases = smem + kExpandStages * C::EXPAND_B + warp * 2048 + lane * 16;
+  // this thread's piece of each BROWS rows of B, and where this lane reads B
+  const int bc = tid / CHUNKS, bk = tid % CHUNKS * 8;
+  __half* const bput = reinterpret_cast<__half*>(smem) + bc * LD + bk;
+  const __half* const bget = reinterpret_cast<const __half*>(smem) + (8 * (g >> 1) + (g & 1)) * LD + 8 * q;
   griddep_launch();
   griddep_wait();
   // all steps of all tiles in one row, an equal run of them for each CTA
@@ -517,14 +572,19 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     const int row0 = tile.row0 + tr + warp * 16;
     const bool none = tile.index >= p.n, live = tr + warp * 16 < tile.rows;
     const int rank = none ? 0 : lora_rank(p, tile.index);
-    const __half* const B = none ? p.b : p.b + tile.index * p.b_stride;
+    const __half* bsrc = none ? p.b : p.b + tile.index * p.b_stride + (int64_t)(lo * kExpandCols + bc) * p.ldb + bk;
+    const bool bmine = bk < rank;                        // else zeros
     int tok[2];
     float down[2];
+    const __half* src[2];                                // this lane's columns of its tokens' rows, at step lo
+    __half* dst[2];
     uint4 u[2][2][RS];                                   // [hi, lo][row g, g + 8][step]
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       tok[h] = live ? w.slot[row0 + h * 8 + g] : -1;
       down[h] = tok[h] >= 0 && !none ? w.down[row0 + h * 8 + g] : 0.f;
+      src[h] = p.base + (int64_t)max(tok[h], 0) * p.ld_base + lo * kExpandCols + 8 * q;
+      dst[h] = p.out + (int64_t)max(tok[h], 0) * p.ldo + lo * kExpandCols + 8 * q;
 #pragma unroll
       for (int s = 0; s < RS; ++s) {
         u[0][h][s] = u[1][h][s] = make_uint4(0, 0, 0, 0);
@@ -535,67 +595,113 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
         }
       }
     }
-    auto ask = [&](int st) {
-      if (st < hi) {
-        const int ring = (st - lo) % kExpandStages;
-        __half* const bs = reinterpret_cast<__half*>(smem + ring * C::EXPAND_B);
-        const int n0 = st * kExpandCols;
+    int ring_in = 0, ahead = 0;                          // next ring to fill, its distance from lo in steps
+    auto ask = [&]() {
+      if (lo + ahead < hi) {
+        const int n0 = (lo + ahead) * kExpandCols;
         if (rank > 0) {
 #pragma unroll
-          for (int e = tid; e < kExpandCols * CHUNKS; e += kLoraThreads) {
-            const int c = e / CHUNKS, k = e % CHUNKS * 8;
-            const bool in = n0 + c < p.N && k < rank;
-            cp_async_16(bs + c * LD + k, in ? B + (n0 + c) * p.ldb + k : p.b, in);
+          for (int e = 0; e < kExpandCols / BROWS; ++e) {
+            const bool in = bmine && n0 + bc + e * BROWS < p.N;
+            cp_async_16(bput + ring_in * (C::EXPAND_B / 2) + e * BROWS * LD, in ? bsrc + e * BROWS * p.ldb : p.b, in);
           }
+          bsrc += kExpandCols * p.ldb;
         }
-        if (p.vec) {
+        if (VEC) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {                  // [column half][row half]
-            const int col = n0 + (e >> 1) * 32 + 8 * q;
-            if (tok[e & 1] >= 0 && col + 8 <= p.N)
-              cp_async_16(bases + ring * C::EXPAND_BASE + e * 512, p.base + tok[e & 1] * p.ld_base + col, true);
+            if (tok[e & 1] >= 0 && n0 + (e >> 1) * 32 + 8 * q + 8 <= p.N)
+              cp_async_16(bases + ring_in * C::EXPAND_BASE + e * 512, src[e & 1] + ahead * kExpandCols + (e >> 1) * 32, true);
           }
         }
+        ring_in = ring_in + 1 == kExpandStages ? 0 : ring_in + 1;
+        ++ahead;
       }
       cp_async_commit();
     };
-    __syncthreads();                                     // the previous item's ring is read
+    __syncthreads();                                     // the previous run's ring is read
 #pragma unroll
-    for (int s = 0; s < kExpandStages - 1; ++s) ask(lo + s);
+    for (int s = 0; s < kExpandStages - 1; ++s) ask();
+    int ring = 0;
     for (int st = lo; st < hi; ++st) {
       cp_async_wait<kExpandStages - 2>();
       __syncthreads();                                   // step st is here, step st - 1's ring free
-      ask(st + kExpandStages - 1);
-      const int ring = (st - lo) % kExpandStages;
-      const __half* const bs = reinterpret_cast<const __half*>(smem + ring * C::EXPAND_B) + (8 * (g >> 1) + (g & 1)) * LD + 8 * q;
-      if (!live) continue;
+      ask();
+      if (live) {
+        const __half* const bs = bget + ring * (C::EXPAND_B / 2);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        float acc[4][4] = {};
+        for (int half = 0; half < 2; ++half) {
+          const int n0 = st * kExpandCols + half * 32, col = n0 + 8 * q, off = (st - lo) * kExpandCols + half * 32;
+          __half plain[16];                              // !VEC: base of this lane's column for the 16 tokens
+          if (!VEC) {
 #pragma unroll
-        for (int s = 0; s < RS; ++s) {
-          if (s * 32 >= rank) break;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint4 b = *reinterpret_cast<const uint4*>(bs + (half * 32 + 2 * j) * LD + s * 32);
-            if (rank & 7) b = below_rank(b, s * 32 + 8 * q, rank);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              mma_16816(acc[j], u[h][0][s].x, u[h][1][s].x, u[h][0][s].y, u[h][1][s].y, b.x, b.y);
-              mma_16816(acc[j], u[h][0][s].z, u[h][1][s].z, u[h][0][s].w, u[h][1][s].w, b.z, b.w);
+            for (int t = 0; t < 16; ++t) {
+              const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
+              plain[t] = tk >= 0 && n0 + lane < p.N ? p.base[tk * p.ld_base + n0 + lane] : __float2half_rn(0.f);
             }
           }
-        }
-        const int col = st * kExpandCols + half * 32 + 8 * q;
+          float acc[4][4] = {};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (tok[h] < 0 || col >= p.N) continue;
-          float d[8];
+          for (int s = 0; s < RS; ++s) {
+            if (s * 32 >= rank) break;
+            uint4 b[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) d[2 * j] = acc[j][2 * h], d[2 * j + 1] = acc[j][2 * h + 1];
-          add_eight(p, tok[h], col, d, down[h], *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512));
+            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint4*>(bs + (half * 32 + 2 * j) * LD + s * 32);
+            if (rank & 7) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) b[j] = below_rank(b[j], s * 32 + 8 * q, rank);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {                // neighbouring mma's add to different accumulators
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u[h][0][s].x, u[h][1][s].x, u[h][0][s].y, u[h][1][s].y, b[j].x, b[j].y);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u[h][0][s].z, u[h][1][s].z, u[h][0][s].w, u[h][1][s].w, b[j].z, b[j].w);
+            }
+          }
+          if (VEC) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (tok[h] < 0) continue;
+              if (col + 8 <= p.N) {
+                const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
+                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
+                  const __half2 r = __floats2half2_rn(fmaf(acc[j][2 * h], down[h], f.x), fmaf(acc[j][2 * h + 1], down[h], f.y));
+                  o[j] = *reinterpret_cast<const uint32_t*>(&r);
+                }
+                *reinterpret_cast<uint4*>(dst[h] + off) = make_uint4(o[0], o[1], o[2], o[3]);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (col + e < p.N)
+                    dst[h][off + e] = __float2half_rn(fmaf(acc[e >> 1][2 * h + (e & 1)], down[h], __half2float(src[h][off + e])));
+              }
+            }
+          } else {
+            // rows of any alignment: through a patch of [16 tokens][32 columns], a lane a column
+            float* const patch = reinterpret_cast<float*>(smem + kExpandStages * C::EXPAND_B + warp * 2048);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                *reinterpret_cast<float2*>(patch + (h * 8 + g) * 32 + 8 * q + 2 * j) =
+                    make_float2(acc[j][2 * h] * down[h], acc[j][2 * h + 1] * down[h]);
+            __syncwarp();
+#pragma unroll
+            for (int t = 0; t < 16; ++t) {
+              const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
+              if (tk >= 0 && n0 + lane < p.N)
+                p.out[tk * p.ldo + n0 + lane] = __float2half_rn(__half2float(plain[t]) + patch[t * 32 + lane]);
+            }
+            __syncwarp();
+          }
         }
       }
+      ring = ring + 1 == kExpandStages ? 0 : ring + 1;
     }
     cp_async_wait<0>();
   }
@@ -657,24 +763,34 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(16));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(16));
     if (e == cudaSuccess) {
       int fit = 0;
       cfg.gridDim = dim3(16);
-      wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT>, &cfg) == cudaSuccess && fit > 0;
+      cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(16);
+      wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT, true>, &cfg) == cudaSuccess && fit > 0;
       cudaGetLastError();
       e = cudaFuncSetAttribute(shrink_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHRINK_SMEM);
     }
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(expand_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
+      e = cudaFuncSetAttribute(expand_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(expand_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(low-rank products)");
     attr_set[dev] = true;
   }
   if (p.T <= kDecodeTokens) {
     const int ncta = p.T <= 4 && wide[dev] ? 16 : 8;
     attr[0].val.clusterDim.x = (unsigned)ncta;
+    cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(ncta);
     cfg.gridDim = dim3((unsigned)(std::min(p.T, std::max(1, sm_count() * 2 / ncta)) * ncta));
-    cudaError_t e = cudaLaunchKernelEx(&cfg, decode_kernel<RT>, p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, p.vec ? decode_kernel<RT, true> : decode_kernel<RT, false>, p);
     return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaLaunchKernelEx(decode)");
   }
   const Plan plan = {reinterpret_cast<int*>(ws), reinterpret_cast<PlanTile*>(ws + m.tiles),
@@ -689,7 +805,7 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
                          kLoraThreads, C::SHRINK_SMEM, stream, p, rows)))
     return rc;
   const int64_t steps = (p.N + kExpandCols - 1) / kExpandCols;
-  return launch_after(expand_kernel<RT>, "expand_kernel",
+  return launch_after(p.vec ? expand_kernel<RT, true> : expand_kernel<RT, false>, "expand_kernel",
                       (unsigned)std::min<int64_t>(m.max_tiles * ((steps + 3) / 4), (int64_t)sm_count() * 2), kLoraThreads,
                       C::EXPAND_SMEM, stream, p, rows);
 }

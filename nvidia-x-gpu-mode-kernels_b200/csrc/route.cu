@@ -288,28 +288,40 @@ __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float
   return false;
 }
 
-// Row t's logits (expert i * 32 + lane): -inf where the expert is off, at most the largest float.
-template <int VPL, bool BIAS>
-__device__ __forceinline__ void load_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
-                                         float (&x)[VPL]) {
+// Row t's logits as they are, expert i * 32 + lane in x[i]; -inf past the last expert.
+template <int VPL>
+__device__ __forceinline__ void load_raw(const RouteArgs& p, int64_t t, int lane, float (&x)[VPL]) {
+  const bool full = p.E == VPL * 32;
 #pragma unroll
   for (int i = 0; i < VPL; ++i) x[i] = -INFINITY;
   if (p.dtype == 0) {
-    const float* row = static_cast<const float*>(p.logits) + t * p.ld;
+    const float* row = static_cast<const float*>(p.logits) + t * p.ld + lane;
+    if (full) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (i * 32 + lane < p.E) x[i] = row[i * 32 + lane];
+      for (int i = 0; i < VPL; ++i) x[i] = row[i * 32];
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (i * 32 + lane < p.E) x[i] = row[i * 32];
+    }
   } else if (p.dtype == 1) {
-    const __half* row = static_cast<const __half*>(p.logits) + t * p.ld;
+    const __half* row = static_cast<const __half*>(p.logits) + t * p.ld + lane;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (i * 32 + lane < p.E) x[i] = __half2float(row[i * 32 + lane]);
+      if (i * 32 + lane < p.E) x[i] = __half2float(row[i * 32]);
   } else {
-    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld;
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.logits) + t * p.ld + lane;
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
-      if (i * 32 + lane < p.E) x[i] = __bfloat162float(row[i * 32 + lane]);
+      if (i * 32 + lane < p.E) x[i] = __bfloat162float(row[i * 32]);
   }
+}
+
+// The same, -inf where the expert is off, at most the largest float.
+template <int VPL, bool BIAS>
+__device__ __forceinline__ void load_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
+                                         float (&x)[VPL]) {
+  load_raw<VPL>(p, t, lane, x);
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     x[i] = x[i] > -INFINITY ? fminf(x[i], FLT_MAX) : -INFINITY;       // NaN is off
@@ -322,7 +334,7 @@ __device__ __forceinline__ void load_bias(const RouteArgs& p, int lane, float (&
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     bias[i] = BIAS && i * 32 + lane < p.E ? p.bias[i * 32 + lane] : 0.f;
-    if (!(bias[i] > -INFINITY)) bias[i] = -INFINITY;     // NaN: off, too
+    bias[i] = bias[i] > -INFINITY ? bias[i] : -INFINITY;     // NaN: off, too
   }
 }
 
@@ -373,9 +385,9 @@ __device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane
   constexpr uint32_t kPlace = VPL - 1;
   constexpr float kTol = 4e-6f + 2 * VPL * 1.2e-7f;
   float c[VPL];
-  load_row<VPL, true>(p, t, lane, bias, c);
   float m = 0.f;
   if (SOFTMAX) {
+    load_row<VPL, true>(p, t, lane, bias, c);
     float mx = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, c[i]);
@@ -390,17 +402,18 @@ __device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane
     z = reciprocal_approx(warp_sum(z));
 #pragma unroll
     for (int i = 0; i < VPL; ++i) c[i] *= z;
-  } else {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const float s = reciprocal_approx(1.f + exp2_approx(-c[i] * kLog2e));
-      c[i] = c[i] > -INFINITY ? s : -INFINITY;
+      const float v = c[i] + bias[i];
+      c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
     }
-  }
+  } else {
+    load_raw<VPL>(p, t, lane, c);
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    const float v = fminf(c[i] + bias[i], FLT_MAX);      // where the expert is off: whatever, its logit says so
-    c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
+    for (int i = 0; i < VPL; ++i) {      // a logit of +inf scores 1, NaN fails both comparisons
+      const float v = reciprocal_approx(1.f + exp2_approx(c[i] * -kLog2e)) + bias[i];
+      c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
+    }
   }
   auto near = [&](float hi, float lo) { return !(hi - lo > kTol * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo)))); };
   if (GROUPS) {
@@ -535,6 +548,8 @@ __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ Rout
   float bias[VPL];
   int grp[VPL];
   load_bias<VPL, BIAS>(p, lane, bias);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) bias[i] = fminf(bias[i], FLT_MAX);   // the 64-bit pass tells it from +inf
 #pragma unroll
   for (int i = 0; i < VPL; ++i) grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
   for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < p.T; t += warps) {
