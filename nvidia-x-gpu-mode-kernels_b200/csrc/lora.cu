@@ -8,8 +8,8 @@
 //
 // The products run on mma.sync (fp16 operands, fp32 accumulators): with ranks of 16 to 128 there is too
 // little arithmetic per byte for tensor memory and its round trips to pay.  u = x . A^T enters the second
-// product as two fp16 halves, u = 2^-p (hi + lo), 2^p bringing the token's largest |u| to 2^14: 22 bits of
-// u survive, whatever its range, and the sum stays in fp32.
+// product as two fp16 halves, u = 2^-p (hi + lo), with a 2^p per token that keeps them in fp16's range: 22 bits of
+// the token's largest |u| survive, and the sum stays in fp32.
 //
 // The k index of an mma is summed over, so its 16 slots may stand for any 16 elements as long as both operands
 // agree.  Two mma's take 32 elements, slots {2q, 2q+1, 2q+8, 2q+9} of lane q of 4 standing for elements 8q..8q+3 in
@@ -60,11 +60,13 @@ __device__ __forceinline__ int lora_rank(const LoraArgs& p, int i) {
   return p.ranks ? max(0, min(p.ranks[i], p.r)) : p.r;
 }
 
-// The power of two that brings magnitude m to [2^14, 2^15), and its inverse.
+// A power of two under which two halves hold 22 bits of every u up to magnitude m, and its inverse: 1 where m is
+// in [2^-2, 2^15), so that most tokens need no scaling, else what brings m to [2^14, 2^15).  At most 2^110: base
+// times it stays finite.
 __device__ __forceinline__ void half_scale(float m, float& up, float& down) {
   int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-  if (m == 0.f || e == 128) e = 14;                      // nothing to bring up, or infinite already
-  const int q = min(14 - e, 126);
+  if (m == 0.f || e == 128 || (e >= -2 && e < 14)) e = 14;   // nothing to bring up, infinite already, or fine
+  const int q = min(14 - e, 110);
   up = __uint_as_float((uint32_t)(q + 127) << 23);
   down = __uint_as_float((uint32_t)(127 - q) << 23);
 }
@@ -412,10 +414,19 @@ struct LoraRows {
   const int* ntiles;
   const PlanTile* tiles;
   const int* slot;                       // token of each row, -1 for padding
-  __half* hi;                            // [rows][R], R = r rounded up to 32, 64 or 128
+  __half* hi;                            // [rows][R], R = r rounded up to 32, 64 or 128, laid out by u_at
   __half* lo;
   float* down;                           // [rows]
 };
+
+// Where u of (row, rank index k) lies: in blocks of 16 rows x 16 k, the 4 registers of an mma's first operand of
+// each lane together.  Two neighbouring blocks hold 32 k, of which lane q of 4 has 8q..8q+3 and 8q+4..8q+7.
+template <int R>
+__device__ __forceinline__ int64_t u_at(int64_t row, int k) {
+  const int64_t block = row / 16 * (R / 16) + k / 32 * 2 + k % 8 / 4;
+  const int lane = (int)(row % 8) * 4 + k % 32 / 8, reg = k % 4 / 2 * 2 + (int)(row % 16) / 8;
+  return (block * 32 + lane) * 8 + reg * 2 + k % 2;
+}
 
 // Row length in halves of a tile in shared memory that is read 16 bytes a lane, two neighbouring rows of 4 lanes
 // at a time: rows 16 words apart modulo the 32 banks.
@@ -531,8 +542,8 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
       for (int e = 0; e < R / 32; ++e) {
         __half h, l;
         split_halves(u[e] * up, h, l);
-        w.hi[row * R + e * 32 + lane] = h;
-        w.lo[row * R + e * 32 + lane] = l;
+        w.hi[u_at<R>(row, e * 32 + lane)] = h;
+        w.lo[u_at<R>(row, e * 32 + lane)] = l;
       }
       if (lane == 0) w.down[row] = dn;
     }
@@ -578,23 +589,24 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
     float down[2];
     const __half* src[2];                                // this lane's columns of its tokens' rows, at step lo
     __half* dst[2];
-    uint4 u[2][2][RS];                                   // [hi, lo][row g, g + 8][step]
+    uint4 u[2][2 * RS];                                  // [hi, lo][16 ranks]: first operands of the mma's
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       tok[h] = live ? w.slot[row0 + h * 8 + g] : -1;
-      down[h] = tok[h] >= 0 && !none ? w.down[row0 + h * 8 + g] : 0.f;
+      down[h] = tok[h] >= 0 && !none ? w.down[row0 + h * 8 + g] : 1.f;
       src[h] = p.base + (int64_t)max(tok[h], 0) * p.ld_base + lo * kExpandCols + 8 * q;
       dst[h] = p.out + (int64_t)max(tok[h], 0) * p.ldo + lo * kExpandCols + 8 * q;
+    }
 #pragma unroll
-      for (int s = 0; s < RS; ++s) {
-        u[0][h][s] = u[1][h][s] = make_uint4(0, 0, 0, 0);
-        if (s * 32 < rank && live) {
-          const int64_t from = (int64_t)(row0 + h * 8 + g) * R + s * 32 + 8 * q;
-          u[0][h][s] = *reinterpret_cast<const uint4*>(w.hi + from);
-          u[1][h][s] = *reinterpret_cast<const uint4*>(w.lo + from);
-        }
+    for (int s = 0; s < 2 * RS; ++s) {
+      u[0][s] = u[1][s] = make_uint4(0, 0, 0, 0);
+      if (s / 2 * 32 < rank && live) {
+        const int64_t from = ((int64_t)(row0 / 16) * (2 * RS) + s) * 32 + lane;
+        u[0][s] = reinterpret_cast<const uint4*>(w.hi)[from];
+        u[1][s] = reinterpret_cast<const uint4*>(w.lo)[from];
       }
     }
+    const bool unit = __all_sync(0xffffffffu, down[0] == 1.f && down[1] == 1.f);
     int ring_in = 0, ahead = 0;                          // next ring to fill, its distance from lo in steps
     auto ask = [&]() {
       if (lo + ahead < hi) {
@@ -640,7 +652,30 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
               plain[t] = tk >= 0 && n0 + lane < p.N ? p.base[tk * p.ld_base + n0 + lane] : __float2half_rn(0.f);
             }
           }
+          // VEC: the sums start from base (times 2^p)
           float acc[4][4] = {};
+          const bool whole = col + 8 <= p.N;
+          if (VEC) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
+              const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
+                if (!whole) f = make_float2(col + 2 * j < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j]) : 0.f,
+                                            col + 2 * j + 1 < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j + 1]) : 0.f);
+                acc[j][2 * h] = f.x;
+                acc[j][2 * h + 1] = f.y;
+              }
+            }
+            if (!unit) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j][e] *= 1.f / down[e >> 1];     // a power of two: exact
+            }
+          }
 #pragma unroll
           for (int s = 0; s < RS; ++s) {
             if (s * 32 >= rank) break;
@@ -653,32 +688,35 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {                // neighbouring mma's add to different accumulators
+              const uint4 u0 = u[h][2 * s], u1 = u[h][2 * s + 1];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u[h][0][s].x, u[h][1][s].x, u[h][0][s].y, u[h][1][s].y, b[j].x, b[j].y);
+              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u0.x, u0.y, u0.z, u0.w, b[j].x, b[j].y);
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u[h][0][s].z, u[h][1][s].z, u[h][0][s].w, u[h][1][s].w, b[j].z, b[j].w);
+              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u1.x, u1.y, u1.z, u1.w, b[j].z, b[j].w);
             }
           }
           if (VEC) {
+            if (!unit) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j][e] *= down[e >> 1];
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               if (tok[h] < 0) continue;
-              if (col + 8 <= p.N) {
-                const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
-                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
+              if (whole) {
                 uint32_t o[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
-                  const __half2 r = __floats2half2_rn(fmaf(acc[j][2 * h], down[h], f.x), fmaf(acc[j][2 * h + 1], down[h], f.y));
+                  const __half2 r = __floats2half2_rn(acc[j][2 * h], acc[j][2 * h + 1]);
                   o[j] = *reinterpret_cast<const uint32_t*>(&r);
                 }
                 *reinterpret_cast<uint4*>(dst[h] + off) = make_uint4(o[0], o[1], o[2], o[3]);
               } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  if (col + e < p.N)
-                    dst[h][off + e] = __float2half_rn(fmaf(acc[e >> 1][2 * h + (e & 1)], down[h], __half2float(src[h][off + e])));
+                  if (col + e < p.N) dst[h][off + e] = __float2half_rn(acc[e >> 1][2 * h + (e & 1)]);
               }
             }
           } else {

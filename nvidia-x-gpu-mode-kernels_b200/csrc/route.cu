@@ -377,70 +377,113 @@ __device__ __forceinline__ float reciprocal_approx(float v) {
 // The 32-bit pass over a row with a bias, where every choice is approximate anyway: floats instead of keys
 // (-inf: off), and the lowest bits of a choice replaced by its place in the lane, so that a lane's choices
 // differ and carry their index.  That moves a choice by less than VPL units of 2^-23 relative.  grp: each
-// expert's group.  Returns true where a comparison is too near: the row then needs the 64-bit pass.
-template <int VPL, bool SOFTMAX, bool GROUPS>
-__device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
-                                         const int (&grp)[VPL], int& id, float& weight) {
+// expert's group.
+//
+// The pass is bound by comparisons and selections (the ALU pipe, half the rate of the others), so the
+// common row takes the form that has few of them (CAREFUL false, kOdd where it will not do): no expert off or
+// below a logit of -88, group's and lane's maxima without ties, no lane with more than DEPTH of the k best.
+enum RowState { kDone, kOdd, kNear };   // kNear: a comparison is too near, the row needs the 64-bit pass
+
+template <int VPL, bool SOFTMAX, bool GROUPS, bool CAREFUL>
+__device__ __forceinline__ RowState fast_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
+                                             const int (&grp)[VPL], float2* slots, int& id, float& weight) {
   constexpr float kLog2e = 1.4426950408889634f;
   constexpr uint32_t kPlace = VPL - 1;
   constexpr float kTol = 4e-6f + 2 * VPL * 1.2e-7f;
   float c[VPL];
   float m = 0.f;
-  if (SOFTMAX) {
-    load_row<VPL, true>(p, t, lane, bias, c);
-    float mx = -INFINITY;
+  load_raw<VPL>(p, t, lane, c);
+  if (CAREFUL) {
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) mx = fmaxf(mx, c[i]);
+    for (int i = 0; i < VPL; ++i) c[i] = c[i] > -INFINITY && bias[i] > -INFINITY ? fminf(c[i], FLT_MAX) : -INFINITY;
+  }
+  if (SOFTMAX) {
+    float mx = c[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) mx = fmaxf(mx, c[i]);
     m = warp_max_float(mx);
     float z = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {      // a row that is off as a whole has NaN here, and no expert that is on
       const float e = exp2_approx((c[i] - m) * kLog2e);
-      z += c[i] > -INFINITY ? e : 0.f;
-      c[i] = c[i] > -INFINITY ? e : -INFINITY;
+      if (CAREFUL) {
+        z += c[i] > -INFINITY ? e : 0.f;
+        c[i] = c[i] > -INFINITY ? e : -INFINITY;
+      } else {
+        // NaN from a logit of NaN or an infinity, 1/0 * 0 from one too far below (their exponential is 0)
+        z += e;
+        c[i] = fmaf(reciprocal_approx(e), 0.f, e);
+      }
     }
     z = reciprocal_approx(warp_sum(z));
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] *= z;
+    for (int i = 0; i < VPL; ++i) c[i] = fmaf(c[i], z, bias[i]);
+  } else {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const float v = c[i] + bias[i];
-      c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
-    }
-  } else {
-    load_raw<VPL>(p, t, lane, c);
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) {      // a logit of +inf scores 1, NaN fails both comparisons
-      const float v = reciprocal_approx(1.f + exp2_approx(c[i] * -kLog2e)) + bias[i];
-      c[i] = c[i] > -INFINITY && v > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
+      const float e = exp2_approx(c[i] * -kLog2e);
+      const float v = reciprocal_approx(1.f + e) + bias[i];
+      // NaN from a logit of NaN, and inf * 0 from one that is -inf or below -88
+      if (CAREFUL) c[i] = c[i] > -INFINITY ? v : -INFINITY;
+      else c[i] = fmaf(e, 0.f, v);
     }
   }
+  if (!CAREFUL) {
+    float any = 0.f;                     // NaN if one of them is
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) any = fmaf(c[i], 0.f, any);
+    if (__any_sync(kAll, !(any == 0.f))) return kOdd;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] = __uint_as_float((__float_as_uint(c[i]) & ~kPlace) | (kPlace - i));
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      c[i] = c[i] > -INFINITY ? __uint_as_float((__float_as_uint(c[i]) & ~kPlace) | (kPlace - i)) : -INFINITY;
+  }
   auto near = [&](float hi, float lo) { return !(hi - lo > kTol * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo)))); };
+  const unsigned below = (1u << lane) - 1;
   if (GROUPS) {
     float mine = -INFINITY;              // lane g: group g's score
     auto group_score = [&](int g, float top, float next) {
       const float first = warp_max_float(top);
       float sum = first;
       if (p.group_top == 2) {
-        const unsigned holders = __ballot_sync(kAll, top == first);
-        if (lane == __ffs(holders) - 1) top = next;
+        // the second largest: the lowest lane that holds the largest offers its next
+        const bool hold = top == first;
+        const unsigned holders = __ballot_sync(kAll, hold);
+        if (hold && !(holders & below)) top = next;
         const float second = warp_max_float(top);
         if (second > -INFINITY) sum += second;
       }
       if (lane == g) mine = sum;
     };
+    unsigned chosen = 0;
+    float last = -INFINITY;
+    auto choose = [&]() {
+      for (int q = 0; q < p.top_groups; ++q) {
+        const bool open = !((chosen >> lane) & 1);
+        const float best = warp_max_float(open ? mine : -INFINITY);
+        if (best == -INFINITY) break;
+        const unsigned at = __ballot_sync(kAll, open && mine == best);
+        chosen |= at & (0u - at);
+        last = best;
+      }
+    };
     auto by_registers = [&](auto regs) {
       constexpr int RPG = decltype(regs)::value;
 #pragma unroll
       for (int g = 0; g * RPG < VPL; ++g) {
-        float top = -INFINITY, next = -INFINITY;
+        float top = c[g * RPG], next = -INFINITY;
 #pragma unroll
-        for (int i = g * RPG; i < (g + 1) * RPG && i < VPL; ++i) {
+        for (int i = g * RPG + 1; i < (g + 1) * RPG && i < VPL; ++i) {
           next = fmaxf(next, fminf(top, c[i]));
           top = fmaxf(top, c[i]);
         }
         group_score(g, top, next);
       }
+      choose();
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) c[i] = chosen & (1u << (i / RPG)) ? c[i] : -INFINITY;
     };
     // groups of 32, 64 or 128 experts are whole registers: compile-time loops, whose warp-wide maxima overlap
     if (p.group_size == 32) {
@@ -460,70 +503,67 @@ __device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane
         }
         group_score(g, top, next);
       }
-    }
-    unsigned chosen = 0;
-    float last = -INFINITY;
-    for (int q = 0; q < p.top_groups; ++q) {
-      const bool open = !((chosen >> lane) & 1);
-      const float best = warp_max_float(open ? mine : -INFINITY);
-      if (best == -INFINITY) break;
-      const unsigned at = __ballot_sync(kAll, open && mine == best);
-      chosen |= at & (0u - at);
-      last = best;
+      choose();
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) c[i] = (chosen >> grp[i]) & 1 ? c[i] : -INFINITY;
     }
     const float out = warp_max_float((chosen >> lane) & 1 ? -INFINITY : mine);
-    if (out > -INFINITY && near(0.5f * last, 0.5f * out)) return true;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] = (chosen >> grp[i]) & 1 ? c[i] : -INFINITY;
+    if (out > -INFINITY && near(0.5f * last, 0.5f * out)) return kNear;
   }
-  // Each lane keeps its DEPTH largest in order; a lane whose DEPTH have all been taken looks for the next ones
-  // below the last taken (rare: of 256 experts' 8 best, 3 share a lane in one row of twenty).
-  constexpr int DEPTH = VPL < 3 ? VPL : 3;
+  // Each lane keeps its DEPTH largest in order.  4 of 256 experts' 8 best share a lane in one row of five hundred;
+  // only the careful form then looks for the lane's next ones, below the last taken.
+  constexpr int kDepth = CAREFUL ? 3 : 4, DEPTH = VPL < kDepth ? VPL : kDepth;
   float top[DEPTH];
-  auto refill = [&](float below) {
+  auto fill = [&](float limit) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) top[d] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      float v = c[i] < below ? c[i] : -INFINITY;
+      float v = CAREFUL ? (c[i] < limit ? c[i] : -INFINITY) : c[i];
 #pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {
+      for (int d = 0; d < DEPTH && d <= i; ++d) {
         const float lower = fminf(top[d], v);
         top[d] = fmaxf(top[d], v);
         v = lower;
       }
     }
   };
-  refill(INFINITY);
-  int taken = 0;
-  float mine = -INFINITY, left_out = -INFINITY;          // lane j: the j-th choice
-  unsigned holder = 0;
-  for (int j = 0; j <= p.k; ++j) {
+  fill(INFINITY);
+  int taken = 0, all_taken = 0;
+  float left_out = -INFINITY;
+  if (CAREFUL) {
+    if (lane < p.k) slots[lane] = make_float2(-INFINITY, 0.f);
+    __syncwarp();
+  }
+  for (int j = 0; j < p.k; ++j) {
     const float best = warp_max_float(top[0]);
-    if (best == -INFINITY) break;
-    if (j == p.k) {
-      left_out = best;
-      break;
-    }
-    const bool hold = top[0] == best;
-    const unsigned who = __ballot_sync(kAll, hold);
-    if (lane == j) mine = best, holder = who;
-    if (hold) {
+    if (CAREFUL && best == -INFINITY) break;
+    if (top[0] == best) {                // one lane; two where choices are equal, found below
+      slots[j] = make_float2(best, __int_as_float(lane));
 #pragma unroll
       for (int d = 0; d + 1 < DEPTH; ++d) top[d] = top[d + 1];
       top[DEPTH - 1] = -INFINITY;
-      if (VPL > DEPTH && ++taken == DEPTH) {
+      ++all_taken;
+      if (CAREFUL && VPL > DEPTH && ++taken == DEPTH) {
         taken = 0;
-        refill(best);
+        fill(best);
       }
     }
   }
-  const float up = __shfl_up_sync(kAll, mine, 1);
+  left_out = warp_max_float(top[0]);
+  // an exhausted lane may hold more of the best than it offered
+  if (!CAREFUL && VPL > DEPTH && __any_sync(kAll, all_taken >= DEPTH)) return kOdd;
+  __syncwarp();
+  const float2 slot = lane < p.k ? slots[lane] : make_float2(-INFINITY, 0.f);
+  const float mine = slot.x;
   const bool on = mine > -INFINITY;
-  bool bad = on && ((holder & (holder - 1)) != 0 || (lane > 0 && near(up, mine)));
+  const int found = CAREFUL ? __popc(__ballot_sync(kAll, on)) : p.k;
+  if ((int)__reduce_add_sync(kAll, (unsigned)all_taken) != found) return kNear;      // equal choices
+  const float up = __shfl_up_sync(kAll, mine, 1);
+  bool bad = on && lane > 0 && near(up, mine);
   if (lane == p.k - 1 && left_out > -INFINITY) bad = bad || near(mine, left_out);
-  if (__any_sync(kAll, bad)) return true;
-  id = on ? (int)(kPlace - (__float_as_uint(mine) & kPlace)) * 32 + __ffs(holder) - 1 : -1;
+  if (__any_sync(kAll, bad)) return kNear;
+  id = on ? (int)(kPlace - (__float_as_uint(mine) & kPlace)) * 32 + __float_as_int(slot.y) : -1;
   float w = 0.f;
   if (on) {
     const int64_t from = t * p.ld + id;
@@ -538,33 +578,62 @@ __device__ __forceinline__ bool fast_row(const RouteArgs& p, int64_t t, int lane
     w = total > 0.f ? w / total : 0.f;
   }
   weight = w * p.scale;
-  return false;
+  return kDone;
+}
+
+// The careful form, a function of its own like the 64-bit pass.
+template <int VPL, bool SOFTMAX, bool GROUPS>
+__device__ __noinline__ RowState careful_row(const RouteArgs& p, int64_t t, int lane, float2* slots) {
+  float bias[VPL];
+  int grp[VPL];
+  load_bias<VPL, true>(p, lane, bias);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    bias[i] = fminf(bias[i], FLT_MAX);
+    grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
+  }
+  int id;
+  float w;
+  const RowState state = fast_row<VPL, SOFTMAX, GROUPS, true>(p, t, lane, bias, grp, slots, id, w);
+  if (state == kDone) store_row(p, t, lane, id, w);
+  return state;
 }
 
 template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
-__global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouteArgs p) {
-  const int lane = threadIdx.x & 31;
+__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : VPL == 16 ? 2 : 1) route_kernel(const __grid_constant__ RouteArgs p) {
+  __shared__ float2 slots[8][kMaxTopK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
   float bias[VPL];
   int grp[VPL];
   load_bias<VPL, BIAS>(p, lane, bias);
+  bool odd = false;                      // an expert is off by its bias
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) bias[i] = fminf(bias[i], FLT_MAX);   // the 64-bit pass tells it from +inf
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
-  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); t < p.T; t += warps) {
+  for (int i = 0; i < VPL; ++i) {
+    odd = odd || (BIAS && !(bias[i] > -INFINITY));
+    bias[i] = fminf(bias[i], FLT_MAX);   // the 64-bit pass tells it from +inf
+    grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
+  }
+  odd = p.E != VPL * 32 || __any_sync(kAll, odd);
+  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp; t < p.T; t += warps) {
     int id;
     float w;
-    bool again;
+    RowState state;
     if (BIAS && (!SOFTMAX || p.renorm)) {   // softmax weights as they are want an accurate sum: the other pass
-      again = fast_row<VPL, SOFTMAX, GROUPS>(p, t, lane, bias, grp, id, w);
+      state = odd ? kOdd : fast_row<VPL, SOFTMAX, GROUPS, false>(p, t, lane, bias, grp, slots[warp], id, w);
+      if (state == kOdd) {
+        __syncwarp();
+        state = careful_row<VPL, SOFTMAX, GROUPS>(p, t, lane, slots[warp]);
+        if (state == kDone) continue;
+      }
     } else {
       float x[VPL];
       load_row<VPL, BIAS>(p, t, lane, bias, x);
-      again = route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w);
+      state = route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w) ? kNear : kDone;
     }
-    if (again) route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
+    if (state == kNear) route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
     else store_row(p, t, lane, id, w);
+    __syncwarp();
   }
 }
 
