@@ -4,14 +4,15 @@
 //   xq = nvfp4(x[t]);  h = silu(xq . Wg_e^T) * (xq . Wu_e^T);  hq = nvfp4(h)
 //   out[t] = fp16( sum_j weights[t, j] * (hq . Wd_e^T) ),  e = ids[t, j], slots in order of j
 //
-// Five launches: the plan (plan.cuh), quantising the tokens into their rows
-// (each token once, stored for each of its experts), the two expert products
-// (moe_gemm.cuh) and the sum over a token's slots.  h never leaves the first
+// The plan (plan.cuh), quantising the tokens into their rows (each token once,
+// stored for each of its experts; one launch with the plan for few slots),
+// the two expert products (moe_gemm.cuh) and the sum over a token's slots.  h never leaves the first
 // product but as NVFP4.  y = weight * product stays in fp32 between the second
 // product and the sum: the sum then rounds once, and a product beyond fp16's
 // range does no harm.
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <cstdlib>
 #include <cstring>
 #include "ptx.cuh"
 #include "tcgen05.cuh"
@@ -25,47 +26,126 @@ namespace {
 
 constexpr int kMoeMaxExperts = kPlanMaxIndexes, kMoeMaxTopK = 32;
 
-// Each CTA takes whole tokens: a thread quantises one 16-element block and
-// stores it for each of the token's slots.
-__global__ void __launch_bounds__(256) scatter_quantize_kernel(const __half* __restrict__ x, int64_t ldx, int64_t T,
-                                                               int k, int D, const int* __restrict__ rows,
-                                                               const float* __restrict__ weights, uint8_t* codes,
-                                                               uint8_t* sf, float* row_weight) {
-  const int kb = D / 16, lane = threadIdx.x & 31;
-  griddep_launch();
-  griddep_wait();
-  for (int64_t t = blockIdx.x; t < T; t += gridDim.x) {
-    for (int c0 = threadIdx.x & ~31; c0 < kb; c0 += blockDim.x) {
-      const int c = c0 + lane;
-      const bool live = c < kb;
-      uint32_t w[8], packed[2], sbyte = 0;
-      if (live) {
-        load_block(x + t * ldx + (int64_t)c * 16, w);
-        sbyte = quant_halves(w, packed);
-      }
-      const uint32_t b1 = __shfl_down_sync(0xffffffffu, sbyte, 1);
-      const uint32_t b2 = __shfl_down_sync(0xffffffffu, sbyte, 2);
-      const uint32_t b3 = __shfl_down_sync(0xffffffffu, sbyte, 3);
-      if (!live) continue;
-      for (int j = 0; j < k; ++j) {
-        const int r = rows[t * k + j];
-        if (r < 0) continue;
-        *reinterpret_cast<uint2*>(codes + (int64_t)r * (D / 2) + c * 8) = make_uint2(packed[0], packed[1]);
-        if ((lane & 3) == 0)             // D is a multiple of 64: whole words of four blocks
-          *reinterpret_cast<uint32_t*>(sf + blocked_at(r, c, D / 64)) = sbyte | (b1 << 8) | (b2 << 16) | (b3 << 24);
-      }
+struct ScatterArgs {
+  const __half* x;
+  int64_t ldx, T;
+  int k, D;
+  const float* weights;
+  uint8_t* codes;
+  uint8_t* sf;
+  float* row_weight;
+};
+
+// Quantises token t and stores it for each of its slots: a thread takes one 16-element block.
+__device__ __forceinline__ void scatter_token(const ScatterArgs& a, int64_t t, const int* rows) {
+  const int kb = a.D / 16, lane = threadIdx.x & 31;
+  for (int c0 = threadIdx.x & ~31; c0 < kb; c0 += blockDim.x) {
+    const int c = c0 + lane;
+    const bool live = c < kb;
+    uint32_t w[8], packed[2], sbyte = 0;
+    if (live) {
+      load_block(a.x + t * a.ldx + (int64_t)c * 16, w);
+      sbyte = quant_halves(w, packed);
     }
-    if ((int)threadIdx.x < k) {
-      const int r = rows[t * k + threadIdx.x];
-      if (r >= 0) row_weight[r] = weights[t * k + threadIdx.x];
+    const uint32_t b1 = __shfl_down_sync(0xffffffffu, sbyte, 1);
+    const uint32_t b2 = __shfl_down_sync(0xffffffffu, sbyte, 2);
+    const uint32_t b3 = __shfl_down_sync(0xffffffffu, sbyte, 3);
+    if (!live) continue;
+    for (int j = 0; j < a.k; ++j) {
+      const int r = rows[j];
+      if (r < 0) continue;
+      *reinterpret_cast<uint2*>(a.codes + (int64_t)r * (a.D / 2) + c * 8) = make_uint2(packed[0], packed[1]);
+      if ((lane & 3) == 0)             // D is a multiple of 64: whole words of four blocks
+        *reinterpret_cast<uint32_t*>(a.sf + blocked_at(r, c, a.D / 64)) = sbyte | (b1 << 8) | (b2 << 16) | (b3 << 24);
     }
   }
+  if ((int)threadIdx.x < a.k && rows[threadIdx.x] >= 0)
+    a.row_weight[rows[threadIdx.x]] = a.weights[t * a.k + threadIdx.x];
 }
 
-// out[t] = sum of its slots' rows of y, in slot order; eight columns a thread.
-__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ y, const int* __restrict__ rows,
-                                                      int64_t T, int k, int D, __half* __restrict__ out, int64_t ldo,
-                                                      int vec) {
+__global__ void __launch_bounds__(256) scatter_kernel(const int* rows, ScatterArgs a) {
+  griddep_launch();
+  griddep_wait();
+  for (int64_t t = blockIdx.x; t < a.T; t += gridDim.x) scatter_token(a, t, rows + t * a.k);
+}
+
+// Plan and scatter in one launch, for few slots: every CTA (one per token) counts all of them for itself and
+// finds the rows of its own token's, a warp a slot: its expert's first row plus the number of equal ids before
+// it.  CTA 0 lists the tiles.  Against the two kernels one after the other: 3 us less at 512 slots.
+constexpr int kFusedSlots = 1024;
+
+__global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __restrict__ ids, int n, int experts, int align,
+                                                           int tile, Plan p, ScatterArgs a) {
+  __shared__ int id[kFusedSlots];
+  __shared__ int count[kPlanMaxIndexes], row0[kPlanMaxIndexes];
+  __shared__ int mine[kMoeMaxTopK], sums[8][2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t t = blockIdx.x;
+  griddep_launch();
+  for (int e = tid; e < kPlanMaxIndexes; e += 256) count[e] = 0;
+  __syncthreads();
+  for (int s = tid; s < n; s += 256) {
+    const int e = ids[s];
+    id[s] = (unsigned)e < (unsigned)experts ? e : -1;
+    if (id[s] >= 0) atomicAdd(&count[e], 1);
+  }
+  __syncthreads();
+  // thread i: experts 4i .. 4i + 3
+  int span = 0, tiles = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = count[4 * tid + j];
+    span += (c + align - 1) / align * align;
+    tiles += (c + tile - 1) / tile;
+  }
+  int r = span, m = tiles;                       // inclusive scans
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, r, o), v = __shfl_up_sync(0xffffffffu, m, o);
+    if (lane >= o) r += u, m += v;
+  }
+  if (lane == 31) sums[warp][0] = r, sums[warp][1] = m;
+  __syncthreads();
+  int first = m - tiles, from = r - span, all = 0;
+  for (int w = 0; w < 8; ++w) {
+    if (w < warp) from += sums[w][0], first += sums[w][1];
+    all += sums[w][1];
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int e = 4 * tid + j, c = count[e], here = (c + tile - 1) / tile;
+    row0[e] = from;
+    if (t == 0)
+      for (int i = 0; i < here; ++i) {
+        PlanTile q;
+        q.index = e; q.row0 = from; q.first = first; q.tiles = here; q.rows = c;
+        q.pad[0] = q.pad[1] = q.pad[2] = 0;
+        p.tiles[first + i] = q;
+      }
+    from += (c + align - 1) / align * align;
+    first += here;
+  }
+  if (t == 0 && tid == 0) p.head[0] = all;
+  __syncthreads();
+  for (int j = warp; j < a.k; j += 8) {
+    const int s = (int)t * a.k + j, e = id[s];
+    int before = 0;
+    for (int o = lane; o < s; o += 32) before += id[o] == e;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (lane == 0) {
+      mine[j] = e >= 0 ? row0[e] + before : -1;
+      p.row[s] = mine[j];
+    }
+  }
+  __syncthreads();
+  scatter_token(a, t, mine);
+}
+
+// out[t] = sum of its slots' rows of y, in slot order (and of the parts of each); eight columns a thread.
+__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ y, int parts, int64_t part_stride,
+                                                      const int* __restrict__ rows, int64_t T, int k, int D,
+                                                      __half* __restrict__ out, int64_t ldo, int vec) {
   griddep_launch();
   griddep_wait();
   const int per = D / 8;
@@ -77,10 +157,12 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ 
     for (int j = 0; j < k; ++j) {
       const int r = rows[t * k + j];
       if (r < 0) continue;
-      const float4* src = reinterpret_cast<const float4*>(y + (int64_t)r * D + c);
-      const float4 a = src[0], b = src[1];
-      acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
-      acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
+      for (int s = 0; s < parts; ++s) {
+        const float4* src = reinterpret_cast<const float4*>(y + s * part_stride + (int64_t)r * D + c);
+        const float4 a = src[0], b = src[1];
+        acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
+        acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
+      }
     }
     const uint4 piece = make_uint4(pack_h2(acc[0], acc[1]), pack_h2(acc[2], acc[3]), pack_h2(acc[4], acc[5]),
                                    pack_h2(acc[6], acc[7]));
@@ -94,15 +176,36 @@ __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ 
 struct MoeLayout {
   bool trans;           // few tokens per expert: weights as the MMA's first operand
   int tile;             // token rows per tile, and the alignment of an expert's rows
+  int parts;            // of the down product's inner dimension
   int64_t rows, max_tiles;
   int64_t tiles, row, row_weight, xq, xs, hq, hs, y, bytes;
 };
 
+// Into how many parts the down product of few tokens cuts its inner dimension, so that its tiles fill the SMs:
+// the count with the fewest stages on the busiest SM, if every expert that can be active is.  A part more
+// costs a y to write and to read again, which is counted at half a stage (32 KB of weights).
+int down_parts(int64_t n, int64_t E, int64_t D, int64_t F, int tile) {
+  const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(std::min(n, E) + n / tile, n)) * ((D + 127) / 128);
+  const int64_t stages = (F + 511) / 512, sms = sm_count();
+  int best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= std::min<int64_t>(8, stages); ++s) {
+    const double cost = (double)((tiles * s + sms - 1) / sms) * ((stages + s - 1) / s) + 0.5 * (s - 1);
+    if (cost < least - 1e-9) {
+      least = cost;
+      best = (int)s;
+    }
+  }
+  return best;
+}
+
 MoeLayout moe_layout(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F) {
   MoeLayout m;
   const int64_t n = T * k;
-  m.trans = n <= 64 * E;
+  static const int kMT = getenv("MT") ? atoi(getenv("MT")) : 64;
+  m.trans = n <= kMT * E;
   m.tile = !m.trans ? 128 : n <= 8 * E ? 16 : n <= 16 * E ? 32 : 64;
+  m.parts = m.trans ? down_parts(n, E, D, F, m.tile) : 1;
   m.rows = (plan_max_rows(n, E, m.tile) + 127) / 128 * 128;
   m.max_tiles = plan_max_tiles(n, E, m.tile);
   int64_t at = 0;
@@ -119,7 +222,7 @@ MoeLayout moe_layout(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F) {
   m.xs = take(m.rows * D / 16);
   m.hq = take(m.rows * F / 2);
   m.hs = take(m.rows * F / 16);
-  m.y = take(m.rows * D * 4);
+  m.y = take(m.parts * m.rows * D * 4);
   m.bytes = at;
   return m;
 }
@@ -133,14 +236,19 @@ int moe_check(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F) {
   return NVFP4_OK;
 }
 
-int weight_maps(const char* name, CUtensorMap* tw, CUtensorMap* tsw, const void* w, const void* sf, int64_t E,
-                int64_t N, int64_t K, int64_t ld, int64_t es, int64_t sfe, int box_rows, int kps) {
+int check_weights(const char* name, const void* w, const void* sf, int64_t E, int64_t K, int64_t ld, int64_t es,
+                  int64_t sfe) {
   if (!w || !sf) return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: %s: null pointer", name);
   if (ld < K / 2 || (E > 1 && (es <= 0 || sfe <= 0)))
     return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: %s: row stride below K/2, or an expert stride that is not positive", name);
-  if (E == 1) es = N * ld, sfe = (N + 127) / 128 * (K / 64) * 512;
-  if (!aligned16(w) || !aligned16(sf) || ld % 16 || es % 16 || sfe % 16)
+  if (!aligned16(w) || !aligned16(sf) || ld % 16 || (E > 1 && (es % 16 || sfe % 16)))
     return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_moe_mlp: %s: pointers and strides must be multiples of 16 bytes", name);
+  return NVFP4_OK;
+}
+
+int weight_maps(CUtensorMap* tw, CUtensorMap* tsw, const void* w, const void* sf, int64_t E, int64_t N, int64_t K,
+                int64_t ld, int64_t es, int64_t sfe, int box_rows, int kps) {
+  if (E == 1) es = N * ld, sfe = (N + 127) / 128 * (K / 64) * 512;
   const uint64_t dims[3] = {(uint64_t)(K / 2), (uint64_t)N, (uint64_t)E};
   const uint64_t str[2] = {(uint64_t)ld, (uint64_t)es};
   const uint32_t box[3] = {KSTEP_BYTES, (uint32_t)box_rows, 1};
@@ -167,6 +275,12 @@ int token_maps(ExpertParams& P, const void* codes, const void* sf, int64_t rows,
 }
 
 struct MoeCall {
+  const __half* x;
+  int64_t ldx;
+  const int32_t* ids;
+  const float* weights;
+  __half* out;
+  int64_t ldo, T, k;
   const void *wg, *wu, *wd, *sg, *su, *sd;
   int64_t E, D, F;
   int64_t ld_in, es_in, sfe_in, ld_down, es_down, sfe_down;   // byte strides: rows, experts, scales of an expert
@@ -174,22 +288,23 @@ struct MoeCall {
   uint8_t* ws;
   uint32_t* err;
   cudaStream_t stream;
+  int dev;
 };
 
+// Everything of a product's launch that can be refused, before the first launch of the call.
 template <class C>
-int expert_product(const MoeCall& c) {
-  ExpertParams P;
+int expert_params(const MoeCall& c, ExpertParams& P) {
   std::memset(&P, 0, sizeof(P));
   const MoeLayout& m = c.m;
   int rc;
   if (C::DUAL) {
     if ((rc = token_maps(P, c.ws + m.xq, c.ws + m.xs, m.rows, c.D, C::T_ROWS, C::KPS)) ||
-        (rc = weight_maps("gate", &P.tw[0], &P.tsw[0], c.wg, c.sg, c.E, c.F, c.D, c.ld_in, c.es_in, c.sfe_in, C::W_ROWS, C::KPS)) ||
-        (rc = weight_maps("up", &P.tw[1], &P.tsw[1], c.wu, c.su, c.E, c.F, c.D, c.ld_in, c.es_in, c.sfe_in, C::W_ROWS, C::KPS)))
+        (rc = weight_maps(&P.tw[0], &P.tsw[0], c.wg, c.sg, c.E, c.F, c.D, c.ld_in, c.es_in, c.sfe_in, C::W_ROWS, C::KPS)) ||
+        (rc = weight_maps(&P.tw[1], &P.tsw[1], c.wu, c.su, c.E, c.F, c.D, c.ld_in, c.es_in, c.sfe_in, C::W_ROWS, C::KPS)))
       return rc;
   } else {
     if ((rc = token_maps(P, c.ws + m.hq, c.ws + m.hs, m.rows, c.F, C::T_ROWS, C::KPS)) ||
-        (rc = weight_maps("down", &P.tw[0], &P.tsw[0], c.wd, c.sd, c.E, c.D, c.F, c.ld_down, c.es_down, c.sfe_down, C::W_ROWS, C::KPS)))
+        (rc = weight_maps(&P.tw[0], &P.tsw[0], c.wd, c.sd, c.E, c.D, c.F, c.ld_down, c.es_down, c.sfe_down, C::W_ROWS, C::KPS)))
       return rc;
   }
   P.tiles = reinterpret_cast<const PlanTile*>(c.ws + m.tiles);
@@ -201,26 +316,52 @@ int expert_product(const MoeCall& c) {
   P.sf = c.ws + m.hs;
   P.y = reinterpret_cast<float*>(c.ws + m.y);
   P.row_weight = reinterpret_cast<const float*>(c.ws + m.row_weight);
+  P.parts = m.parts;
+  P.part_stride = m.rows * c.D;
   P.err = c.err;
+  if (m.max_tiles * P.wtiles * m.parts > INT32_MAX / 2) return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: too many tiles");
   static bool attr_set[64] = {};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
-  if (!attr_set[dev]) {
+  if (!attr_set[c.dev]) {
     cudaError_t e = cudaFuncSetAttribute(expert_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(expert product)");
-    attr_set[dev] = true;
+    attr_set[c.dev] = true;
   }
-  const int64_t most = m.max_tiles * P.wtiles;
-  if (most > INT32_MAX / 2) return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: too many tiles");
+  return NVFP4_OK;
+}
+
+template <class C>
+int launch_product(const MoeCall& c, const ExpertParams& P) {
+  const int64_t most = c.m.max_tiles * P.wtiles * (C::TRANS && !C::DUAL ? P.parts : 1);
   return launch_after(expert_kernel<C>, "expert_kernel", (unsigned)std::min<int64_t>(sm_count(), most), C::THREADS,
                       C::SMEM, c.stream, P);
 }
 
-template <int BN, int STAGES_IN, int STAGES_DOWN>
-int expert_products_trans(const MoeCall& c) {
-  const int rc = expert_product<ExpertCfg<true, true, BN, 1, STAGES_IN>>(c);
-  return rc ? rc : expert_product<ExpertCfg<true, false, BN, 2, STAGES_DOWN>>(c);
+template <class In, class Down>
+int moe_run(const MoeCall& c) {
+  ExpertParams in, down;
+  int rc;
+  if ((rc = expert_params<In>(c, in)) || (rc = expert_params<Down>(c, down))) return rc;
+  const MoeLayout& m = c.m;
+  int* const rows = reinterpret_cast<int*>(c.ws + m.row);
+  const Plan plan = {reinterpret_cast<int*>(c.ws), reinterpret_cast<PlanTile*>(c.ws + m.tiles), rows, nullptr};
+  const ScatterArgs a = {c.x, c.ldx, c.T, (int)c.k, (int)c.D, c.weights, c.ws + m.xq, c.ws + m.xs,
+                         reinterpret_cast<float*>(c.ws + m.row_weight)};
+  const int64_t n = c.T * c.k;
+  if (n <= kFusedSlots) {
+    plan_scatter_kernel<<<(unsigned)c.T, 256, 0, c.stream>>>(c.ids, (int)n, (int)c.E, m.tile, m.tile, plan, a);
+    if ((rc = check_launch("plan_scatter_kernel"))) return rc;
+  } else {
+    if ((rc = launch_plan(c.ids, n, c.E, -1, m.tile, m.tile, plan, c.stream))) return rc;
+    if ((rc = launch_after(scatter_kernel, "scatter_kernel", (unsigned)std::min<int64_t>(c.T, (int64_t)sm_count() * 8),
+                           256, 0, c.stream, (const int*)rows, a)))
+      return rc;
+  }
+  if ((rc = launch_product<In>(c, in)) || (rc = launch_product<Down>(c, down))) return rc;
+  const int64_t pieces = c.T * (c.D / 8);
+  return launch_after(combine_kernel, "combine_kernel",
+                      (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)sm_count() * 8), 256, 0, c.stream,
+                      (const float*)(c.ws + m.y), m.parts, m.rows * c.D, (const int*)rows, c.T, (int)c.k, (int)c.D,
+                      c.out, c.ldo, (int)(aligned16(c.out) && (c.ldo % 8 == 0 || c.T == 1)));
 }
 
 }  // namespace
@@ -251,42 +392,22 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
   if ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) & 3)
     return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_moe_mlp: ids and weights must be 4-byte aligned");
   if (reinterpret_cast<uintptr_t>(workspace) & 255) return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_moe_mlp: workspace not 256-byte aligned");
-  MoeCall c = {w_gate, w_up, w_down, sf_gate, sf_up, sf_down, E, D, F, ld_in, es_in, sfe_in, ld_down, es_down, sfe_down,
-               moe_layout(T, k, E, D, F), static_cast<uint8_t*>(workspace), nullptr, static_cast<cudaStream_t>(stream)};
+  MoeCall c = {static_cast<const __half*>(x), ldx, ids, weights, static_cast<__half*>(out), ldo, T, k,
+               w_gate, w_up, w_down, sf_gate, sf_up, sf_down, E, D, F, ld_in, es_in, sfe_in, ld_down, es_down, sfe_down,
+               moe_layout(T, k, E, D, F), static_cast<uint8_t*>(workspace), nullptr, static_cast<cudaStream_t>(stream), 0};
   const MoeLayout& m = c.m;
   if (workspace_bytes < m.bytes)
     return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: workspace of %lld bytes, need %lld", (long long)workspace_bytes, (long long)m.bytes);
-  {
-    // everything that can be refused is refused before the first launch
-    CUtensorMap a, b;
-    if ((rc = weight_maps("gate", &a, &b, w_gate, sf_gate, E, F, D, ld_in, es_in, sfe_in, 128, 4)) ||
-        (rc = weight_maps("up", &a, &b, w_up, sf_up, E, F, D, ld_in, es_in, sfe_in, 128, 4)) ||
-        (rc = weight_maps("down", &a, &b, w_down, sf_down, E, D, F, ld_down, es_down, sfe_down, 128, 4)))
-      return rc;
-  }
+  if ((rc = check_weights("gate", w_gate, sf_gate, E, D, ld_in, es_in, sfe_in)) ||
+      (rc = check_weights("up", w_up, sf_up, E, D, ld_in, es_in, sfe_in)) ||
+      (rc = check_weights("down", w_down, sf_down, E, F, ld_down, es_down, sfe_down)))
+    return rc;
+  cudaGetDevice(&c.dev);
+  if (c.dev < 0 || c.dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   c.err = device_error_word();
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
-  int* const rows = reinterpret_cast<int*>(c.ws + m.row);
-  const Plan plan = {reinterpret_cast<int*>(c.ws), reinterpret_cast<PlanTile*>(c.ws + m.tiles), rows, nullptr};
-  if ((rc = launch_plan(ids, T * k, E, -1, m.tile, m.tile, plan, c.stream))) return rc;
-  const int threads = (int)std::min<int64_t>(256, (D / 16 + 31) / 32 * 32);
-  if ((rc = launch_after(scatter_quantize_kernel, "scatter_quantize_kernel",
-                         (unsigned)std::min<int64_t>(T, (int64_t)sm_count() * 8), threads, 0, c.stream,
-                         static_cast<const __half*>(x), ldx, T, (int)k, (int)D, (const int*)rows, weights, c.ws + m.xq,
-                         c.ws + m.xs, reinterpret_cast<float*>(c.ws + m.row_weight))))
-    return rc;
-  if (!m.trans) {
-    if ((rc = expert_product<ExpertCfg<false, true, 128, 2, 2>>(c)) || (rc = expert_product<ExpertCfg<false, false, 256, 1, 4>>(c)))
-      return rc;
-  } else {
-    rc = m.tile == 16   ? expert_products_trans<16, 5, 5>(c)
-         : m.tile == 32 ? expert_products_trans<32, 4, 4>(c)
-                        : expert_products_trans<64, 4, 4>(c);
-    if (rc) return rc;
-  }
-  const int64_t pieces = T * (D / 8);
-  return launch_after(combine_kernel, "combine_kernel",
-                      (unsigned)std::min<int64_t>((pieces + 255) / 256, (int64_t)sm_count() * 8), 256, 0, c.stream,
-                      (const float*)(c.ws + m.y), (const int*)rows, T, (int)k, (int)D, static_cast<__half*>(out), ldo,
-                      (int)(aligned16(out) && (ldo % 8 == 0 || T == 1)));
+  if (!m.trans) return moe_run<ExpertCfg<false, true, 128, 2, 2>, ExpertCfg<false, false, 256, 1, 4>>(c);
+  if (m.tile == 16) return moe_run<ExpertCfg<true, true, 16, 1, 5>, ExpertCfg<true, false, 16, 2, 5>>(c);
+  if (m.tile == 32) return moe_run<ExpertCfg<true, true, 32, 1, 4>, ExpertCfg<true, false, 32, 2, 4>>(c);
+  return moe_run<ExpertCfg<true, true, 64, 1, 4>, ExpertCfg<true, false, 64, 2, 4>>(c);
 }

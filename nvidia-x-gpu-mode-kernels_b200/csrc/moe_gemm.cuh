@@ -17,8 +17,15 @@
 // weights stream; an epilogue lane holds one weight row of every token.
 //
 // Warp roles and the two-barrier stages are those of gemm_kernel: warp 0 TMA
-// producer, warp 1 MMA, warps 2-5 epilogue, warps 6-9 copy the scales into
-// tensor memory.  Every wait is bounded.
+// producer, warp 1 MMA, then the epilogue's warps, then four that copy the
+// scales into tensor memory.  Every wait is bounded.
+//
+// TRANS 0 has 16 epilogue warps, four to a lane quarter of tensor memory: each
+// drains its quarter of the accumulators' columns into registers (64 a thread)
+// and releases them, and the SiLU, quantisation and stores run under the next
+// tile's products.  With 4 warps that worked their way through the columns
+// before releasing them the tensor pipe idled half of the time (gate and up of
+// 8192 rows, 8 experts of 4096 x 14336: %s).
 #pragma once
 #include "plan.cuh"
 #include "quant.cuh"
@@ -33,6 +40,8 @@ struct ExpertParams {
   const int* ntiles;
   int N, K;                         // weight rows of one matrix, inner dimension
   int wtiles;                       // tiles of weight rows
+  int parts;                        // TRANS down: the inner dimension is cut into so many parts, each with a y of its own
+  int64_t part_stride;              // of y, in elements
   uint8_t* codes;                   // DUAL: h [rows][N/2] and its blocked scales
   uint8_t* sf;
   float* y;                         // down: [rows][N]
@@ -75,7 +84,8 @@ struct ExpertCfg {
   static_assert(SF_BASE + STAGES * SF_STAGE_COLS <= TMEM_COLS, "tensor memory budget");
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(SMEM < (1 << 18), "descriptor address field");
-  static constexpr int THREADS = 320;
+  static constexpr int EPI_WARPS = TRANS ? 4 : 16;
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS + 4);
   static constexpr uint32_t IDESC = tc::idesc_mxf4nvf4(BM, BN);
 };
 
@@ -93,6 +103,15 @@ __device__ __forceinline__ void expert_mma(uint32_t tmem, uint64_t dt, uint64_t 
   }
 }
 
+// Through L2: the down product's early reads come before its griddep_wait.
+__device__ __forceinline__ PlanTile load_tile(const PlanTile* p) {
+  const int4 a = __ldcg(reinterpret_cast<const int4*>(p));
+  PlanTile q;
+  q.index = a.x; q.row0 = a.y; q.first = a.z; q.tiles = a.w;
+  q.rows = __ldcg(&p->rows);
+  return q;
+}
+
 // Byte of the blocked scale layout that belongs to (row, 16-element block).
 __device__ __forceinline__ int64_t blocked_at(int row, int block, int64_t nk64) {
   return ((int64_t)(row >> 7) * nk64 + (block >> 2)) * 512 + (row & 31) * 16 + ((row >> 5) & 3) * 4 + (block & 3);
@@ -104,7 +123,6 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   const uint32_t sbase = smem_u32(smem_raw);
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  griddep_launch();
   if (sbase & 1023u) {  // the swizzled tiles need a 1024-aligned base; the launch guarantees it
     if (threadIdx.x == 0) atomicOr(P.err, kDevErrTimeoutMma);
     griddep_wait();
@@ -126,7 +144,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       mbar_init(bar_sff + 8 * s, 1);
     }
     mbar_init(bar_accf, 1);
-    mbar_init(bar_acce, 4);
+    mbar_init(bar_acce, C::EPI_WARPS);
     fence_mbar_init();
     prefetch_tmap(&P.tt);
     prefetch_tmap(&P.tst);
@@ -144,44 +162,82 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   __syncthreads();
   tc::fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - sbase));
-  griddep_wait();                                           // the plan and the operands are written
-  const int total = *P.ntiles * P.wtiles;
+  // The down product's producer starts on weights before its predecessor, the gate and up product, has ended:
+  // that one lets its dependents start only after the plan was written (below).
+  const bool early = !C::DUAL && warp == 0;
+  if (!early) {
+    griddep_wait();                                         // the plan and the operands are written
+    griddep_launch();
+  }
+  const int parts = C::TRANS && !C::DUAL ? P.parts : 1;
+  const int wtiles = P.wtiles * parts;
+  const int total = __ldcg(P.ntiles) * wtiles;
   const int nk64 = P.K / 64;
-  const int nks = (nk64 + C::KPS - 1) / C::KPS;
+  const int nks = (nk64 + C::KPS - 1) / C::KPS;             // stages of a whole product
+  // the stages of item t (all but the TRANS down product: all of them): parts are the fastest index
+  auto from_stage = [&](int t) { return parts == 1 ? 0 : nks * (t % parts) / parts; };
+  auto to_stage = [&](int t) { return parts == 1 ? nks : nks * (t % parts + 1) / parts; };
 
   if (warp == 0) {
     // ---------------------------- producer ----------------------------
     if (lane == 0) {
       const uint64_t pol_t = policy_evict_last();    // token tiles are re-read by every weight tile
       const uint64_t pol_w = policy_evict_first();
-      uint32_t it = 0;
-      for (int t = blockIdx.x; t < total; t += gridDim.x) {
-        const PlanTile q = P.tiles[t / P.wtiles];
-        const int local = t - q.first * P.wtiles;
-        const int row = q.row0 + local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
-        for (int ks = 0; ks < nks; ++ks, ++it) {
-          const int s = it % C::STAGES;
-          if (!mbar_wait(bar_empty + 8 * s, ((it / C::STAGES) & 1) ^ 1, P.err, kDevErrTimeoutEmpty)) goto done;
-          const uint32_t st = sbase + s * C::STAGE_BYTES;
-          // scales first, on their own barrier; boxes always count in full
-          // (what lies past the end of a matrix or of K reads as zeros)
-          const uint32_t sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
-          mbar_arrive_expect_tx(sb, C::SF_BYTES);
-          tma_load_3d(st + C::OFF_SFT, &P.tst, sb, 0, C::KPS * ks, row / 128, pol_t);
+      // Stage `it` (of item t's stage ks): its weights, its tokens.  Scales come first, on their own barrier;
+      // boxes always count in full (what lies past the end of a matrix or of K reads as zeros).
+      auto ask_weights = [&](uint32_t it, int ks, int index, int w0) {
+        const int s = it % C::STAGES;
+        const uint32_t st = sbase + s * C::STAGE_BYTES, sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
+        mbar_arrive_expect_tx(sb, C::SF_BYTES);
+#pragma unroll
+        for (int m = 0; m < C::NW; ++m)
+          tma_load_4d(st + C::OFF_SFW + m * C::SFW_BYTES, &P.tsw[m], sb, 0, C::KPS * ks, w0 / 128, index, pol_w);
+        mbar_arrive_expect_tx(fb, C::OP_BYTES);
+#pragma unroll
+        for (int a = 0; a < C::KA; ++a)
 #pragma unroll
           for (int m = 0; m < C::NW; ++m)
-            tma_load_4d(st + C::OFF_SFW + m * C::SFW_BYTES, &P.tsw[m], sb, 0, C::KPS * ks, w0 / 128, q.index, pol_w);
-          mbar_arrive_expect_tx(fb, C::OP_BYTES);
+            tma_load_3d(st + C::OFF_W + m * C::W_BYTES + a * C::W_ATOM, &P.tw[m], fb, (ks * C::KA + a) * KSTEP_BYTES, w0, index, pol_w);
+      };
+      auto ask_tokens = [&](uint32_t it, int ks, int row) {
+        const int s = it % C::STAGES;
+        const uint32_t st = sbase + s * C::STAGE_BYTES, sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
+        tma_load_3d(st + C::OFF_SFT, &P.tst, sb, 0, C::KPS * ks, row / 128, pol_t);
 #pragma unroll
-          for (int a = 0; a < C::KA; ++a) {
-            const int x = (ks * C::KA + a) * KSTEP_BYTES;
-            tma_load_2d(st + a * C::T_ATOM, &P.tt, fb, x, row, pol_t);
-#pragma unroll
-            for (int m = 0; m < C::NW; ++m)
-              tma_load_3d(st + C::OFF_W + m * C::W_BYTES + a * C::W_ATOM, &P.tw[m], fb, x, w0, q.index, pol_w);
-          }
+        for (int a = 0; a < C::KA; ++a) tma_load_2d(st + a * C::T_ATOM, &P.tt, fb, (ks * C::KA + a) * KSTEP_BYTES, row, pol_t);
+      };
+      // calls body(it, ks, expert, first weight row, first token row) for every stage of this CTA until it says no
+      auto walk = [&](auto body) {
+        uint32_t it = 0;
+        for (int t = blockIdx.x; t < total; t += gridDim.x) {
+          const PlanTile q = load_tile(P.tiles + t / wtiles);
+          const int local = t / parts - q.first * P.wtiles;
+          const int row = q.row0 + local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
+          for (int ks = from_stage(t); ks < to_stage(t); ++ks, ++it)
+            if (!body(it, ks, q.index, w0, row)) return;
         }
+      };
+      if (early) {
+        walk([&](uint32_t it, int ks, int index, int w0, int) {
+          if (it == C::STAGES) return false;
+          ask_weights(it, ks, index, w0);                   // the ring is empty
+          return true;
+        });
+        griddep_wait();                                     // h is written
+        griddep_launch();
       }
+      walk([&](uint32_t it, int ks, int index, int w0, int row) {
+        const int s = it % C::STAGES;
+        if (!early || it >= C::STAGES) {
+          if (!mbar_wait(bar_empty + 8 * s, ((it / C::STAGES) & 1) ^ 1, P.err, kDevErrTimeoutEmpty)) return false;
+          ask_weights(it, ks, index, w0);
+        }
+        ask_tokens(it, ks, row);
+        return true;
+      });
+    } else if (early) {
+      griddep_wait();
+      griddep_launch();
     }
   } else if (warp == 1) {
     // ------------------------------ MMA -------------------------------
@@ -191,7 +247,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
         if (!mbar_wait(bar_acce, (tile_it & 1) ^ 1, P.err, kDevErrTimeoutMma)) goto done;
         tc::fence_after_sync();
-        for (int ks = 0; ks < nks; ++ks, ++it) {
+        const int first = from_stage(t);
+        for (int ks = first; ks < to_stage(t); ++ks, ++it) {
           const int s = it % C::STAGES;
           const uint32_t par = (it / C::STAGES) & 1;
           if (!mbar_wait(bar_sfr + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
@@ -203,17 +260,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
           if (nch == C::KPS) {   // a compile-time count: straight-line MMA issues
 #pragma unroll
             for (int kk = 0; kk < C::KPS; ++kk)
-              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
           } else {
             for (int kk = 0; kk < nch; ++kk)
-              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > 0 || kk > 0) ? 1u : 0u);
+              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
           }
           tc::commit(bar_empty + 8 * s);
         }
         tc::commit(bar_accf);
       }
     }
-  } else if (warp >= 6) {
+  } else if (warp >= 2 + C::EPI_WARPS) {
     // --------------------------- scale warps ---------------------------
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     uint32_t it = 0;
@@ -223,11 +280,11 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       // `from`: byte of this lane's first word in a 512-byte block.
       int from = lane * 16;
       if (C::TRANS) {
-        const PlanTile q = P.tiles[t / P.wtiles];
-        const int off = (q.row0 + (t - q.first * P.wtiles) % q.tiles * C::T_ROWS) % 128;
+        const PlanTile q = load_tile(P.tiles + t / wtiles);
+        const int off = (q.row0 + (t / parts - q.first * P.wtiles) % q.tiles * C::T_ROWS) % 128;
         from = (lane + off) % 32 * 16 + off / 32 * 4;
       }
-      for (int ks = 0; ks < nks; ++ks, ++it) {
+      for (int ks = from_stage(t); ks < to_stage(t); ++ks, ++it) {
         const int s = it % C::STAGES;
         if (!mbar_wait(bar_sff + 8 * s, (it / C::STAGES) & 1, P.err, kDevErrTimeoutFull)) goto done;
         const uint8_t* st = smem_raw + s * C::STAGE_BYTES;
@@ -270,8 +327,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       if (lane == 0) mbar_arrive(bar_acce);
     };
     for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
-      const PlanTile q = P.tiles[t / P.wtiles];
-      const int local = t - q.first * P.wtiles;
+      const PlanTile q = load_tile(P.tiles + t / wtiles);
+      const int local = t / parts - q.first * P.wtiles;
       const int t0 = local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
       if (!mbar_wait(bar_accf, tile_it & 1, P.err, kDevErrTimeoutMma)) break;
       tc::fence_after_sync();
@@ -309,6 +366,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       } else if constexpr (C::TRANS) {
         constexpr int CHUNK = C::BN < 32 ? C::BN : 32;
         const int col = w0 + sub * 32 + lane;
+        float* const y = P.y + t % parts * P.part_stride;
 #pragma unroll 1
         for (int cb = 0; cb < C::BN / CHUNK; ++cb) {
           uint32_t v[32];
@@ -321,56 +379,51 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
             for (int j = 0; j < CHUNK; ++j) {
               const int tok = t0 + cb * CHUNK + j;
               if (tok < q.rows)
-                P.y[(int64_t)(q.row0 + tok) * P.N + col] = P.row_weight[q.row0 + tok] * __uint_as_float(v[j]);
+                y[(int64_t)(q.row0 + tok) * P.N + col] = P.row_weight[q.row0 + tok] * __uint_as_float(v[j]);
             }
           }
         }
-      } else if constexpr (C::DUAL) {
-        // thread = token row: its blocks of 16 columns lie in its registers
+      } else {
+        // thread = token row, warp = a quarter of the columns: all of them into registers first
+        constexpr int COLS = C::NW * C::BN / (C::EPI_WARPS / 4);
+        static_assert(COLS == 64, "accumulator values per thread");
+        const int part = (warp - 2) >> 2;
         const int tok = t0 + sub * 32 + lane, row = q.row0 + tok;
-#pragma unroll 1
-        for (int cb = 0; cb < C::BN / 64; ++cb) {
-          uint32_t codes[8], scales = 0;
+        uint32_t v[32], u[32];
+        tc::ld_32x32b_x32(acc + part * (C::DUAL ? 32 : 64), v);
+        tc::ld_32x32b_x32(acc + (C::DUAL ? C::BN + part * 32 : part * 64 + 32), u);
+        tc::wait_ld();
+        release();
+        const bool live = tok < q.rows;
+        if constexpr (C::DUAL) {
+          // 32 columns: two blocks of 16
+          const int col0 = w0 + part * 32;           // N is a multiple of 64
+          uint32_t codes[4], scales = 0;
 #pragma unroll
-          for (int b = 0; b < 4; ++b) {
-            uint32_t g[32], u[32];
-            tc::ld_32x32b_x16(acc + cb * 64 + b * 16, g);
-            tc::ld_32x32b_x16(acc + C::BN + cb * 64 + b * 16, u);
-            tc::wait_ld();
-            if (cb == C::BN / 64 - 1 && b == 3) release();
-            float v[16];
+          for (int b = 0; b < 2; ++b) {
+            float h[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
+            for (int j = 0; j < 16; ++j) h[j] = silu_mul(__uint_as_float(v[16 * b + j]), __uint_as_float(u[16 * b + j]));
             uint32_t packed[2];
-            scales |= quant_floats(v, packed) << (8 * b);
+            scales |= quant_floats(h, packed) << (8 * b);
             codes[2 * b] = packed[0];
             codes[2 * b + 1] = packed[1];
           }
-          const int col0 = w0 + cb * 64;             // N is a multiple of 64
-          if (tok < q.rows && col0 < P.N) {
-            uint4* dst = reinterpret_cast<uint4*>(P.codes + (int64_t)row * (P.N / 2) + col0 / 2);
-            dst[0] = make_uint4(codes[0], codes[1], codes[2], codes[3]);
-            dst[1] = make_uint4(codes[4], codes[5], codes[6], codes[7]);
-            *reinterpret_cast<uint32_t*>(P.sf + blocked_at(row, col0 / 16, P.N / 64)) = scales;
-          }
-        }
-      } else {
-        const int tok = t0 + sub * 32 + lane, row = q.row0 + tok;
-        const bool live = tok < q.rows;
-        const float weight = live ? P.row_weight[row] : 0.f;
-#pragma unroll 1
-        for (int cb = 0; cb < C::BN / 32; ++cb) {
-          uint32_t v[32];
-          tc::ld_32x32b_x32(acc + cb * 32, v);
-          tc::wait_ld();
-          if (cb == C::BN / 32 - 1) release();
-          const int col0 = w0 + cb * 32;             // N is a multiple of 64
           if (live && col0 < P.N) {
+            *reinterpret_cast<uint4*>(P.codes + (int64_t)row * (P.N / 2) + col0 / 2) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+            *reinterpret_cast<uint16_t*>(P.sf + blocked_at(row, col0 / 16, P.N / 64)) = (uint16_t)scales;
+          }
+        } else {
+          const int col0 = w0 + part * 64;
+          if (live && col0 < P.N) {
+            const float weight = P.row_weight[row];
             float4* dst = reinterpret_cast<float4*>(P.y + (int64_t)row * P.N + col0);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              dst[j] = make_float4(weight * __uint_as_float(v[4 * j]), weight * __uint_as_float(v[4 * j + 1]),
-                                   weight * __uint_as_float(v[4 * j + 2]), weight * __uint_as_float(v[4 * j + 3]));
+            for (int j = 0; j < 16; ++j) {
+              const uint32_t* w = j < 8 ? v + 4 * j : u + 4 * (j - 8);
+              dst[j] = make_float4(weight * __uint_as_float(w[0]), weight * __uint_as_float(w[1]),
+                                   weight * __uint_as_float(w[2]), weight * __uint_as_float(w[3]));
+            }
           }
         }
       }
