@@ -12,7 +12,6 @@
 // range does no harm.
 #include <cuda_fp16.h>
 #include <algorithm>
-#include <cstdlib>
 #include <cstring>
 #include "ptx.cuh"
 #include "tcgen05.cuh"
@@ -202,8 +201,7 @@ int down_parts(int64_t n, int64_t E, int64_t D, int64_t F, int tile) {
 MoeLayout moe_layout(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F) {
   MoeLayout m;
   const int64_t n = T * k;
-  static const int kMT = getenv("MT") ? atoi(getenv("MT")) : 64;
-  m.trans = n <= kMT * E;
+  m.trans = n <= 64 * E;
   m.tile = !m.trans ? 128 : n <= 8 * E ? 16 : n <= 16 * E ? 32 : 64;
   m.parts = m.trans ? down_parts(n, E, D, F, m.tile) : 1;
   m.rows = (plan_max_rows(n, E, m.tile) + 127) / 128 * 128;

@@ -20,7 +20,7 @@ class Problem:
         g = torch.Generator().manual_seed(seed + T + 7 * E + D + F)
         self.x = torch.randn((T, D), generator=g).to(torch.float16)
         if ids is None:
-            ids = torch.rand((T, E), generator=g).argsort(dim=1)[:, :k]
+            ids = torch.rand((T, max(E, k)), generator=g).argsort(dim=1)[:, :k] % E
         self.ids = ids.to(torch.int32).contiguous()
         self.weights = torch.softmax(torch.randn(self.ids.shape, generator=g), dim=1)
         self.wg, self.sg, self.sg_plain = _expert_weights(pkg, E, F, D, g)
@@ -77,6 +77,7 @@ SHAPES = [
     (1, 2, 8, 512, 1024), (1, 1, 1, 64, 64), (5, 1, 3, 64, 64), (16, 8, 64, 256, 320), (64, 8, 16, 256, 192),
     (33, 3, 7, 192, 448), (100, 4, 8, 320, 576), (128, 1, 2, 128, 128), (129, 1, 1, 128, 128),
     (300, 2, 2, 256, 384), (333, 4, 8, 448, 320), (700, 2, 4, 192, 320), (3000, 2, 16, 64, 64), (40, 2, 300, 64, 128),
+    (1000, 2, 2, 512, 768), (901, 1, 2, 256, 1024), (1500, 4, 5, 256, 256), (130, 6, 2, 768, 256),
 ]
 
 
@@ -91,11 +92,11 @@ def test_moe(pkg, oracle, cuda, T, k, E, D, F):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("T,k,E", [(60, 2, 32), (90, 4, 16), (500, 2, 4)])
-def test_moe_everyone_wants_one_expert(pkg, oracle, cuda, T, k, E):
+@pytest.mark.parametrize("T,k,E,D,F", [(60, 2, 32, 128, 192), (90, 4, 16, 128, 192), (500, 2, 4, 128, 192), (1000, 2, 4, 256, 256)])
+def test_moe_everyone_wants_one_expert(pkg, oracle, cuda, T, k, E, D, F):
     g = torch.Generator().manual_seed(9)
     ids = torch.stack([torch.full((T,), E - 2)] + [torch.randint(0, E - 2, (T,), generator=g) for _ in range(k - 1)], dim=1)
-    p = Problem(pkg, T, k, E, 128, 192, ids=ids)
+    p = Problem(pkg, T, k, E, D, F, ids=ids)
     p.check(oracle, pkg.moe_mlp(*p.args()))
     assert pkg._lib.device_errors() == 0
 
