@@ -404,7 +404,7 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
   if (c.dev < 0 || c.dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   c.err = device_error_word();
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
-  if (!m.trans) return moe_run<ExpertCfg<false, true, 128, 2, 2>, ExpertCfg<false, false, 256, 1, 4>>(c);
+  if (!m.trans) return moe_run<ExpertCfg<false, true, 128, 1, 4>, ExpertCfg<false, false, 256, 1, 4>>(c);
   if (m.tile == 16) return moe_run<ExpertCfg<true, true, 16, 1, 5>, ExpertCfg<true, false, 16, 2, 5>>(c);
   if (m.tile == 32) return moe_run<ExpertCfg<true, true, 32, 1, 4>, ExpertCfg<true, false, 32, 2, 4>>(c);
   return moe_run<ExpertCfg<true, true, 64, 1, 4>, ExpertCfg<true, false, 64, 2, 4>>(c);

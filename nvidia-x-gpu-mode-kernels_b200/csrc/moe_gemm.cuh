@@ -16,9 +16,13 @@
 // 64) the other, so the tensor cores' work shrinks with the tokens and the
 // weights stream; an epilogue lane holds one weight row of every token.
 //
-// Warp roles and the two-barrier stages are those of gemm_kernel: warp 0 TMA
-// producer, warp 1 MMA, then the epilogue's warps, then four that copy the
-// scales into tensor memory.  Every wait is bounded.
+// Warp roles: warp 0 TMA producer of the operands, warp 1 MMA, then the
+// epilogue's warps, four that copy the scales into tensor memory, and the
+// scales' own TMA producer (a thread needs about 50 ns to issue a box).  The
+// MMA thread waits for one barrier a stage, which the operands' bytes and the
+// scale warps complete: the tensor pipe holds about two MMAs ahead, so what
+// the thread does between two stages must fit into their time.  Every wait is
+// bounded.
 //
 // TRANS 0 has 16 epilogue warps, four to a lane quarter of tensor memory: each
 // drains its quarter of the accumulators' columns into registers (64 a thread)
@@ -60,9 +64,13 @@ struct ExpertCfg {
   static constexpr int NBW = W_ROWS / 128;                 // scale blocks of a weight tile
   static_assert(W_ROWS % 128 == 0, "weight tiles are whole scale blocks");
   static_assert(!TRANS || BN == 16 || BN == 32 || BN == 64, "token tiles");
+  // One MMA does it where the weights are its second operand: the gate rows and the up rows of a K atom lie one
+  // after the other, as its N = 2 BN rows.
+  static constexpr int MMA_N = TRANS ? BN : NW * BN;
+  static_assert(MMA_N <= 256, "N of an MMA");
   static constexpr int T_ATOM = T_ROWS * KSTEP_BYTES, W_ATOM = W_ROWS * KSTEP_BYTES;
   static constexpr int T_BYTES = KA * T_ATOM, W_BYTES = KA * W_ATOM;
-  static constexpr int OFF_W = T_BYTES;
+  static constexpr int OFF_W = T_BYTES;                    // [K atom][matrix][rows]
   static constexpr int SFT_BYTES = KPS * 512;
   static constexpr int SFW_BYTES = NBW * KPS * 512;        // per weight matrix
   static constexpr int OFF_SFT = OFF_W + NW * W_BYTES;
@@ -72,34 +80,35 @@ struct ExpertCfg {
   static constexpr int OFF_BUF = OFF_BAR + 512;            // TRANS && DUAL: a 16 x 36 float patch per epilogue warp
   static constexpr int BUF_BYTES = TRANS && DUAL ? 4 * 16 * 36 * 4 : 0;
   static constexpr int SMEM = OFF_BUF + BUF_BYTES;
-  static_assert((4 * STAGES + 2) * 8 + 4 <= 512, "barriers");
+  static_assert((3 * STAGES + 2) * 8 + 4 <= 512, "barriers");
   static constexpr uint32_t OP_BYTES = T_BYTES + NW * W_BYTES;
   static constexpr uint32_t SF_BYTES = SFT_BYTES + NW * SFW_BYTES;
   // tensor memory columns
   static constexpr int SF_BASE = NW * BN;                  // the accumulators come first
   static constexpr int SFT_COLS = 4 * KPS;
-  static constexpr int SFW_COLS = KPS * NBW * 4;           // per weight matrix
-  static constexpr int SF_STAGE_COLS = SFT_COLS + NW * SFW_COLS;
+  static constexpr int SFW_COLS = KPS * NW * NBW * 4;      // [K block][matrix][128 rows]
+  static constexpr int SF_STAGE_COLS = SFT_COLS + SFW_COLS;
   static constexpr int TMEM_COLS = 512;
   static_assert(SF_BASE + STAGES * SF_STAGE_COLS <= TMEM_COLS, "tensor memory budget");
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(SMEM < (1 << 18), "descriptor address field");
   static constexpr int EPI_WARPS = TRANS ? 4 : 16;
-  static constexpr int THREADS = 32 * (2 + EPI_WARPS + 4);
-  static constexpr uint32_t IDESC = tc::idesc_mxf4nvf4(BM, BN);
+  static constexpr int THREADS = 32 * (2 + EPI_WARPS + 4 + 1);   // producer, MMA, epilogue, scales, scales' producer
+  static constexpr uint32_t IDESC = tc::idesc_mxf4nvf4(BM, MMA_N);
 };
 
 template <class C>
 __device__ __forceinline__ void expert_mma(uint32_t tmem, uint64_t dt, uint64_t dw, uint32_t sft, uint32_t sfw,
                                            int kk, uint32_t accum) {
   const uint64_t ot = (uint64_t)((kk >> 2) * (C::T_ATOM >> 4) + 2 * (kk & 3));
-  const uint64_t ow = (uint64_t)((kk >> 2) * (C::W_ATOM >> 4) + 2 * (kk & 3));
+  const uint64_t ow = (uint64_t)((kk >> 2) * (C::NW * C::W_ATOM >> 4) + 2 * (kk & 3));
+  if (C::TRANS) {
 #pragma unroll
-  for (int m = 0; m < C::NW; ++m) {
-    const uint64_t w = dw + (uint64_t)(m * (C::W_BYTES >> 4)) + ow;
-    const uint32_t s = sfw + m * C::SFW_COLS + kk * C::NBW * 4;
-    if (C::TRANS) tc::mma_mxf4nvf4(tmem + m * C::BN, w, dt + ot, C::IDESC, s, sft + 4 * kk, accum);
-    else tc::mma_mxf4nvf4(tmem + m * C::BN, dt + ot, w, C::IDESC, sft + 4 * kk, s, accum);
+    for (int m = 0; m < C::NW; ++m)
+      tc::mma_mxf4nvf4(tmem + m * C::BN, dw + (uint64_t)(m * (C::W_ATOM >> 4)) + ow, dt + ot, C::IDESC,
+                       sfw + (kk * C::NW + m) * 4, sft + 4 * kk, accum);
+  } else {
+    tc::mma_mxf4nvf4(tmem, dt + ot, dw + ow, C::IDESC, sft + 4 * kk, sfw + kk * C::NW * C::NBW * 4, accum);
   }
 }
 
@@ -128,19 +137,17 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
     griddep_wait();
     return;
   }
-  const uint32_t bar_full = sbase + C::OFF_BAR;             // operand boxes landed
+  const uint32_t bar_full = sbase + C::OFF_BAR;             // operand boxes landed and scales staged in tensor memory
   const uint32_t bar_empty = bar_full + 8 * C::STAGES;      // stage consumed by the MMAs
-  const uint32_t bar_sfr = bar_empty + 8 * C::STAGES;       // scales staged in tensor memory
-  const uint32_t bar_sff = bar_sfr + 8 * C::STAGES;         // scale boxes landed
+  const uint32_t bar_sff = bar_empty + 8 * C::STAGES;       // scale boxes landed
   const uint32_t bar_accf = bar_sff + 8 * C::STAGES;
   const uint32_t bar_acce = bar_accf + 8;
   const uint32_t tmem_slot = bar_acce + 8;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(bar_full + 8 * s, 1);
+      mbar_init(bar_full + 8 * s, 5);                       // the producer with its bytes, four scale warps
       mbar_init(bar_empty + 8 * s, 1);
-      mbar_init(bar_sfr + 8 * s, 4);
       mbar_init(bar_sff + 8 * s, 1);
     }
     mbar_init(bar_accf, 1);
@@ -164,7 +171,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem_raw + (tmem_slot - sbase));
   // The down product's producer starts on weights before its predecessor, the gate and up product, has ended:
   // that one lets its dependents start only after the plan was written (below).
-  const bool early = !C::DUAL && warp == 0;
+  const bool scales = warp == C::THREADS / 32 - 1;          // the producer of scales
+  const bool early = !C::DUAL && (warp == 0 || scales);
   if (!early) {
     griddep_wait();                                         // the plan and the operands are written
     griddep_launch();
@@ -178,33 +186,42 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   auto from_stage = [&](int t) { return parts == 1 ? 0 : nks * (t % parts) / parts; };
   auto to_stage = [&](int t) { return parts == 1 ? nks : nks * (t % parts + 1) / parts; };
 
-  if (warp == 0) {
-    // ---------------------------- producer ----------------------------
+  if (warp == 0 || scales) {
+    // ------------------- producers: operands, scales -------------------
     if (lane == 0) {
       const uint64_t pol_t = policy_evict_last();    // token tiles are re-read by every weight tile
       const uint64_t pol_w = policy_evict_first();
-      // Stage `it` (of item t's stage ks): its weights, its tokens.  Scales come first, on their own barrier;
-      // boxes always count in full (what lies past the end of a matrix or of K reads as zeros).
+      // Stage `it` (of item t's stage ks): its weights, its tokens.  Boxes always count in full (what lies past
+      // the end of a matrix or of K reads as zeros).
       auto ask_weights = [&](uint32_t it, int ks, int index, int w0) {
         const int s = it % C::STAGES;
-        const uint32_t st = sbase + s * C::STAGE_BYTES, sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
-        mbar_arrive_expect_tx(sb, C::SF_BYTES);
-#pragma unroll
-        for (int m = 0; m < C::NW; ++m)
-          tma_load_4d(st + C::OFF_SFW + m * C::SFW_BYTES, &P.tsw[m], sb, 0, C::KPS * ks, w0 / 128, index, pol_w);
-        mbar_arrive_expect_tx(fb, C::OP_BYTES);
-#pragma unroll
-        for (int a = 0; a < C::KA; ++a)
+        const uint32_t st = sbase + s * C::STAGE_BYTES;
+        if (scales) {
+          const uint32_t sb = bar_sff + 8 * s;
+          mbar_arrive_expect_tx(sb, C::SF_BYTES);
 #pragma unroll
           for (int m = 0; m < C::NW; ++m)
-            tma_load_3d(st + C::OFF_W + m * C::W_BYTES + a * C::W_ATOM, &P.tw[m], fb, (ks * C::KA + a) * KSTEP_BYTES, w0, index, pol_w);
+            tma_load_4d(st + C::OFF_SFW + m * C::SFW_BYTES, &P.tsw[m], sb, 0, C::KPS * ks, w0 / 128, index, pol_w);
+        } else {
+          const uint32_t fb = bar_full + 8 * s;
+          mbar_arrive_expect_tx(fb, C::OP_BYTES);
+#pragma unroll
+          for (int a = 0; a < C::KA; ++a)
+#pragma unroll
+            for (int m = 0; m < C::NW; ++m)
+              tma_load_3d(st + C::OFF_W + (a * C::NW + m) * C::W_ATOM, &P.tw[m], fb, (ks * C::KA + a) * KSTEP_BYTES, w0, index, pol_w);
+        }
       };
       auto ask_tokens = [&](uint32_t it, int ks, int row) {
         const int s = it % C::STAGES;
-        const uint32_t st = sbase + s * C::STAGE_BYTES, sb = bar_sff + 8 * s, fb = bar_full + 8 * s;
-        tma_load_3d(st + C::OFF_SFT, &P.tst, sb, 0, C::KPS * ks, row / 128, pol_t);
+        const uint32_t st = sbase + s * C::STAGE_BYTES;
+        if (scales) {
+          tma_load_3d(st + C::OFF_SFT, &P.tst, bar_sff + 8 * s, 0, C::KPS * ks, row / 128, pol_t);
+        } else {
 #pragma unroll
-        for (int a = 0; a < C::KA; ++a) tma_load_2d(st + a * C::T_ATOM, &P.tt, fb, (ks * C::KA + a) * KSTEP_BYTES, row, pol_t);
+          for (int a = 0; a < C::KA; ++a)
+            tma_load_2d(st + a * C::T_ATOM, &P.tt, bar_full + 8 * s, (ks * C::KA + a) * KSTEP_BYTES, row, pol_t);
+        }
       };
       // calls body(it, ks, expert, first weight row, first token row) for every stage of this CTA until it says no
       auto walk = [&](auto body) {
@@ -247,20 +264,26 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
         if (!mbar_wait(bar_acce, (tile_it & 1) ^ 1, P.err, kDevErrTimeoutMma)) goto done;
         tc::fence_after_sync();
-        const int first = from_stage(t);
-        for (int ks = first; ks < to_stage(t); ++ks, ++it) {
+        const int first = from_stage(t), last = to_stage(t);
+        bool ready = false;                                 // the stage is known to be there
+        for (int ks = first; ks < last; ++ks, ++it) {
           const int s = it % C::STAGES;
           const uint32_t par = (it / C::STAGES) & 1;
-          if (!mbar_wait(bar_sfr + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
-          if (!mbar_wait(bar_full + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
+          if (!ready && !mbar_wait(bar_full + 8 * s, par, P.err, kDevErrTimeoutFull)) goto done;
           tc::fence_after_sync();
           const uint64_t soff = (uint64_t)((s * C::STAGE_BYTES) >> 4);
           const uint32_t sf = tmem + C::SF_BASE + s * C::SF_STAGE_COLS;
           const int nch = min(C::KPS, nk64 - C::KPS * ks);
+          ready = false;
           if (nch == C::KPS) {   // a compile-time count: straight-line MMA issues
 #pragma unroll
-            for (int kk = 0; kk < C::KPS; ++kk)
+            for (int kk = 0; kk < C::KPS; ++kk) {
+              // A look at the next stage while MMAs are queued: the wait, when there is nothing to wait for, costs
+              // the pipe nothing.
+              if (kk == C::KPS - 1 && ks + 1 < last)
+                ready = mbar_test(bar_full + 8 * ((it + 1) % C::STAGES), ((it + 1) / C::STAGES) & 1);
               expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
+            }
           } else {
             for (int kk = 0; kk < nch; ++kk)
               expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
@@ -307,13 +330,13 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
 #pragma unroll
             for (int nb = 0; nb < C::NBW; ++nb) {
               v = *reinterpret_cast<const uint4*>(st + C::OFF_SFW + m * C::SFW_BYTES + (nb * C::KPS + kk) * 512 + lane * 16);
-              tc::st_32x32b_x4(sf + C::SFT_COLS + m * C::SFW_COLS + (kk * C::NBW + nb) * 4, v.x, v.y, v.z, v.w);
+              tc::st_32x32b_x4(sf + C::SFT_COLS + ((kk * C::NW + m) * C::NBW + nb) * 4, v.x, v.y, v.z, v.w);
             }
         }
         tc::wait_st();
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_sfr + 8 * s);
+        if (lane == 0) mbar_arrive(bar_full + 8 * s);
       }
     }
   } else {
