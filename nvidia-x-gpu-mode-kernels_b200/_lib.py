@@ -94,15 +94,15 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
-def call(name: str, device, *args) -> None:
-    """Calls an entry point whose last argument is the stream, with `device`
-    current, on its current stream, and checks the status."""
+def call(name: str, index: int, *args) -> None:
+    """Calls an entry point whose last argument is the stream, with device
+    `index` current, on its current stream, and checks the status."""
     f = getattr(_lib or lib(), name)
-    if device.index == torch.cuda.current_device():
-        status = f(*args, raw_stream(device.index))
+    if index == torch.cuda.current_device():
+        status = f(*args, raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            status = f(*args, raw_stream(device.index))
+        with torch.cuda.device(index):
+            status = f(*args, raw_stream(index))
     if status != 0:
         check(status)
 

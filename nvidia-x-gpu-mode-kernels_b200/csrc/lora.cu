@@ -126,7 +126,7 @@ __device__ __forceinline__ int cluster_nctas() {
   return (int)v;
 }
 
-constexpr int kDecodeTokens = 128;       // most tokens of one call
+constexpr int kDecodeTokens = 256;       // most tokens of one call
 static_assert(kDecodeTokens <= kDecodeWarps * 32, "a thread per token");
 
 template <int RT>
@@ -445,7 +445,8 @@ struct LoraCfg {
 };
 
 // u of 32 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
-// of 128-element stages; two warps take 16 tokens each over each quarter of a stage.
+// of 128-element stages; two warps take 16 tokens each over each quarter of a stage.  Where there are fewer tiles than
+// SMs, a cluster of CTAs shares a tile's K (each a run of stages) and each finishes its share of the tokens.
 template <int RT>
 __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
   using C = LoraCfg<RT>;
@@ -453,11 +454,13 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int m0 = (warp & 1) * 16, share = warp >> 1;     // of kShrinkK: 32 elements, two mma's
+  const int me = (int)cluster_ctarank(), ncta = cluster_nctas();
   griddep_launch();
   griddep_wait();
   const int total = *w.ntiles * PER;
   const int nk = (p.K + kShrinkK - 1) / kShrinkK;
-  for (int item = blockIdx.x; item < total; item += gridDim.x) {
+  const int klo = nk * me / ncta, khi = nk * (me + 1) / ncta;
+  for (int item = blockIdx.x / ncta; item < total; item += gridDim.x / ncta) {
     const PlanTile tile = w.tiles[item / PER];
     const int tr = (item / PER - tile.first) * kTile + item % PER * kShrinkTokens;   // first token within the adapter
     if (tile.index >= p.n || tr >= tile.rows) continue;
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
       xp[e] = s >= 0 ? p.x + (int64_t)s * p.ldx : nullptr;
     }
     auto ask = [&](int ks) {
-      if (ks < nk) {
+      if (ks < khi) {
         __half* const st = reinterpret_cast<__half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
         const int k = ks * kShrinkK + pc;
 #pragma unroll
@@ -493,9 +496,9 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
     };
     __syncthreads();                                     // the previous item's shared memory is read
 #pragma unroll
-    for (int s = 0; s < kShrinkStages - 1; ++s) ask(s);
+    for (int s = 0; s < kShrinkStages - 1; ++s) ask(klo + s);
     float acc[NT][4] = {};
-    for (int ks = 0; ks < nk; ++ks) {
+    for (int ks = klo; ks < khi; ++ks) {
       cp_async_wait<kShrinkStages - 2>();
       __syncthreads();                                   // stage ks is here, stage ks - 1 free
       ask(ks + kShrinkStages - 1);
@@ -523,14 +526,24 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
       *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[nt][2], acc[nt][3]);
     }
     __syncthreads();
+    for (int e = tid; e < kShrinkTokens * R; e += kLoraThreads)
+      part[e] += part[e + kShrinkTokens * R] + part[e + 2 * kShrinkTokens * R] + part[e + 3 * kShrinkTokens * R];
+    if (ncta > 1) cluster_sync();                        // every CTA's sums are there
+    else __syncthreads();
     const float scale = p.scales ? p.scales[tile.index] : 1.f;
-    for (int t = warp; t < kShrinkTokens; t += kLoraThreads / 32) {
+    const int thi = kShrinkTokens * (me + 1) / ncta;
+    for (int t = kShrinkTokens * me / ncta + warp; t < thi; t += kLoraThreads / 32) {
       float u[R / 32];
       float m = 0.f;
 #pragma unroll
       for (int e = 0; e < R / 32; ++e) {
         const float* at = part + t * R + e * 32 + lane;
-        u[e] = (at[0] + at[kShrinkTokens * R] + at[2 * kShrinkTokens * R] + at[3 * kShrinkTokens * R]) * scale;
+        u[e] = *at;
+        if (ncta > 1) {                                  // in the same order whoever adds them
+          u[e] = 0.f;
+          for (int c = 0; c < ncta; ++c) u[e] += __uint_as_float(ld_cluster_u32(mapa(smem_u32(at), c)));
+        }
+        u[e] *= scale;
         m = fmaxf(m, fabsf(u[e]));
       }
 #pragma unroll
@@ -547,6 +560,7 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
       }
       if (lane == 0) w.down[row] = dn;
     }
+    if (ncta > 1) cluster_sync();                        // the others have read this CTA's sums
   }
 }
 
@@ -838,13 +852,27 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   if (rc) return rc;
   const LoraRows rows = {plan.head, plan.tiles, plan.slot, reinterpret_cast<__half*>(ws + m.hi),
                          reinterpret_cast<__half*>(ws + m.lo), reinterpret_cast<float*>(ws + m.down)};
-  if ((rc = launch_after(shrink_kernel<RT>, "shrink_kernel",
-                         (unsigned)std::min<int64_t>(m.max_tiles * (kTile / kShrinkTokens), (int64_t)sm_count() * 2),
-                         kLoraThreads, C::SHRINK_SMEM, stream, p, rows)))
-    return rc;
+  // CTAs per tile: as many as the SMs have room for, each with at least four stages.  T = 256, K = 4096: 14 us
+  // with one, 5 with eight.
+  const int64_t items = (p.T + kShrinkTokens - 1) / kShrinkTokens;
+  int share = 1;
+  while (share < 8 && items * share * 2 <= sm_count() && p.K >= share * 2 * 4 * kShrinkK) share *= 2;
+  {
+    cudaLaunchAttribute both[2] = {attr[0], attr[0]};
+    both[0].val.clusterDim.x = (unsigned)share;
+    both[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    both[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(m.max_tiles * (kTile / kShrinkTokens), std::max(1, sm_count() * 2 / share)) * share));
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = C::SHRINK_SMEM;
+    cfg.attrs = both;
+    cfg.numAttrs = 2;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, shrink_kernel<RT>, p, rows);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernelEx(shrink)");
+  }
   const int64_t steps = (p.N + kExpandCols - 1) / kExpandCols;
   return launch_after(p.vec ? expand_kernel<RT, true> : expand_kernel<RT, false>, "expand_kernel",
-                      (unsigned)std::min<int64_t>(m.max_tiles * ((steps + 3) / 4), (int64_t)sm_count() * 2), kLoraThreads,
+                      (unsigned)std::min<int64_t>(m.max_tiles * steps, (int64_t)sm_count() * 2), kLoraThreads,
                       C::EXPAND_SMEM, stream, p, rows);
 }
 

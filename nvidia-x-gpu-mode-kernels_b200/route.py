@@ -27,26 +27,31 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = 
                   scale: float = 1.0, weights: torch.Tensor | None = None, ids: torch.Tensor | None = None):
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _DTYPES or logits.dim() != 2:
         raise TypeError("logits must be a 2-D float32, float16 or bfloat16 tensor [T, E]")
-    dev = logits.device
-    if dev.type != "cuda":
+    index = logits.get_device()
+    if index < 0:
         raise ValueError("logits must be a CUDA tensor")
     T, E = logits.shape
-    if E > 1 and logits.stride(1) != 1:
+    strides = logits.stride()
+    if E > 1 and strides[1] != 1:
         raise ValueError("logits must be contiguous along the experts")
     if score not in _SCORES:
         raise ValueError(f"score must be one of {sorted(_SCORES)}, got {score!r}")
-    if bias is not None and (not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape != (E,)
-                             or bias.device != dev or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous float32 tensor [{E}] on the device of logits")
+    bias_at = None
+    if bias is not None:
+        if not isinstance(bias, torch.Tensor) or bias.dtype != torch.float32 or bias.shape != (E,) \
+                or bias.get_device() != index or not bias.is_contiguous():
+            raise ValueError(f"bias must be a contiguous float32 tensor [{E}] on the device of logits")
+        bias_at = bias.data_ptr()
     if weights is None:
         weights = logits.new_empty((T, top_k), dtype=torch.float32)
-    elif weights.dtype != torch.float32 or weights.shape != (T, top_k) or weights.device != dev or not weights.is_contiguous():
+    elif weights.dtype != torch.float32 or weights.shape != (T, top_k) or weights.get_device() != index \
+            or not weights.is_contiguous():
         raise ValueError(f"weights must be a contiguous float32 tensor [{T}, {top_k}] on the device of logits")
     if ids is None:
         ids = logits.new_empty((T, top_k), dtype=torch.int32)
-    elif ids.dtype != torch.int32 or ids.shape != (T, top_k) or ids.device != dev or not ids.is_contiguous():
+    elif ids.dtype != torch.int32 or ids.shape != (T, top_k) or ids.get_device() != index or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 tensor [{T}, {top_k}] on the device of logits")
-    _lib.call("nvfp4_route_experts", dev, logits.data_ptr(), _DTYPES[logits.dtype], T, E, logits.stride(0),
-              None if bias is None else bias.data_ptr(), _SCORES[score], top_k, num_groups, top_groups, group_top,
-              renormalize, scale, weights.data_ptr(), ids.data_ptr())
+    _lib.call("nvfp4_route_experts", index, logits.data_ptr(), _DTYPES[logits.dtype], T, E, strides[0], bias_at,
+              _SCORES[score], top_k, num_groups, top_groups, group_top, renormalize, scale, weights.data_ptr(),
+              ids.data_ptr())
     return weights, ids
