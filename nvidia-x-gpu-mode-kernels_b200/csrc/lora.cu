@@ -789,6 +789,16 @@ LoraLayout lora_layout(int64_t T, int64_t r, int64_t n) {
   return m;
 }
 
+// Whether two sets of `rows` rows of fp16 elements share any: row strides ld, row lengths len.  Rows of one stride
+// may lie between one another (column slices of one buffer); with two strides, ranges that meet count as shared.
+bool rows_meet(const void* a, int64_t lda, int64_t lena, const void* b, int64_t ldb, int64_t lenb, int64_t rows) {
+  const int64_t d = (static_cast<const char*>(b) - static_cast<const char*>(a)) / 2;
+  if (d >= (rows - 1) * lda + lena || -d >= (rows - 1) * ldb + lenb) return false;
+  if (rows == 1 || lda != ldb) return true;
+  const int64_t m = (d % lda + lda) % lda;       // where b's rows begin within a's
+  return m < lena || m + lenb > lda;
+}
+
 int lora_check(int64_t T, int64_t r, int64_t n) {
   if (T < 0 || T > (1 << 24)) return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: need 0..2^24 tokens");
   if (r < 16 || r > kLoraMaxRank || r % 16) return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: the largest rank must be a multiple of 16 up to %d", kLoraMaxRank);
@@ -910,6 +920,9 @@ extern "C" int nvfp4_lora_add(const void* base, int64_t ld_base, const void* x, 
     return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_lora_add: fp16 pointer not 2-byte aligned");
   if ((reinterpret_cast<uintptr_t>(adapters) | reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(ranks)) & 3)
     return fail(NVFP4_ERR_ALIGNMENT, "nvfp4_lora_add: adapters, scales and ranks must be 4-byte aligned");
+  if (rows_meet(x, ldx, K, out, ldo, N, T)) return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: out overlaps x");
+  if (base != out && rows_meet(base, ld_base, N, out, ldo, N, T))
+    return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: out overlaps base without being it");
   if (base == out && ld_base != ldo) return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: out is base but has another row stride");
   const LoraLayout m = lora_layout(T, r, n);
   if (m.bytes && !workspace) return fail(NVFP4_ERR_INVALID, "nvfp4_lora_add: null workspace");

@@ -27,9 +27,15 @@
 // TRANS 0 has 16 epilogue warps, four to a lane quarter of tensor memory: each
 // drains its quarter of the accumulators' columns into registers (64 a thread)
 // and releases them, and the SiLU, quantisation and stores run under the next
-// tile's products.  With 4 warps that worked their way through the columns
-// before releasing them the tensor pipe idled half of the time (gate and up of
-// 8192 rows, 8 experts of 4096 x 14336: %s).
+// tile's products (4096 tokens, 2 of 8 experts of 4096 x 14336, gate and up:
+// 547 us with 4 warps that worked their way through the columns before
+// releasing them, 485 with 16; 446 with one 256-column MMA for both matrices
+// and one barrier a stage).  What bounds a stage of 256 elements then is the
+// round trip of the ring: 4 slots of 54 KB, all of shared memory, each taking
+// 0.3 us from the MMAs' end to its refill, 1.4 us until the operands land and
+// 0.28 us of MMAs.  CTA pairs (38 KB a stage, 5 slots) measured the same within
+// 2 %, prefetching weights into L2 slower.  Under minutes of such work the power
+// limit takes another 15 % (768 us a call before it sets in, 913 after).
 #pragma once
 #include "plan.cuh"
 #include "quant.cuh"

@@ -55,7 +55,9 @@ def test_lora_refuses_without_gpu(pkg):
     assert ws(-1, 16, 4) == 1 and ws(4, 8, 4) == 1 and ws(4, 24, 4) == 1 and ws(4, 144, 4) == 1
     assert ws(4, 16, 0) == 1 and ws(4, 16, 1024) == 1 and b"adapters" in l.nvfp4_last_error()
 
-    def call(base=p, ldb=16, x=p, ldx=64, lda=64, sa=1024, T=4, K=64, r=16, n=2, out=p, ldo=100, N=100, ldbase=100,
+    far = p + (1 << 30)
+
+    def call(base=p, ldb=16, x=far, ldx=64, lda=64, sa=1024, T=4, K=64, r=16, n=2, out=p, ldo=100, N=100, ldbase=100,
              w=None, wb=0, ad=p):
         return l.nvfp4_lora_add(base, ldbase, x, ldx, p, lda, sa, p, ldb, 1600, ad, None, None, T, K, N, r, n, out, ldo,
                                 w, wb, None)
@@ -63,12 +65,17 @@ def test_lora_refuses_without_gpu(pkg):
     assert call(K=60) == 1 and call(N=0) == 1 and call(K=0) == 1
     assert call(ldx=56) == 1 and call(ldo=99, out=p + 2) == 1 and call(ldbase=99, out=p + 2) == 1 and call(lda=32) == 1
     assert call(sa=-8) == 1 and call(ldb=8) == 1
-    assert call(x=p + 8) == 2 and call(ldx=68) == 2 and call(sa=1028) == 2 and call(base=p + 1, out=p) == 2
+    assert call(x=far + 8) == 2 and call(ldx=68) == 2 and call(sa=1028) == 2 and call(base=p + 1, out=p) == 2
     assert call(ad=p + 2) == 2
     assert call(ldo=104) == 1 and b"stride" in l.nvfp4_last_error()          # in place with another row stride
     assert call(T=5000) == 1 and b"workspace" in l.nvfp4_last_error()
     assert call(T=5000, w=p, wb=64) == 1
     assert call(T=0, base=None) == 0
+    # out over x, out over a shifted base; column slices of one buffer do not meet
+    assert call(x=p, ldx=104, ldbase=104, ldo=104) == 1 and b"overlaps x" in l.nvfp4_last_error()
+    assert call(x=p + 96, ldx=152, ldbase=152, ldo=152) == 1 and b"overlaps x" in l.nvfp4_last_error()
+    assert call(out=p + 2, ldo=104, ldbase=104) == 1 and b"overlaps base" in l.nvfp4_last_error()
+    assert call(T=5000, x=p + 208, ldx=168, ldbase=168, ldo=168) == 1 and b"workspace" in l.nvfp4_last_error()
 
 
 # ------------------------------------------------------------------- GPU
@@ -78,6 +85,7 @@ SHAPES = [
     (40, 256, 520, 128, 2, 1), (128, 1000, 333, 48, 40, 3), (100, 136, 64, 96, 1, 100),
     (129, 64, 64, 16, 2, 10), (200, 72, 1, 16, 3, 1), (777, 1000, 203, 48, 9, 37), (300, 520, 264, 128, 5, 20),
     (500, 128, 520, 64, 1, 500), (1000, 8, 96, 32, 300, 1), (5000, 64, 40, 112, 7, 90),
+    (256, 64, 72, 32, 60, 1), (257, 64, 72, 32, 60, 1), (300, 4096, 72, 64, 3, 50), (260, 2048, 33, 128, 2, 1),
 ]
 
 
@@ -184,6 +192,29 @@ def test_lora_graphs_and_streams(pkg, oracle, cuda, T):
     torch.cuda.synchronize()
     ps[0].adapters = ps[1].adapters
     ps[0].check(oracle, outs[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 300])
+def test_lora_calls_at_once_and_column_slices(pkg, oracle, cuda, T):
+    """Two eager calls on two streams, and base and x as column slices of one
+    buffer."""
+    ps = [Problem(T, 256, 192, 32, 4, seed=s) for s in (5, 6)]
+    args = [p.args() for p in ps]
+    for a in args:
+        buf = torch.zeros((T, 256 + 192 + 8), dtype=torch.float16, device=cuda)
+        buf[:, :256], buf[:, 256:448] = a[1], a[0]
+        a[0], a[1] = buf[:, 256:448], buf[:, :256]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    for s, a in zip(streams, args):
+        with torch.cuda.stream(s):
+            pkg.lora_add(*a)
+    torch.cuda.synchronize()
+    for p, a in zip(ps, args):
+        p.check(oracle, a[0])
+    with pytest.raises(RuntimeError, match="overlaps x"):
+        pkg.lora_add(args[0][1][:, :192], *args[0][1:])
 
 
 @pytest.mark.gpu

@@ -204,6 +204,25 @@ def test_moe_graphs_and_streams(pkg, oracle, cuda, T, E):
 
 
 @pytest.mark.gpu
+def test_moe_calls_at_once(pkg, oracle, cuda):
+    """Eager calls on three streams at once, of three sizes (each of the paths)."""
+    ps = [Problem(pkg, 10, 2, 4, 256, 256, seed=3), Problem(pkg, 200, 2, 8, 256, 256, seed=4), Problem(pkg, 600, 2, 4, 256, 256, seed=5)]
+    args = [p.args() for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    torch.cuda.synchronize()
+    outs = [[], [], []]
+    for _ in range(3):
+        for o, s, a in zip(outs, streams, args):
+            with torch.cuda.stream(s):
+                o.append(pkg.moe_mlp(*a))
+    torch.cuda.synchronize()
+    for p, o in zip(ps, outs):
+        p.check(oracle, o[0])
+        assert all(torch.equal(o[0], x) for x in o[1:])
+    assert pkg._lib.device_errors() == 0
+
+
+@pytest.mark.gpu
 def test_moe_rows_do_not_depend_on_the_batch_order(pkg, cuda):
     """The same tokens in another order, at the same sizes, give the same bits."""
     p = Problem(pkg, 300, 4, 8, 256, 256)
