@@ -837,7 +837,6 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
       cfg.gridDim = dim3(16);
       cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(16);
       wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT, true>, &cfg) == cudaSuccess && fit > 0;
-      cudaGetLastError();
       e = cudaFuncSetAttribute(shrink_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHRINK_SMEM);
     }
     if (e == cudaSuccess)

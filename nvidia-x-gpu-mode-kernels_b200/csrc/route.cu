@@ -40,6 +40,9 @@ struct RouteArgs {
   int64_t T, ld;
   int E, k, groups, top_groups, group_top, group_size;
   int dtype;               // of the logits: 0 float, 1 half, 2 bfloat16
+  int vec;                 // 16-byte aligned rows
+  int group_lanes;         // quick_row: lanes per group, 0 where groups are no power-of-two runs of lanes
+  int batch;               // rows a warp takes at a time
   int renorm;
   float scale;
 };
@@ -376,27 +379,35 @@ __device__ __forceinline__ float reciprocal_approx(float v) {
 
 // The 32-bit pass over a row with a bias, where every choice is approximate anyway: floats instead of keys
 // (-inf: off), and the lowest bits of a choice replaced by its place in the lane, so that a lane's choices
-// differ and carry their index.  That moves a choice by less than VPL units of 2^-23 relative.  grp: each
-// expert's group.
-//
-// The pass is bound by comparisons and selections (the ALU pipe, half the rate of the others), so the
-// common row takes the form that has few of them (CAREFUL false, kOdd where it will not do): no expert off or
-// below a logit of -88, group's and lane's maxima without ties, no lane with more than DEPTH of the k best.
-enum RowState { kDone, kOdd, kNear };   // kNear: a comparison is too near, the row needs the 64-bit pass
+// differ and carry their index.  That moves a choice by less than VPL units of 2^-23 relative.  Two forms of it:
+// quick_row for rows without surprises, careful_row for all.
+enum RowState { kDone, kOdd, kNear };   // kOdd: not for quick_row; kNear: a comparison is too near, 64 bits must decide
 
-template <int VPL, bool SOFTMAX, bool GROUPS, bool CAREFUL>
-__device__ __forceinline__ RowState fast_row(const RouteArgs& p, int64_t t, int lane, const float (&bias)[VPL],
-                                             const int (&grp)[VPL], float2* slots, int& id, float& weight) {
-  constexpr float kLog2e = 1.4426950408889634f;
-  constexpr uint32_t kPlace = VPL - 1;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int VPL>
+__device__ __forceinline__ bool near_choices(float hi, float lo) {
   constexpr float kTol = 4e-6f + 2 * VPL * 1.2e-7f;
-  float c[VPL];
+  return !(hi - lo > kTol * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo))));
+}
+
+// The logit of an expert that is on, as the passes see it.
+__device__ __forceinline__ float logit_at(const RouteArgs& p, int64_t t, int e) {
+  const int64_t from = t * p.ld + e;
+  return fminf(p.dtype == 0   ? static_cast<const float*>(p.logits)[from]
+               : p.dtype == 1 ? __half2float(static_cast<const __half*>(p.logits)[from])
+                              : __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[from]),
+               FLT_MAX);
+}
+
+// Any row, expert i * 32 + lane in register i.
+template <int VPL, bool SOFTMAX, bool GROUPS>
+__device__ __noinline__ RowState careful_row(const RouteArgs& p, int64_t t, int lane, float2* slots) {
+  constexpr uint32_t kPlace = VPL - 1;
+  float bias[VPL], c[VPL];
+  load_bias<VPL, true>(p, lane, bias);
+  load_row<VPL, true>(p, t, lane, bias, c);
   float m = 0.f;
-  load_raw<VPL>(p, t, lane, c);
-  if (CAREFUL) {
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] = c[i] > -INFINITY && bias[i] > -INFINITY ? fminf(c[i], FLT_MAX) : -INFINITY;
-  }
   if (SOFTMAX) {
     float mx = c[0];
 #pragma unroll
@@ -406,122 +417,72 @@ __device__ __forceinline__ RowState fast_row(const RouteArgs& p, int64_t t, int 
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {      // a row that is off as a whole has NaN here, and no expert that is on
       const float e = exp2_approx((c[i] - m) * kLog2e);
-      if (CAREFUL) {
-        z += c[i] > -INFINITY ? e : 0.f;
-        c[i] = c[i] > -INFINITY ? e : -INFINITY;
-      } else {
-        // NaN from a logit of NaN or an infinity, 1/0 * 0 from one too far below (their exponential is 0)
-        z += e;
-        c[i] = fmaf(reciprocal_approx(e), 0.f, e);
-      }
+      z += c[i] > -INFINITY ? e : 0.f;
+      c[i] = c[i] > -INFINITY ? e : -INFINITY;
     }
     z = reciprocal_approx(warp_sum(z));
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] = fmaf(c[i], z, bias[i]);
+    for (int i = 0; i < VPL; ++i) c[i] *= z;
   } else {
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const float e = exp2_approx(c[i] * -kLog2e);
-      const float v = reciprocal_approx(1.f + e) + bias[i];
-      // NaN from a logit of NaN, and inf * 0 from one that is -inf or below -88
-      if (CAREFUL) c[i] = c[i] > -INFINITY ? v : -INFINITY;
-      else c[i] = fmaf(e, 0.f, v);
+      const float s = reciprocal_approx(1.f + exp2_approx(c[i] * -kLog2e));
+      c[i] = c[i] > -INFINITY ? s : -INFINITY;
     }
   }
-  if (!CAREFUL) {
-    float any = 0.f;                     // NaN if one of them is
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) any = fmaf(c[i], 0.f, any);
-    if (__any_sync(kAll, !(any == 0.f))) return kOdd;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) c[i] = __uint_as_float((__float_as_uint(c[i]) & ~kPlace) | (kPlace - i));
-  } else {
-#pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      c[i] = c[i] > -INFINITY ? __uint_as_float((__float_as_uint(c[i]) & ~kPlace) | (kPlace - i)) : -INFINITY;
+  for (int i = 0; i < VPL; ++i) {
+    const float v = c[i] + fminf(bias[i], FLT_MAX);
+    c[i] = c[i] > -INFINITY ? __uint_as_float((__float_as_uint(v) & ~kPlace) | (kPlace - i)) : -INFINITY;
   }
-  auto near = [&](float hi, float lo) { return !(hi - lo > kTol * fmaxf(1.f, fmaxf(fabsf(hi), fabsf(lo)))); };
-  const unsigned below = (1u << lane) - 1;
   if (GROUPS) {
     float mine = -INFINITY;              // lane g: group g's score
-    auto group_score = [&](int g, float top, float next) {
+    for (int g = 0; g < p.groups; ++g) {
+      float top = -INFINITY, next = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        const int e = i * 32 + lane - g * p.group_size;
+        const float v = e >= 0 && e < p.group_size ? c[i] : -INFINITY;
+        next = fmaxf(next, fminf(top, v));
+        top = fmaxf(top, v);
+      }
       const float first = warp_max_float(top);
       float sum = first;
       if (p.group_top == 2) {
         // the second largest: the lowest lane that holds the largest offers its next
-        const bool hold = top == first;
-        const unsigned holders = __ballot_sync(kAll, hold);
-        if (hold && !(holders & below)) top = next;
+        if (lane == __ffs(__ballot_sync(kAll, top == first)) - 1) top = next;
         const float second = warp_max_float(top);
         if (second > -INFINITY) sum += second;
       }
       if (lane == g) mine = sum;
-    };
+    }
     unsigned chosen = 0;
     float last = -INFINITY;
-    auto choose = [&]() {
-      for (int q = 0; q < p.top_groups; ++q) {
-        const bool open = !((chosen >> lane) & 1);
-        const float best = warp_max_float(open ? mine : -INFINITY);
-        if (best == -INFINITY) break;
-        const unsigned at = __ballot_sync(kAll, open && mine == best);
-        chosen |= at & (0u - at);
-        last = best;
-      }
-    };
-    auto by_registers = [&](auto regs) {
-      constexpr int RPG = decltype(regs)::value;
-#pragma unroll
-      for (int g = 0; g * RPG < VPL; ++g) {
-        float top = c[g * RPG], next = -INFINITY;
-#pragma unroll
-        for (int i = g * RPG + 1; i < (g + 1) * RPG && i < VPL; ++i) {
-          next = fmaxf(next, fminf(top, c[i]));
-          top = fmaxf(top, c[i]);
-        }
-        group_score(g, top, next);
-      }
-      choose();
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) c[i] = chosen & (1u << (i / RPG)) ? c[i] : -INFINITY;
-    };
-    // groups of 32, 64 or 128 experts are whole registers: compile-time loops, whose warp-wide maxima overlap
-    if (p.group_size == 32) {
-      by_registers(std::integral_constant<int, 1>());
-    } else if (p.group_size == 64) {
-      by_registers(std::integral_constant<int, 2>());
-    } else if (p.group_size == 128) {
-      by_registers(std::integral_constant<int, 4>());
-    } else {
-      for (int g = 0; g < p.groups; ++g) {
-        float top = -INFINITY, next = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const float v = grp[i] == g ? c[i] : -INFINITY;
-          next = fmaxf(next, fminf(top, v));
-          top = fmaxf(top, v);
-        }
-        group_score(g, top, next);
-      }
-      choose();
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) c[i] = (chosen >> grp[i]) & 1 ? c[i] : -INFINITY;
+    for (int q = 0; q < p.top_groups; ++q) {
+      const bool open = !((chosen >> lane) & 1);
+      const float best = warp_max_float(open ? mine : -INFINITY);
+      if (best == -INFINITY) break;
+      const unsigned at = __ballot_sync(kAll, open && mine == best);
+      chosen |= at & (0u - at);
+      last = best;
     }
     const float out = warp_max_float((chosen >> lane) & 1 ? -INFINITY : mine);
-    if (out > -INFINITY && near(0.5f * last, 0.5f * out)) return kNear;
+    if (out > -INFINITY && near_choices<VPL>(0.5f * last, 0.5f * out)) return kNear;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] = (chosen >> min((i * 32 + lane) / p.group_size, 31)) & 1 ? c[i] : -INFINITY;
   }
-  // Each lane keeps its DEPTH largest in order.  4 of 256 experts' 8 best share a lane in one row of five hundred;
-  // only the careful form then looks for the lane's next ones, below the last taken.
-  constexpr int kDepth = CAREFUL ? 3 : 4, DEPTH = VPL < kDepth ? VPL : kDepth;
+  // Each lane keeps its DEPTH largest in order; a lane whose DEPTH have all been taken looks for the next ones
+  // below the last taken.
+  constexpr int DEPTH = VPL < 3 ? VPL : 3;
   float top[DEPTH];
   auto fill = [&](float limit) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) top[d] = -INFINITY;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      float v = CAREFUL ? (c[i] < limit ? c[i] : -INFINITY) : c[i];
+      float v = c[i] < limit ? c[i] : -INFINITY;
 #pragma unroll
-      for (int d = 0; d < DEPTH && d <= i; ++d) {
+      for (int d = 0; d < DEPTH; ++d) {
         const float lower = fminf(top[d], v);
         top[d] = fmaxf(top[d], v);
         v = lower;
@@ -529,111 +490,287 @@ __device__ __forceinline__ RowState fast_row(const RouteArgs& p, int64_t t, int 
     }
   };
   fill(INFINITY);
-  int taken = 0, all_taken = 0;
-  float left_out = -INFINITY;
-  if (CAREFUL) {
-    if (lane < p.k) slots[lane] = make_float2(-INFINITY, 0.f);
-    __syncwarp();
-  }
+  int taken = 0;
+  unsigned all_taken = 0;
+  if (lane < p.k) slots[lane] = make_float2(-INFINITY, 0.f);
+  __syncwarp();
   for (int j = 0; j < p.k; ++j) {
     const float best = warp_max_float(top[0]);
-    if (CAREFUL && best == -INFINITY) break;
+    if (best == -INFINITY) break;
     if (top[0] == best) {                // one lane; two where choices are equal, found below
       slots[j] = make_float2(best, __int_as_float(lane));
 #pragma unroll
       for (int d = 0; d + 1 < DEPTH; ++d) top[d] = top[d + 1];
       top[DEPTH - 1] = -INFINITY;
       ++all_taken;
-      if (CAREFUL && VPL > DEPTH && ++taken == DEPTH) {
+      if (VPL > DEPTH && ++taken == DEPTH) {
         taken = 0;
         fill(best);
       }
     }
   }
-  left_out = warp_max_float(top[0]);
-  // an exhausted lane may hold more of the best than it offered
-  if (!CAREFUL && VPL > DEPTH && __any_sync(kAll, all_taken >= DEPTH)) return kOdd;
+  const float left_out = warp_max_float(top[0]);
   __syncwarp();
   const float2 slot = lane < p.k ? slots[lane] : make_float2(-INFINITY, 0.f);
   const float mine = slot.x;
   const bool on = mine > -INFINITY;
-  const int found = CAREFUL ? __popc(__ballot_sync(kAll, on)) : p.k;
-  if ((int)__reduce_add_sync(kAll, (unsigned)all_taken) != found) return kNear;      // equal choices
+  if ((int)__reduce_add_sync(kAll, all_taken) != __popc(__ballot_sync(kAll, on))) return kNear;      // equal choices
   const float up = __shfl_up_sync(kAll, mine, 1);
-  bool bad = on && lane > 0 && near(up, mine);
-  if (lane == p.k - 1 && left_out > -INFINITY) bad = bad || near(mine, left_out);
+  bool bad = on && lane > 0 && near_choices<VPL>(up, mine);
+  if (lane == p.k - 1 && left_out > -INFINITY) bad = bad || near_choices<VPL>(mine, left_out);
   if (__any_sync(kAll, bad)) return kNear;
-  id = on ? (int)(kPlace - (__float_as_uint(mine) & kPlace)) * 32 + __float_as_int(slot.y) : -1;
+  const int id = on ? (int)(kPlace - (__float_as_uint(mine) & kPlace)) * 32 + __float_as_int(slot.y) : -1;
   float w = 0.f;
   if (on) {
-    const int64_t from = t * p.ld + id;
-    float x = p.dtype == 0   ? static_cast<const float*>(p.logits)[from]
-              : p.dtype == 1 ? __half2float(static_cast<const __half*>(p.logits)[from])
-                             : __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[from]);
-    x = fminf(x, FLT_MAX);
+    const float x = logit_at(p, t, id);
     w = SOFTMAX ? expf(x - m) : 1.f / (1.f + expf(-x));
   }
   if (p.renorm) {
     const float total = warp_sum(w);
     w = total > 0.f ? w / total : 0.f;
   }
-  weight = w * p.scale;
+  store_row(p, t, lane, id, w * p.scale);
   return kDone;
 }
 
-// The careful form, a function of its own like the 64-bit pass.
-template <int VPL, bool SOFTMAX, bool GROUPS>
-__device__ __noinline__ RowState careful_row(const RouteArgs& p, int64_t t, int lane, float2* slots) {
-  float bias[VPL];
-  int grp[VPL];
-  load_bias<VPL, true>(p, lane, bias);
+// A row of all VPL * 32 experts, none of them off or below a logit of -88, without equal maxima, and with at
+// most DEPTH of the k best in one lane (kOdd where that does not hold).  Such rows are bound by the ALU pipe
+// (comparisons and selections, half the rate of the others), so the form has few of them: expert lane * VPL + i is
+// in register i, a group then is a run of lanes, and all groups' scores come from one pass over the registers
+// and log2(lanes) exchanges (25 instructions a group as maxima over the warp before).  The choices go to slots[0..k) as
+// (value, lane); `m` is the row's maximum (SOFTMAX), left_out the best choice that is left.
+template <int VPL>
+__device__ __forceinline__ void load_run(const RouteArgs& p, int64_t t, int lane, float (&x)[VPL]) {
+  const int64_t from = t * p.ld + lane * VPL;
+  if (p.dtype == 0) {
+    const float* row = static_cast<const float*>(p.logits) + from;
+    if (VPL % 4 == 0 && p.vec) {
 #pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    bias[i] = fminf(bias[i], FLT_MAX);
-    grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
-  }
-  int id;
-  float w;
-  const RowState state = fast_row<VPL, SOFTMAX, GROUPS, true>(p, t, lane, bias, grp, slots, id, w);
-  if (state == kDone) store_row(p, t, lane, id, w);
-  return state;
-}
-
-template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
-__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : VPL == 16 ? 2 : 1) route_kernel(const __grid_constant__ RouteArgs p) {
-  __shared__ float2 slots[8][kMaxTopK];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  float bias[VPL];
-  int grp[VPL];
-  load_bias<VPL, BIAS>(p, lane, bias);
-  bool odd = false;                      // an expert is off by its bias
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    odd = odd || (BIAS && !(bias[i] > -INFINITY));
-    bias[i] = fminf(bias[i], FLT_MAX);   // the 64-bit pass tells it from +inf
-    grp[i] = GROUPS ? min((i * 32 + lane) / p.group_size, 31) : 0;
-  }
-  odd = p.E != VPL * 32 || __any_sync(kAll, odd);
-  for (int64_t t = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp; t < p.T; t += warps) {
-    int id;
-    float w;
-    RowState state;
-    if (BIAS && (!SOFTMAX || p.renorm)) {   // softmax weights as they are want an accurate sum: the other pass
-      state = odd ? kOdd : fast_row<VPL, SOFTMAX, GROUPS, false>(p, t, lane, bias, grp, slots[warp], id, w);
-      if (state == kOdd) {
-        __syncwarp();
-        state = careful_row<VPL, SOFTMAX, GROUPS>(p, t, lane, slots[warp]);
-        if (state == kDone) continue;
+      for (int i = 0; i < VPL / 4; ++i) {
+        const float4 v = reinterpret_cast<const float4*>(row)[i];
+        x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
       }
     } else {
-      float x[VPL];
-      load_row<VPL, BIAS>(p, t, lane, bias, x);
-      state = route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w) ? kNear : kDone;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) x[i] = row[i];
     }
-    if (state == kNear) route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
-    else store_row(p, t, lane, id, w);
-    __syncwarp();
+  } else {
+    const uint16_t* row = static_cast<const uint16_t*>(p.logits) + from;
+    auto value = [&](uint32_t bits) {
+      return p.dtype == 1 ? __half2float(__ushort_as_half((unsigned short)bits)) : __uint_as_float(bits << 16);
+    };
+    if (VPL % 8 == 0 && p.vec) {
+#pragma unroll
+      for (int i = 0; i < VPL / 8; ++i) {
+        const uint4 v = reinterpret_cast<const uint4*>(row)[i];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[8 * i + j] = value(w[j / 2] >> (16 * (j & 1)) & 0xffffu);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) x[i] = value(row[i]);
+    }
+  }
+}
+
+template <int VPL, bool SOFTMAX, bool GROUPS>
+__device__ __forceinline__ RowState quick_row(const RouteArgs& p, int lane, float (&c)[VPL], const float (&bias)[VPL],
+                                              float2* slots, float& m, float& left_out) {
+  constexpr uint32_t kPlace = VPL - 1;
+  if (SOFTMAX) {
+    float mx = c[0];
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) mx = fmaxf(mx, c[i]);
+    m = warp_max_float(mx);
+    float z = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      // NaN from a logit of NaN or an infinity, 1/0 * 0 from one too far below (its exponential is 0)
+      const float e = exp2_approx((c[i] - m) * kLog2e);
+      z += e;
+      c[i] = fmaf(reciprocal_approx(e), 0.f, e);
+    }
+    z = reciprocal_approx(warp_sum(z));
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] = fmaf(c[i], z, bias[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      // a logit of +inf scores 1; NaN from a logit of NaN, inf * 0 from one that is -inf or below -88
+      const float e = exp2_approx(c[i] * -kLog2e);
+      c[i] = fmaf(e, 0.f, reciprocal_approx(1.f + e) + bias[i]);
+    }
+  }
+  float any = 0.f;                       // NaN if one of them is
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) any = fmaf(c[i], 0.f, any);
+  if (__any_sync(kAll, !(any == 0.f))) return kOdd;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) c[i] = __uint_as_float((__float_as_uint(c[i]) & ~kPlace) | (kPlace - i));
+  if (GROUPS) {
+    float top = c[0], next = -INFINITY;
+#pragma unroll
+    for (int i = 1; i < VPL; ++i) {
+      next = fmaxf(next, fminf(top, c[i]));
+      top = fmaxf(top, c[i]);
+    }
+    for (int o = 1; o < p.group_lanes; o <<= 1) {
+      const float t2 = __shfl_xor_sync(kAll, top, o), n2 = __shfl_xor_sync(kAll, next, o);
+      next = fmaxf(fmaxf(next, n2), fminf(top, t2));
+      top = fmaxf(top, t2);
+    }
+    // every lane holds its group's score; -inf once the group is chosen
+    float mine = p.group_top == 2 && p.group_size > 1 ? top + next : top;
+    bool chosen = false;
+    float last = 0.f;
+    for (int q = 0; q < p.top_groups; ++q) {
+      last = warp_max_float(mine);
+      if (mine == last) {                // one group; more where scores are equal, found below
+        chosen = true;
+        mine = -INFINITY;
+      }
+    }
+    const float out = warp_max_float(mine);
+    if (__popc(__ballot_sync(kAll, chosen)) != p.top_groups * p.group_lanes) return kNear;
+    if (out > -INFINITY && near_choices<VPL>(0.5f * last, 0.5f * out)) return kNear;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) c[i] = chosen ? c[i] : -INFINITY;
+  }
+  constexpr int DEPTH = VPL < 4 ? VPL : 4;
+  float top[DEPTH];
+#pragma unroll
+  for (int d = 0; d < DEPTH; ++d) top[d] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    float v = c[i];
+#pragma unroll
+    for (int d = 0; d < DEPTH && d <= i; ++d) {
+      const float lower = fminf(top[d], v);
+      top[d] = fmaxf(top[d], v);
+      v = lower;
+    }
+  }
+  unsigned taken = 0;
+  for (int j = 0; j < p.k; ++j) {
+    const float best = warp_max_float(top[0]);
+    if (top[0] == best) {                // one lane; more where choices are equal or have run out, found below
+      slots[j] = make_float2(best, __int_as_float(lane));
+#pragma unroll
+      for (int d = 0; d + 1 < DEPTH; ++d) top[d] = top[d + 1];
+      top[DEPTH - 1] = -INFINITY;
+      ++taken;
+    }
+  }
+  left_out = warp_max_float(top[0]);
+  // an exhausted lane may hold more of the best than it offered
+  if (VPL > DEPTH && __any_sync(kAll, taken >= DEPTH)) return kOdd;
+  return __reduce_add_sync(kAll, taken) == (unsigned)p.k ? kDone : kNear;
+}
+
+// A warp takes `batch` neighbouring rows at a time: quick_row one after the other, then the weights and stores of
+// all of them together, row b's slot j in lane b * width + j.
+template <int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
+__global__ void __launch_bounds__(256, VPL <= 8 ? 4 : VPL == 16 ? 2 : 1) route_kernel(const __grid_constant__ RouteArgs p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5), me = (int64_t)blockIdx.x * (blockDim.x >> 5) + warp;
+  if constexpr (!BIAS) {
+    float bias[VPL];
+    for (int64_t t = me; t < p.T; t += warps) {
+      float x[VPL];
+      load_row<VPL, false>(p, t, lane, bias, x);
+      int id;
+      float w;
+      if (route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w))
+        route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
+      else
+        store_row(p, t, lane, id, w);
+    }
+  } else {
+    __shared__ float2 all_slots[8][kMaxTopK];
+    float2* const slots = all_slots[warp];
+    if (SOFTMAX && !p.renorm) {          // weights as they are want an accurate sum: the other pass
+      float bias[VPL];
+      load_bias<VPL, BIAS>(p, lane, bias);
+      for (int64_t t = me; t < p.T; t += warps) {
+        float x[VPL];
+        load_row<VPL, BIAS>(p, t, lane, bias, x);
+        int id;
+        float w;
+        if (route_row<float, VPL, SOFTMAX, BIAS, GROUPS>(p, x, bias, lane, id, w))
+          route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t, lane);
+        else
+          store_row(p, t, lane, id, w);
+      }
+      return;
+    }
+    constexpr uint32_t kPlace = VPL - 1;
+    float bias[VPL];
+    bool odd = p.E != VPL * 32 || (GROUPS && p.group_lanes == 0);
+    if (!odd) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        bias[i] = p.bias[lane * VPL + i];
+        odd = odd || !(bias[i] > -INFINITY);           // off by its bias
+        bias[i] = fminf(bias[i], FLT_MAX);             // the 64-bit pass tells it from +inf
+      }
+    }
+    odd = __any_sync(kAll, odd);
+    const int shift = p.k <= 4 ? 2 : p.k <= 8 ? 3 : p.k <= 16 ? 4 : 5, width = 1 << shift;
+    for (int64_t t0 = me * p.batch; t0 < p.T; t0 += warps * p.batch) {
+      const int rows = (int)min((int64_t)p.batch, p.T - t0);
+      unsigned odd_rows = odd ? (1u << rows) - 1 : 0, near_rows = 0;
+      float m = 0.f, left_out = -INFINITY;             // of this lane's row below
+      if (!odd) {
+        float c[VPL], ahead[VPL];
+        load_run<VPL>(p, t0, lane, ahead);
+        for (int b = 0; b < rows; ++b) {
+#pragma unroll
+          for (int i = 0; i < VPL; ++i) c[i] = ahead[i];
+          if (b + 1 < rows) load_run<VPL>(p, t0 + b + 1, lane, ahead);
+          float row_m = 0.f, row_out = -INFINITY;
+          const RowState state = quick_row<VPL, SOFTMAX, GROUPS>(p, lane, c, bias, slots + b * width, row_m, row_out);
+          if (state == kOdd) odd_rows |= 1u << b;
+          if (state == kNear) near_rows |= 1u << b;
+          if ((lane >> shift) == b) m = row_m, left_out = row_out;
+        }
+        __syncwarp();
+        const int b = (lane >> shift), j = lane & (width - 1);
+        const bool on = j < p.k && b < rows && !(((odd_rows | near_rows) >> b) & 1);
+        const float2 slot = on ? slots[lane] : make_float2(0.f, 0.f);
+        const float mine = slot.x;
+        const float up = __shfl_up_sync(kAll, mine, 1);
+        const bool bad = on && ((j > 0 && near_choices<VPL>(up, mine)) ||
+                                (j == p.k - 1 && left_out > -INFINITY && near_choices<VPL>(mine, left_out)));
+        const unsigned bad_lanes = __ballot_sync(kAll, bad);
+        const int id = (int)(__float_as_int(slot.y) * VPL + (kPlace - (__float_as_uint(mine) & kPlace)));
+        float w = 0.f;
+        if (on) {
+          const float x = logit_at(p, t0 + b, id);
+          w = SOFTMAX ? expf(x - m) : 1.f / (1.f + expf(-x));
+        }
+        if (p.renorm) {
+          float total = w;
+          for (int o = width / 2; o; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
+          w = total > 0.f ? w / total : 0.f;
+        }
+        const unsigned first_row = width == 32 ? kAll : (1u << width) - 1, row_lanes = first_row << (b << shift);
+        if (on && !(bad_lanes & row_lanes)) {
+          p.ids[(t0 + b) * p.k + j] = id;
+          p.weights[(t0 + b) * p.k + j] = w * p.scale;
+        }
+        for (int r = 0; r < rows; ++r)
+          if (bad_lanes & (first_row << (r << shift))) near_rows |= 1u << r;
+        __syncwarp();
+      }
+      for (unsigned left = odd_rows; left; left &= left - 1) {
+        const int r = __ffs(left) - 1;
+        if (careful_row<VPL, SOFTMAX, GROUPS>(p, t0 + r, lane, slots) == kNear) near_rows |= 1u << r;
+        __syncwarp();
+      }
+      for (unsigned left = near_rows; left; left &= left - 1)
+        route_row_in_64_bits<VPL, SOFTMAX, BIAS, GROUPS>(p, t0 + __ffs(left) - 1, lane);
+    }
   }
 }
 
@@ -646,8 +783,14 @@ int launch_route(const RouteArgs& p, bool softmax, cudaStream_t stream) {
       route_kernel<VPL, false, true, false>,  route_kernel<VPL, false, true, true>,
       route_kernel<VPL, true, false, false>,  route_kernel<VPL, true, false, true>,
       route_kernel<VPL, true, true, false>,   route_kernel<VPL, true, true, true>};
-  const int64_t ctas = std::min<int64_t>((p.T + 7) / 8, (int64_t)sm_count() * 8);
-  table[softmax * 4 + b * 2 + g]<<<(unsigned)ctas, 256, 0, stream>>>(p);
+  RouteArgs q = p;
+  const int lanes = p.group_size / VPL;
+  q.group_lanes = g && p.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  // as many rows a batch as its lanes hold, if that leaves every SM its 32 warps
+  const int most = p.k <= 4 ? 8 : p.k <= 8 ? 4 : p.k <= 16 ? 2 : 1;
+  q.batch = (int)std::max<int64_t>(1, std::min<int64_t>(most, p.T / ((int64_t)sm_count() * 32)));
+  const int64_t ctas = std::min<int64_t>((p.T + 8 * q.batch - 1) / (8 * q.batch), (int64_t)sm_count() * 8);
+  table[softmax * 4 + b * 2 + g]<<<(unsigned)ctas, 256, 0, stream>>>(q);
   return check_launch("route_kernel");
 }
 
@@ -679,6 +822,9 @@ extern "C" int nvfp4_route_experts(const void* logits, int dtype, int64_t T, int
   p.group_top = group_top; p.group_size = (int)(E / groups);
   p.renorm = renorm; p.scale = scale;
   p.dtype = dtype;
+  p.vec = aligned16(logits) && (ld * (int64_t)size % 16 == 0 || T == 1);
+  p.group_lanes = 0;
+  p.batch = 1;
   const bool softmax = score == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int vpl = (p.E + 31) / 32;

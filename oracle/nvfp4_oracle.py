@@ -463,7 +463,9 @@ def lora_add(base, x, a, b, adapters, scales=None, ranks=None):
     sum over K and the sum over r are off by at most their number of terms (in
     mma steps of 16, each adding 16 products and rounding or truncating at most
     twice, plus 24 joined partial sums) times 2^-23 of their magnitudes, u's two
-    halves by 2^-21, and the result is rounded to fp16 once."""
+    halves by 2^-21, and the result is rounded to fp16 once.  The second sum may
+    start from base: its 2 r / 16 mma steps then round or truncate a value of
+    base's size, too."""
     base, x, a, b = (t.detach().cpu().double().numpy() for t in (base, x, a, b))
     ids = adapters.detach().cpu().numpy()
     n, r, K = a.shape
@@ -480,4 +482,5 @@ def lora_add(base, x, a, b, adapters, scales=None, ranks=None):
         out[t] += s * (bi @ u)
         eu = (K / 16 + 24) * 2.0 ** -23 * ua + 2.0 ** -21 * (np.abs(u).max() if rank else 0.0)
         tol[t] = abs(s) * (np.abs(bi) @ (eu + (2 * r / 16 + 8) * 2.0 ** -23 * np.abs(u)))
+        tol[t] += 2 * r / 16 * 2.0 ** -23 * np.abs(base[t])
     return out, tol + (np.abs(out) + tol) * 2.0 ** -11 + 2.0 ** -24

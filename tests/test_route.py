@@ -177,3 +177,28 @@ def test_route_refusals(pkg, cuda):
         pkg.route_experts(torch.zeros((8, 4), device=cuda).t(), 2)
     with pytest.raises(ValueError, match="ids"):
         pkg.route_experts(x, 2, ids=torch.zeros((4, 2), dtype=torch.int64, device=cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,groups,top_groups,off", [
+    (20001, 256, 8, 8, 4, 0), (10007, 256, 3, 16, 2, 0), (9600, 128, 8, 1, 1, 1), (40001, 32, 2, 32, 5, 0), (9500, 64, 16, 4, 3, 4)])
+def test_route_many_rows(pkg, oracle, cuda, T, E, k, groups, top_groups, off, dtype, score):
+    """Enough rows for a warp to take several at once; some masked, equal or
+    far apart among them, and an unaligned row start."""
+    g = torch.Generator().manual_seed(T + E)
+    x = torch.randn((T, E + off), generator=g).mul(2).to(dtype)
+    x[5::97, ::3] = -math.inf
+    x[6::97] = 0.5
+    x[7::97, 1::2] = -1000.0
+    x[8::97, 4:9] = 3.0
+    x[9::97] = math.nan
+    bias = (torch.randn(E, generator=g) * 0.1).to(cuda)
+    x = x.to(cuda)[:, off:]
+    w, ids = pkg.route_experts(x, k, bias=bias, score=score, num_groups=groups, top_groups=top_groups)
+    rows = torch.unique(torch.cat([torch.arange(0, T, 61), torch.arange(5, T, 97), torch.arange(6, T, 97),
+                                   torch.arange(7, T, 97), torch.arange(8, T, 97), torch.arange(9, T, 97), torch.tensor([T - 1])]))
+    rw, ri = oracle.route(x[rows.to(cuda)], k, bias, score=score, groups=groups, top_groups=top_groups)
+    np.testing.assert_array_equal(ids[rows.to(cuda)].cpu().numpy(), ri)
+    np.testing.assert_allclose(w[rows.to(cuda)].cpu().numpy().astype(np.float64), rw, rtol=RTOL, atol=ATOL)
