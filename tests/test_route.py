@@ -182,9 +182,11 @@ def test_route_refusals(pkg, cuda):
 @pytest.mark.gpu
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("with_bias", [True, False])
 @pytest.mark.parametrize("T,E,k,groups,top_groups,off", [
-    (20001, 256, 8, 8, 4, 0), (10007, 256, 3, 16, 2, 0), (9600, 128, 8, 1, 1, 1), (40001, 32, 2, 32, 5, 0), (9500, 64, 16, 4, 3, 4)])
-def test_route_many_rows(pkg, oracle, cuda, T, E, k, groups, top_groups, off, dtype, score):
+    (20001, 256, 8, 8, 4, 0), (10007, 256, 3, 16, 2, 0), (9600, 128, 8, 1, 1, 1), (40001, 32, 2, 32, 5, 0), (9500, 64, 16, 4, 3, 4),
+    (9777, 60, 4, 1, 1, 0), (9600, 160, 6, 20, 3, 0)])
+def test_route_many_rows(pkg, oracle, cuda, T, E, k, groups, top_groups, off, with_bias, dtype, score):
     """Enough rows for a warp to take several at once; some masked, equal or
     far apart among them, and an unaligned row start."""
     g = torch.Generator().manual_seed(T + E)
@@ -194,7 +196,7 @@ def test_route_many_rows(pkg, oracle, cuda, T, E, k, groups, top_groups, off, dt
     x[7::97, 1::2] = -1000.0
     x[8::97, 4:9] = 3.0
     x[9::97] = math.nan
-    bias = (torch.randn(E, generator=g) * 0.1).to(cuda)
+    bias = (torch.randn(E, generator=g) * 0.1).to(cuda) if with_bias else None
     x = x.to(cuda)[:, off:]
     w, ids = pkg.route_experts(x, k, bias=bias, score=score, num_groups=groups, top_groups=top_groups)
     rows = torch.unique(torch.cat([torch.arange(0, T, 61), torch.arange(5, T, 97), torch.arange(6, T, 97),
