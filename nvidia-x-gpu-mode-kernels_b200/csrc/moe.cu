@@ -180,15 +180,15 @@ struct MoeLayout {
   int64_t tiles, row, row_weight, xq, xs, hq, hs, y, bytes;
 };
 
-// Into how many parts the down product of few tokens cuts its inner dimension, so that its tiles fill the SMs:
-// the count with the fewest stages on the busiest SM, if every expert that can be active is.  A part more
+// Into how many parts the down product of few tokens cuts its inner dimension where its tiles would leave SMs
+// idle: the count with the fewest stages on the busiest SM, if every expert that can be active is.  A part more
 // costs a y to write and to read again, which is counted at half a stage (32 KB of weights).
 int down_parts(int64_t n, int64_t E, int64_t D, int64_t F, int tile) {
   const int64_t tiles = std::max<int64_t>(1, std::min<int64_t>(std::min(n, E) + n / tile, n)) * ((D + 127) / 128);
   const int64_t stages = (F + 511) / 512, sms = sm_count();
   int best = 1;
   double least = 1e30;
-  for (int64_t s = 1; s <= std::min<int64_t>(8, stages); ++s) {
+  for (int64_t s = 1; s <= std::min<int64_t>(8, stages) && (s == 1 || tiles < sms); ++s) {
     const double cost = (double)((tiles * s + sms - 1) / sms) * ((stages + s - 1) / s) + 0.5 * (s - 1);
     if (cost < least - 1e-9) {
       least = cost;
@@ -201,8 +201,11 @@ int down_parts(int64_t n, int64_t E, int64_t D, int64_t F, int tile) {
 MoeLayout moe_layout(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F) {
   MoeLayout m;
   const int64_t n = T * k;
-  m.trans = n <= 64 * E;
-  m.tile = !m.trans ? 128 : n <= 8 * E ? 16 : n <= 16 * E ? 32 : 64;
+  // 16-token tiles up to 16 rows an expert, 128-row tiles above.  64 experts of 2048 x 1024, us: 16 rows an expert
+  // 58.9 and 57.9, 8 rows 51.5 and 54.8, 32 rows 78 and 66; 8 experts of 4096 x 14336: 4 rows 124 and 135, 16 rows 146
+  // and 149, 24 rows 172 and 139.  Tiles of 32 and 64 tokens are slower than one or the other everywhere.
+  m.trans = n <= 16 * E;
+  m.tile = m.trans ? 16 : 128;
   m.parts = m.trans ? down_parts(n, E, D, F, m.tile) : 1;
   m.rows = (plan_max_rows(n, E, m.tile) + 127) / 128 * 128;
   m.max_tiles = plan_max_tiles(n, E, m.tile);
@@ -405,7 +408,5 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
   c.err = device_error_word();
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
   if (!m.trans) return moe_run<ExpertCfg<false, true, 128, 1, 4>, ExpertCfg<false, false, 256, 1, 4>>(c);
-  if (m.tile == 16) return moe_run<ExpertCfg<true, true, 16, 1, 5>, ExpertCfg<true, false, 16, 2, 5>>(c);
-  if (m.tile == 32) return moe_run<ExpertCfg<true, true, 32, 1, 4>, ExpertCfg<true, false, 32, 2, 4>>(c);
-  return moe_run<ExpertCfg<true, true, 64, 1, 4>, ExpertCfg<true, false, 64, 2, 4>>(c);
+  return moe_run<ExpertCfg<true, true, 16, 1, 5>, ExpertCfg<true, false, 16, 2, 5>>(c);
 }

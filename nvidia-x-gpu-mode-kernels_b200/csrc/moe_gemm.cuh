@@ -12,9 +12,9 @@
 //
 // TRANS 0: the tokens are the MMA's 128-row operand, BN weight rows its other
 // one; an epilogue thread holds one token's row.  TRANS 1, for few tokens per
-// expert: 128 weight rows are the MMA's first operand and BN tokens (16, 32 or
-// 64) the other, so the tensor cores' work shrinks with the tokens and the
-// weights stream; an epilogue lane holds one weight row of every token.
+// expert: 128 weight rows are the MMA's first operand and BN = 16 tokens the
+// other, so the tensor cores' work shrinks with the tokens and the weights
+// stream; an epilogue lane holds one weight row of every token.
 //
 // Warp roles: warp 0 TMA producer of the operands, warp 1 MMA, then the
 // epilogue's warps, four that copy the scales into tensor memory, and the
@@ -69,7 +69,7 @@ struct ExpertCfg {
   static constexpr int W_ROWS = TRANS ? BM : BN;           // weight rows per tile
   static constexpr int NBW = W_ROWS / 128;                 // scale blocks of a weight tile
   static_assert(W_ROWS % 128 == 0, "weight tiles are whole scale blocks");
-  static_assert(!TRANS || BN == 16 || BN == 32 || BN == 64, "token tiles");
+  static_assert(!TRANS || BN == 16, "token tiles");
   // One MMA does it where the weights are its second operand: the gate rows and the up rows of a K atom lie one
   // after the other, as its N = 2 BN rows.
   static constexpr int MMA_N = TRANS ? BN : NW * BN;
@@ -86,11 +86,13 @@ struct ExpertCfg {
   static constexpr int OFF_BUF = OFF_BAR + 512;            // TRANS && DUAL: a 16 x 36 float patch per epilogue warp
   static constexpr int BUF_BYTES = TRANS && DUAL ? 4 * 16 * 36 * 4 : 0;
   static constexpr int SMEM = OFF_BUF + BUF_BYTES;
-  static_assert((3 * STAGES + 2) * 8 + 4 <= 512, "barriers");
+  static_assert((3 * STAGES + 4) * 8 + 4 <= 512, "barriers");
   static constexpr uint32_t OP_BYTES = T_BYTES + NW * W_BYTES;
   static constexpr uint32_t SF_BYTES = SFT_BYTES + NW * SFW_BYTES;
   // tensor memory columns
-  static constexpr int SF_BASE = NW * BN;                  // the accumulators come first
+  static constexpr int BUFS = TRANS ? 2 : 1;               // accumulators of two tiles where they fit
+  static constexpr int ACC_COLS = NW * BN;
+  static constexpr int SF_BASE = BUFS * ACC_COLS;          // the accumulators come first
   static constexpr int SFT_COLS = 4 * KPS;
   static constexpr int SFW_COLS = KPS * NW * NBW * 4;      // [K block][matrix][128 rows]
   static constexpr int SF_STAGE_COLS = SFT_COLS + SFW_COLS;
@@ -146,9 +148,9 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   const uint32_t bar_full = sbase + C::OFF_BAR;             // operand boxes landed and scales staged in tensor memory
   const uint32_t bar_empty = bar_full + 8 * C::STAGES;      // stage consumed by the MMAs
   const uint32_t bar_sff = bar_empty + 8 * C::STAGES;       // scale boxes landed
-  const uint32_t bar_accf = bar_sff + 8 * C::STAGES;
-  const uint32_t bar_acce = bar_accf + 8;
-  const uint32_t tmem_slot = bar_acce + 8;
+  const uint32_t bar_accf = bar_sff + 8 * C::STAGES;        // accumulators finished, one barrier a buffer
+  const uint32_t bar_acce = bar_accf + 8 * C::BUFS;         // and read
+  const uint32_t tmem_slot = bar_acce + 8 * C::BUFS;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
@@ -156,8 +158,10 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       mbar_init(bar_empty + 8 * s, 1);
       mbar_init(bar_sff + 8 * s, 1);
     }
-    mbar_init(bar_accf, 1);
-    mbar_init(bar_acce, C::EPI_WARPS);
+    for (int b = 0; b < C::BUFS; ++b) {
+      mbar_init(bar_accf + 8 * b, 1);
+      mbar_init(bar_acce + 8 * b, C::EPI_WARPS);
+    }
     fence_mbar_init();
     prefetch_tmap(&P.tt);
     prefetch_tmap(&P.tst);
@@ -268,7 +272,8 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
       const uint64_t dt0 = tc::desc_sw128(sbase), dw0 = tc::desc_sw128(sbase + C::OFF_W);
       uint32_t it = 0, tile_it = 0;
       for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
-        if (!mbar_wait(bar_acce, (tile_it & 1) ^ 1, P.err, kDevErrTimeoutMma)) goto done;
+        const uint32_t buf = tile_it % C::BUFS, acc = tmem + buf * C::ACC_COLS;
+        if (!mbar_wait(bar_acce + 8 * buf, ((tile_it / C::BUFS) & 1) ^ 1, P.err, kDevErrTimeoutMma)) goto done;
         tc::fence_after_sync();
         const int first = from_stage(t), last = to_stage(t);
         bool ready = false;                                 // the stage is known to be there
@@ -288,15 +293,15 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
               // the pipe nothing.
               if (kk == C::KPS - 1 && ks + 1 < last)
                 ready = mbar_test(bar_full + 8 * ((it + 1) % C::STAGES), ((it + 1) / C::STAGES) & 1);
-              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
+              expert_mma<C>(acc, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
             }
           } else {
             for (int kk = 0; kk < nch; ++kk)
-              expert_mma<C>(tmem, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
+              expert_mma<C>(acc, dt0 + soff, dw0 + soff, sf, sf + C::SFT_COLS, kk, (ks > first || kk > 0) ? 1u : 0u);
           }
           tc::commit(bar_empty + 8 * s);
         }
-        tc::commit(bar_accf);
+        tc::commit(bar_accf + 8 * buf);
       }
     }
   } else if (warp >= 2 + C::EPI_WARPS) {
@@ -324,10 +329,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
           if constexpr (!C::TRANS) {
             v = *reinterpret_cast<const uint4*>(st + C::OFF_SFT + kk * 512 + from);
             tc::st_32x32b_x4(sf + 4 * kk, v.x, v.y, v.z, v.w);
-          } else if constexpr (C::BN == 64) {            // off is 0 or 64: two words, 8-byte aligned
-            const uint2 u = *reinterpret_cast<const uint2*>(st + C::OFF_SFT + kk * 512 + from);
-            tc::st_32x32b_x2(sf + 4 * kk, u.x, u.y);
-          } else {                                       // one column of up to 32 tokens
+          } else {                                       // one column of 16 tokens
             const uint32_t u = *reinterpret_cast<const uint32_t*>(st + C::OFF_SFT + kk * 512 + from);
             tc::st_32x32b_x2(sf + 4 * kk, u, u);
           }
@@ -348,69 +350,59 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
   } else {
     // ---------------------------- epilogue ----------------------------
     const int sub = warp & 3;                 // tensor-memory lane quarter of this warp
-    const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16);
     uint32_t tile_it = 0;
     auto release = [&] {                      // the accumulators are read: the next tile's MMAs may start
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_acce);
+      if (lane == 0) mbar_arrive(bar_acce + 8 * (tile_it % C::BUFS));
     };
     for (int t = blockIdx.x; t < total; t += gridDim.x, ++tile_it) {
       const PlanTile q = load_tile(P.tiles + t / wtiles);
       const int local = t / parts - q.first * P.wtiles;
       const int t0 = local % q.tiles * C::T_ROWS, w0 = local / q.tiles * C::W_ROWS;
-      if (!mbar_wait(bar_accf, tile_it & 1, P.err, kDevErrTimeoutMma)) break;
+      const uint32_t acc = tmem + ((uint32_t)(sub * 32) << 16) + tile_it % C::BUFS * C::ACC_COLS;
+      if (!mbar_wait(bar_accf + 8 * (tile_it % C::BUFS), (tile_it / C::BUFS) & 1, P.err, kDevErrTimeoutMma)) break;
       tc::fence_after_sync();
       if constexpr (C::TRANS && C::DUAL) {
-        // lane = weight row, column = token: 16 tokens at a time through a patch of shared memory, so
-        // that a lane gets one token's block of 16 weight rows
+        // lane = weight row, column = token: through a patch of shared memory, so that a lane gets one
+        // token's block of 16 weight rows
         float* buf = reinterpret_cast<float*>(smem_raw + C::OFF_BUF) + sub * 16 * 36;
         const int blk = (w0 + sub * 32) / 16 + (lane & 1);
-#pragma unroll 1
-        for (int cb = 0; cb < C::BN / 16; ++cb) {
-          uint32_t g[32], u[32];
-          tc::ld_32x32b_x16(acc + cb * 16, g);
-          tc::ld_32x32b_x16(acc + C::BN + cb * 16, u);
-          tc::wait_ld();
-          if (cb == C::BN / 16 - 1) release();
+        uint32_t g[32], u[32];
+        tc::ld_32x32b_x16(acc, g);
+        tc::ld_32x32b_x16(acc + C::BN, u);
+        tc::wait_ld();
+        release();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) buf[j * 36 + lane] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
-          __syncwarp();
-          float v[16];
+        for (int j = 0; j < 16; ++j) buf[j * 36 + lane] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
+        __syncwarp();
+        float v[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float4 f = *reinterpret_cast<const float4*>(buf + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * j);
-            v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
-          }
-          __syncwarp();
-          const int tok = t0 + cb * 16 + (lane >> 1);
-          if (tok < q.rows && blk * 16 < P.N) {
-            const int row = q.row0 + tok;
-            uint32_t packed[2];
-            const uint32_t sbyte = quant_floats(v, packed);
-            *reinterpret_cast<uint2*>(P.codes + (int64_t)row * (P.N / 2) + blk * 8) = make_uint2(packed[0], packed[1]);
-            P.sf[blocked_at(row, blk, P.N / 64)] = (uint8_t)sbyte;
-          }
+        for (int j = 0; j < 4; ++j) {
+          const float4 f = *reinterpret_cast<const float4*>(buf + (lane >> 1) * 36 + (lane & 1) * 16 + 4 * j);
+          v[4 * j] = f.x; v[4 * j + 1] = f.y; v[4 * j + 2] = f.z; v[4 * j + 3] = f.w;
+        }
+        __syncwarp();
+        const int tok = t0 + (lane >> 1);
+        if (tok < q.rows && blk * 16 < P.N) {
+          const int row = q.row0 + tok;
+          uint32_t packed[2];
+          const uint32_t sbyte = quant_floats(v, packed);
+          *reinterpret_cast<uint2*>(P.codes + (int64_t)row * (P.N / 2) + blk * 8) = make_uint2(packed[0], packed[1]);
+          P.sf[blocked_at(row, blk, P.N / 64)] = (uint8_t)sbyte;
         }
       } else if constexpr (C::TRANS) {
-        constexpr int CHUNK = C::BN < 32 ? C::BN : 32;
         const int col = w0 + sub * 32 + lane;
         float* const y = P.y + t % parts * P.part_stride;
-#pragma unroll 1
-        for (int cb = 0; cb < C::BN / CHUNK; ++cb) {
-          uint32_t v[32];
-          if constexpr (CHUNK == 32) tc::ld_32x32b_x32(acc + cb * 32, v);
-          else tc::ld_32x32b_x16(acc + cb * CHUNK, v);
-          tc::wait_ld();
-          if (cb == C::BN / CHUNK - 1) release();
-          if (col < P.N) {
+        uint32_t v[32];
+        tc::ld_32x32b_x16(acc, v);
+        tc::wait_ld();
+        release();
+        if (col < P.N) {
 #pragma unroll
-            for (int j = 0; j < CHUNK; ++j) {
-              const int tok = t0 + cb * CHUNK + j;
-              if (tok < q.rows)
-                y[(int64_t)(q.row0 + tok) * P.N + col] = P.row_weight[q.row0 + tok] * __uint_as_float(v[j]);
-            }
-          }
+          for (int j = 0; j < 16; ++j)
+            if (t0 + j < q.rows)
+              y[(int64_t)(q.row0 + t0 + j) * P.N + col] = P.row_weight[q.row0 + t0 + j] * __uint_as_float(v[j]);
         }
       } else {
         // thread = token row, warp = a quarter of the columns: all of them into registers first
