@@ -70,7 +70,8 @@ __global__ void __launch_bounds__(256) scatter_kernel(const int* rows, ScatterAr
 
 // Plan and scatter in one launch, for few slots: every CTA (one per token) counts all of them for itself and
 // finds the rows of its own token's, a warp a slot: its expert's first row plus the number of equal ids before
-// it.  CTA 0 lists the tiles.  Against the two kernels one after the other: 3 us less at 512 slots.
+// it.  CTA 0 lists the tiles.  Against the two kernels one after the other: 2.7 us less a call for one token, 1.4 at
+// 512 slots; with 2048 as the limit 2000 tokens take 64 us instead of 55.
 constexpr int kFusedSlots = 1024;
 
 __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __restrict__ ids, int n, int experts, int align,
@@ -142,6 +143,7 @@ __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __rest
 }
 
 // out[t] = sum of its slots' rows of y, in slot order (and of the parts of each); eight columns a thread.
+// 4096 tokens of 4096 columns in 2 slots each: it ends 38 us after the down product, 4.4 TB/s of y (fp32) and out.
 __global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ y, int parts, int64_t part_stride,
                                                       const int* __restrict__ rows, int64_t T, int k, int D,
                                                       __half* __restrict__ out, int64_t ldo, int vec) {

@@ -33,8 +33,10 @@
 // and one barrier a stage).  What bounds a stage of 256 elements then is the
 // round trip of the ring: 4 slots of 54 KB, all of shared memory, each taking
 // 0.3 us from the MMAs' end to its refill, 1.4 us until the operands land and
-// 0.28 us of MMAs.  CTA pairs (38 KB a stage, 5 slots) measured the same within
-// 2 %, prefetching weights into L2 slower.  Under minutes of such work the power
+// 0.28 us of MMAs.  Stages of 512 elements, two of them: 468 us.  CTA pairs (38 KB
+// a stage, 5 slots; before the one MMA for both): 935 us a call against 954, the
+// gate and up product alone slower (516 against 481).  Prefetching weights into
+// L2: no gain.  Under minutes of such work the power
 // limit takes another 15 % (768 us a call before it sets in, 913 after).
 #pragma once
 #include "plan.cuh"
