@@ -44,12 +44,13 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = 
         bias_at = bias.data_ptr()
     if weights is None:
         weights = logits.new_empty((T, top_k), dtype=torch.float32)
-    elif weights.dtype != torch.float32 or weights.shape != (T, top_k) or weights.get_device() != index \
-            or not weights.is_contiguous():
+    elif not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.shape != (T, top_k) \
+            or weights.get_device() != index or not weights.is_contiguous():
         raise ValueError(f"weights must be a contiguous float32 tensor [{T}, {top_k}] on the device of logits")
     if ids is None:
         ids = logits.new_empty((T, top_k), dtype=torch.int32)
-    elif ids.dtype != torch.int32 or ids.shape != (T, top_k) or ids.get_device() != index or not ids.is_contiguous():
+    elif not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.shape != (T, top_k) \
+            or ids.get_device() != index or not ids.is_contiguous():
         raise ValueError(f"ids must be a contiguous int32 tensor [{T}, {top_k}] on the device of logits")
     _lib.call("nvfp4_route_experts", index, logits.data_ptr(), _DTYPES[logits.dtype], T, E, strides[0], bias_at,
               _SCORES[score], top_k, num_groups, top_groups, group_top, renormalize, scale, weights.data_ptr(),

@@ -204,3 +204,12 @@ def test_route_many_rows(pkg, oracle, cuda, T, E, k, groups, top_groups, off, wi
     rw, ri = oracle.route(x[rows.to(cuda)], k, bias, score=score, groups=groups, top_groups=top_groups)
     np.testing.assert_array_equal(ids[rows.to(cuda)].cpu().numpy(), ri)
     np.testing.assert_allclose(w[rows.to(cuda)].cpu().numpy().astype(np.float64), rw, rtol=RTOL, atol=ATOL)
+
+
+@pytest.mark.gpu
+def test_route_refuses_outputs_that_are_no_tensors(pkg, cuda):
+    x = torch.zeros((4, 8), device=cuda)
+    with pytest.raises(ValueError, match="weights"):
+        pkg.route_experts(x, 2, weights=[0.0] * 8)
+    with pytest.raises(ValueError, match="ids"):
+        pkg.route_experts(x, 2, ids=[0] * 8)
