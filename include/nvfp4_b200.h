@@ -256,7 +256,8 @@ NVFP4_API int nvfp4_route_experts(const void* logits, int dtype, int64_t T, int6
  * with nvfp4() the quantisation of nvfp4_quantize (h from its fp32 value),
  * fp32 accumulation, and one rounding to fp16 at the end.  A slot whose id is
  * not in [0, E) is skipped (nvfp4_route_experts fills empty slots with -1); a
- * token without any gets zeros.  Finite inputs.
+ * token without any gets zeros.  Weights and scales are finite; a row of x that
+ * is not spoils its own row of out only.
  *   x [T, D] fp16 (row stride ldx elements), ids [T, k] int32, weights [T, k]
  *   float32, both contiguous; out [T, D] fp16 (row stride ldo elements; out
  *   may be x);
@@ -290,7 +291,8 @@ NVFP4_API int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, cons
  *   scales float32 [n] or NULL (1); ranks int32 [n] or NULL: adapter i uses its
  *   first ranks[i] rows of A and columns of B (clamped to 0..r), the others may
  *   hold anything.
- * r is a multiple of 16 up to 128, K of 8; N is any; n <= 1023; T may be 0.
+ * r is a multiple of 16 up to 128, K of 8; N, K and T are at most 2^24; n <= 1023; T may
+ * be 0.  A row of x that is not finite spoils its own row of out only.
  * `workspace`: device memory of at least nvfp4_lora_workspace() bytes (0 for few
  * tokens), 256-byte aligned, in use until the call's work on `stream` ends.
  * No counterpart in the reference.

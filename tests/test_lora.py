@@ -257,3 +257,18 @@ def test_lora_refusals(pkg, cuda):
         pkg.lora_add(a[0], a[1], a[2][:, :8].contiguous(), a[3][:, :, :8].contiguous(), a[4])
     with pytest.raises(ValueError, match="out"):
         pkg.lora_add(*a, out=a[0][:3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [5, 24, 300])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_lora_a_token_that_is_not_finite_stays_alone(pkg, cuda, T, bad):
+    p = Problem(T, 128, 96, 32, 3, 7)
+    p.adapters[:5] = 0                       # beside others of its adapter, of full rank
+    want = pkg.lora_add(*p.args())
+    a = list(p.args())
+    a[1] = a[1].clone()
+    a[1][2] = bad
+    got = pkg.lora_add(*a)
+    keep = torch.arange(T, device=cuda) != 2
+    assert torch.equal(got[keep], want[keep])

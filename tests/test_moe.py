@@ -277,3 +277,27 @@ def test_router_into_experts(pkg, oracle, cuda):
     p.ids, p.weights = ids.cpu(), w.cpu()
     assert (p.ids[7, 1:] == -1).all()
     p.check(oracle, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E", [(5, 2, 4), (60, 4, 16), (300, 2, 2)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_moe_a_token_that_is_not_finite_stays_alone(pkg, cuda, T, k, E, bad):
+    a = list(Problem(pkg, T, k, E, 192, 128).args())
+    want = pkg.moe_mlp(*a)
+    a[0] = a[0].clone()
+    a[0][2] = bad
+    got = pkg.moe_mlp(*a)
+    keep = torch.arange(T, device=cuda) != 2
+    assert torch.equal(got[keep], want[keep])
+    assert pkg._lib.device_errors() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [3, 40])
+def test_moe_most_experts_and_slots(pkg, oracle, cuda, T):
+    p = Problem(pkg, T, 32, 1024, 64, 64)
+    out = pkg.moe_mlp(*p.args())
+    torch.cuda.synchronize()
+    assert pkg._lib.device_errors() == 0
+    p.check(oracle, out)
