@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <cstring>
+#include <type_traits>
 #include "common.h"
 #include "plan.cuh"
 #include "ptx.cuh"
@@ -660,103 +661,110 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       ask();
       if (live) {
         const __half* const bs = bget + ring * (C::EXPAND_B / 2);
+        auto columns = [&](auto full) {
+          // all 64 columns exist: without the code for the last ones 141.7 -> 137.2 us a call (8192 tokens, r = 64); for
+          // ranks above 64 no gain (600 tokens: 26.6 against 27.2)
+          constexpr bool FULL = decltype(full)::value;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int n0 = st * kExpandCols + half * 32, col = n0 + 8 * q, off = (st - lo) * kExpandCols + half * 32;
-          __half plain[16];                              // !VEC: base of this lane's column for the 16 tokens
-          if (!VEC) {
+          for (int half = 0; half < 2; ++half) {
+            const int n0 = st * kExpandCols + half * 32, col = n0 + 8 * q, off = (st - lo) * kExpandCols + half * 32;
+            __half plain[16];                              // !VEC: base of this lane's column for the 16 tokens
+            if (!VEC) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-              const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
-              plain[t] = tk >= 0 && n0 + lane < p.N ? p.base[tk * p.ld_base + n0 + lane] : __float2half_rn(0.f);
-            }
-          }
-          // VEC: the sums start from base (times 2^p)
-          float acc[4][4] = {};
-          const bool whole = col + 8 <= p.N;
-          if (VEC) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
-              const uint32_t b[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
-                if (!whole) f = make_float2(col + 2 * j < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j]) : 0.f,
-                                            col + 2 * j + 1 < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j + 1]) : 0.f);
-                acc[j][2 * h] = f.x;
-                acc[j][2 * h + 1] = f.y;
+              for (int t = 0; t < 16; ++t) {
+                const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
+                plain[t] = tk >= 0 && n0 + lane < p.N ? p.base[tk * p.ld_base + n0 + lane] : __float2half_rn(0.f);
               }
             }
-            if (!unit) {
+            // VEC: the sums start from base (times 2^p)
+            float acc[4][4] = {};
+            const bool whole = FULL || col + 8 <= p.N;
+            if (VEC) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[j][e] *= 1.f / down[e >> 1];     // a power of two: exact
-            }
-          }
-#pragma unroll
-          for (int s = 0; s < RS; ++s) {
-            if (s * 32 >= rank) break;
-            uint4 b[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint4*>(bs + (half * 32 + 2 * j) * LD + s * 32);
-            if (rank & 7) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) b[j] = below_rank(b[j], s * 32 + 8 * q, rank);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {                // neighbouring mma's add to different accumulators
-              const uint4 u0 = u[h][2 * s], u1 = u[h][2 * s + 1];
-#pragma unroll
-              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u0.x, u0.y, u0.z, u0.w, b[j].x, b[j].y);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) mma_16816(acc[j], u1.x, u1.y, u1.z, u1.w, b[j].z, b[j].w);
-            }
-          }
-          if (VEC) {
-            if (!unit) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[j][e] *= down[e >> 1];
-            }
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (tok[h] < 0) continue;
-              if (whole) {
-                uint32_t o[4];
+              for (int h = 0; h < 2; ++h) {
+                const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
+                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  const __half2 r = __floats2half2_rn(acc[j][2 * h], acc[j][2 * h + 1]);
-                  o[j] = *reinterpret_cast<const uint32_t*>(&r);
+                  float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
+                  if (!whole) f = make_float2(col + 2 * j < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j]) : 0.f,
+                                              col + 2 * j + 1 < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j + 1]) : 0.f);
+                  acc[j][2 * h] = f.x;
+                  acc[j][2 * h + 1] = f.y;
                 }
-                *reinterpret_cast<uint4*>(dst[h] + off) = make_uint4(o[0], o[1], o[2], o[3]);
-              } else {
+              }
+              if (!unit) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  if (col + e < p.N) dst[h][off + e] = __float2half_rn(acc[e >> 1][2 * h + (e & 1)]);
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[j][e] *= 1.f / down[e >> 1];     // a power of two: exact
               }
             }
-          } else {
-            // rows of any alignment: through a patch of [16 tokens][32 columns], a lane a column
-            float* const patch = reinterpret_cast<float*>(smem + kExpandStages * C::EXPAND_B + warp * 2048);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int s = 0; s < RS; ++s) {
+              if (s * 32 >= rank) break;
+              uint4 b[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<float2*>(patch + (h * 8 + g) * 32 + 8 * q + 2 * j) =
-                    make_float2(acc[j][2 * h] * down[h], acc[j][2 * h + 1] * down[h]);
-            __syncwarp();
+              for (int j = 0; j < 4; ++j) b[j] = *reinterpret_cast<const uint4*>(bs + (half * 32 + 2 * j) * LD + s * 32);
+              if (rank & 7) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-              const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
-              if (tk >= 0 && n0 + lane < p.N)
-                p.out[tk * p.ldo + n0 + lane] = __float2half_rn(__half2float(plain[t]) + patch[t * 32 + lane]);
+                for (int j = 0; j < 4; ++j) b[j] = below_rank(b[j], s * 32 + 8 * q, rank);
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {                // neighbouring mma's add to different accumulators
+                const uint4 u0 = u[h][2 * s], u1 = u[h][2 * s + 1];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_16816(acc[j], u0.x, u0.y, u0.z, u0.w, b[j].x, b[j].y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mma_16816(acc[j], u1.x, u1.y, u1.z, u1.w, b[j].z, b[j].w);
+              }
             }
-            __syncwarp();
+            if (VEC) {
+              if (!unit) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) acc[j][e] *= down[e >> 1];
+              }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (tok[h] < 0) continue;
+                if (whole) {
+                  uint32_t o[4];
+#pragma unroll
+                  for (int j = 0; j < 4; ++j) {
+                    const __half2 r = __floats2half2_rn(acc[j][2 * h], acc[j][2 * h + 1]);
+                    o[j] = *reinterpret_cast<const uint32_t*>(&r);
+                  }
+                  *reinterpret_cast<uint4*>(dst[h] + off) = make_uint4(o[0], o[1], o[2], o[3]);
+                } else {
+#pragma unroll
+                  for (int e = 0; e < 8; ++e)
+                    if (col + e < p.N) dst[h][off + e] = __float2half_rn(acc[e >> 1][2 * h + (e & 1)]);
+                }
+              }
+            } else {
+              // rows of any alignment: through a patch of [16 tokens][32 columns], a lane a column
+              float* const patch = reinterpret_cast<float*>(smem + kExpandStages * C::EXPAND_B + warp * 2048);
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  *reinterpret_cast<float2*>(patch + (h * 8 + g) * 32 + 8 * q + 2 * j) =
+                      make_float2(acc[j][2 * h] * down[h], acc[j][2 * h + 1] * down[h]);
+              __syncwarp();
+#pragma unroll
+              for (int t = 0; t < 16; ++t) {
+                const int tk = __shfl_sync(0xffffffffu, tok[t >> 3], (t & 7) * 4);
+                if (tk >= 0 && n0 + lane < p.N)
+                  p.out[tk * p.ldo + n0 + lane] = __float2half_rn(__half2float(plain[t]) + patch[t * 32 + lane]);
+              }
+              __syncwarp();
+            }
           }
-        }
+        };
+        if (RT <= 4 && (st + 1) * kExpandCols <= p.N) columns(std::true_type());
+        else columns(std::false_type());
       }
       ring = ring + 1 == kExpandStages ? 0 : ring + 1;
     }
@@ -866,11 +874,12 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   if (rc) return rc;
   const LoraRows rows = {plan.head, plan.tiles, plan.slot, reinterpret_cast<__half*>(ws + m.hi),
                          reinterpret_cast<__half*>(ws + m.lo), reinterpret_cast<float*>(ws + m.down)};
-  // CTAs per tile: as many as the SMs have room for, each with at least four stages.  K = 4096, r = 64, us with one
-  // and with as many as this: 300 tokens 23.0 and 8.0, 1024 tokens 25.9 and 13.2, 2048 tokens 28.1 and 20.1.
+  // CTAs per tile: as many as the SMs have room for, each with at least two stages (K = 1024, 300 tokens: 6.7 us
+  // with four, 5.7 with two, 5.4 with one, and no difference to a whole call between two and one).  K = 4096, r = 64, us
+  // with one CTA and with as many as this: 300 tokens 23.0 and 8.2, 1024 tokens 25.9 and 13.2, 2048 tokens 28.1 and 20.0.
   const int64_t items = (p.T + kShrinkTokens - 1) / kShrinkTokens;
   int share = 1;
-  while (share < 8 && items * share * 2 <= sm_count() && p.K >= share * 2 * 4 * kShrinkK) share *= 2;
+  while (share < 8 && items * share * 2 <= sm_count() && p.K > (share * 2 * 2 - 1) * kShrinkK) share *= 2;
   {
     cudaLaunchAttribute both[2] = {attr[0], attr[0]};
     both[0].val.clusterDim.x = (unsigned)share;
