@@ -662,8 +662,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       if (live) {
         const __half* const bs = bget + ring * (C::EXPAND_B / 2);
         auto columns = [&](auto full) {
-          // all 64 columns exist: without the code for the last ones 141.7 -> 137.2 us a call (8192 tokens, r = 64); for
-          // ranks above 64 no gain (600 tokens: 26.6 against 27.2)
+          // all 64 columns exist: without the code for the last ones 141.7 -> 137.2 us a call (8192 tokens, r = 64)
           constexpr bool FULL = decltype(full)::value;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -763,7 +762,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
             }
           }
         };
-        if (RT <= 4 && (st + 1) * kExpandCols <= p.N) columns(std::true_type());
+        if ((st + 1) * kExpandCols <= p.N) columns(std::true_type());
         else columns(std::false_type());
       }
       ring = ring + 1 == kExpandStages ? 0 : ring + 1;

@@ -71,8 +71,9 @@ __global__ void __launch_bounds__(256) scatter_kernel(const int* rows, ScatterAr
 // Plan and scatter in one launch, for few slots: every CTA (one per token) counts all of them for itself and
 // finds the rows of its own token's, a warp a slot: its expert's first row plus the number of equal ids before
 // it.  CTA 0 lists the tiles.  Against the two kernels one after the other: 2.7 us less a call for one token, 1.4 at
-// 512 slots; with 2048 as the limit 2000 tokens take 64 us instead of 55.
-constexpr int kFusedSlots = 1024;
+// 512 slots; every CTA counts all slots, so many tokens of many slots are slower
+// (2000 tokens of one slot: 64 us instead of 55): up to 2048 slots for up to 384 tokens (333 of 4: 43.2 and 44.2).
+constexpr int kFusedSlots = 2048, kFewSlots = 1024, kFewTokens = 384;
 
 __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __restrict__ ids, int n, int experts, int align,
                                                            int tile, Plan p, ScatterArgs a) {
@@ -350,7 +351,7 @@ int moe_run(const MoeCall& c) {
   const ScatterArgs a = {c.x, c.ldx, c.T, (int)c.k, (int)c.D, c.weights, c.ws + m.xq, c.ws + m.xs,
                          reinterpret_cast<float*>(c.ws + m.row_weight)};
   const int64_t n = c.T * c.k;
-  if (n <= kFusedSlots) {
+  if (n <= kFewSlots || (n <= kFusedSlots && c.T <= kFewTokens)) {
     plan_scatter_kernel<<<(unsigned)c.T, 256, 0, c.stream>>>(c.ids, (int)n, (int)c.E, m.tile, m.tile, plan, a);
     if ((rc = check_launch("plan_scatter_kernel"))) return rc;
   } else {
@@ -409,6 +410,12 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
   if (c.dev < 0 || c.dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   c.err = device_error_word();
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
-  if (!m.trans) return moe_run<ExpertCfg<false, true, 128, 1, 4>, ExpertCfg<false, false, 256, 1, 4>>(c);
+  using Up = ExpertCfg<false, true, 128, 1, 4>;
+  // The down product's tiles: 128 weight rows where its sums are short (F), so that the boundaries between tiles weigh
+  // and the accumulators of two tiles, which fit then, hide them; else 256, which read the tokens half as often.  Calls,
+  // us, with 256 and with 128: F = 1024, D = 2048, 1000 tokens of 8 of 64 experts 113.2 and 105.3, D = 4096, 3000 of 4 of 32
+  // 254 and 237; D = 4096, 1024 tokens of 2 of 8: F = 2048 79.4 and 76.3, 4096 106.2 and 106.6, 8192 180 and 189.
+  if (!m.trans && F <= 2048) return moe_run<Up, ExpertCfg<false, false, 128, 1, 6>>(c);
+  if (!m.trans) return moe_run<Up, ExpertCfg<false, false, 256, 1, 4>>(c);
   return moe_run<ExpertCfg<true, true, 16, 1, 5>, ExpertCfg<true, false, 16, 2, 5>>(c);
 }

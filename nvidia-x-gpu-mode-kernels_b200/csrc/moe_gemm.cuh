@@ -24,9 +24,9 @@
 // the thread does between two stages must fit into their time.  Every wait is
 // bounded.
 //
-// TRANS 0 has 16 epilogue warps, four to a lane quarter of tensor memory: each
-// drains its quarter of the accumulators' columns into registers (64 a thread)
-// and releases them, and the SiLU, quantisation and stores run under the next
+// TRANS 0 has an epilogue warp for every 64 columns of a lane quarter of tensor memory
+// (16 for 256 columns): each drains its columns into registers (64 a thread) and
+// releases them, and the SiLU, quantisation and stores run under the next
 // tile's products (4096 tokens, 2 of 8 experts of 4096 x 14336, gate and up:
 // 547 us with 4 warps that worked their way through the columns before
 // releasing them, 485 with 16; 446 with one 256-column MMA for both matrices
@@ -92,7 +92,7 @@ struct ExpertCfg {
   static constexpr uint32_t OP_BYTES = T_BYTES + NW * W_BYTES;
   static constexpr uint32_t SF_BYTES = SFT_BYTES + NW * SFW_BYTES;
   // tensor memory columns
-  static constexpr int BUFS = TRANS ? 2 : 1;               // accumulators of two tiles where they fit
+  static constexpr int BUFS = TRANS || NW * BN <= 128 ? 2 : 1;   // accumulators of two tiles where they fit
   static constexpr int ACC_COLS = NW * BN;
   static constexpr int SF_BASE = BUFS * ACC_COLS;          // the accumulators come first
   static constexpr int SFT_COLS = 4 * KPS;
@@ -102,7 +102,7 @@ struct ExpertCfg {
   static_assert(SF_BASE + STAGES * SF_STAGE_COLS <= TMEM_COLS, "tensor memory budget");
   static_assert(SMEM <= 232448, "shared memory budget");
   static_assert(SMEM < (1 << 18), "descriptor address field");
-  static constexpr int EPI_WARPS = TRANS ? 4 : 16;
+  static constexpr int EPI_WARPS = TRANS ? 4 : NW * BN / 16;   // 64 accumulator values a thread
   static constexpr int THREADS = 32 * (2 + EPI_WARPS + 4 + 1);   // producer, MMA, epilogue, scales, scales' producer
   static constexpr uint32_t IDESC = tc::idesc_mxf4nvf4(BM, MMA_N);
 };

@@ -301,3 +301,17 @@ def test_moe_most_experts_and_slots(pkg, oracle, cuda, T):
     torch.cuda.synchronize()
     assert pkg._lib.device_errors() == 0
     p.check(oracle, out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E,D,F", [
+    (333, 4, 8, 192, 2048), (333, 4, 8, 192, 2112),      # both sides of the rule on the down product's tiles
+    (384, 5, 8, 128, 128), (385, 5, 8, 128, 128), (384, 6, 8, 128, 128),   # and of that on the plan's launch
+    (700, 2, 3, 1088, 64),
+])
+def test_moe_both_sides_of_the_rules(pkg, oracle, cuda, T, k, E, D, F):
+    p = Problem(pkg, T, k, E, D, F)
+    out = pkg.moe_mlp(*p.args())
+    torch.cuda.synchronize()
+    assert pkg._lib.device_errors() == 0
+    p.check(oracle, out)
