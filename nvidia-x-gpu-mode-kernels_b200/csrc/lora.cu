@@ -406,7 +406,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
 // ------------------------------------------------------------------ many tokens
 
 constexpr int kTile = 128;               // tokens per tile of the plan
-constexpr int kShrinkTokens = 32;        // tokens per CTA of the first product
 constexpr int kShrinkK = 128;            // elements of K per stage
 constexpr int kShrinkStages = 3;
 constexpr int kExpandCols = 64;          // columns per step of the second product
@@ -438,26 +437,33 @@ constexpr int padded_row(int halves) { return halves % 64 ? halves : halves + 32
 template <int RT>
 struct LoraCfg {
   static constexpr int R = RT * 16;
-  static constexpr int LDK = padded_row(kShrinkK), LDR = padded_row(R);
-  static constexpr int SHRINK_STAGE = (kShrinkTokens + R) * LDK * 2;
-  static constexpr int SHRINK_SMEM = kShrinkStages * SHRINK_STAGE;
-  static_assert(SHRINK_SMEM >= 4 * kShrinkTokens * R * 4, "the four shares of u");
+  static constexpr int LDR = padded_row(R);
   static constexpr int EXPAND_B = kExpandCols * LDR * 2;
   static constexpr int EXPAND_BASE = 8 * 4 * 512;        // a warp's 16 tokens x 64 columns, 4 pieces a lane
   static constexpr int EXPAND_SMEM = kExpandStages * (EXPAND_B + EXPAND_BASE);
 };
 
-// u of 32 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
-// of 128-element stages; two warps take 16 tokens each over each quarter of a stage.  Where there are fewer tiles than
-// SMs, a cluster of CTAs shares a tile's K (each a run of stages) and each finishes its share of the tokens.
-// 8192 tokens, K = 4096, r = 64: 35 us at 22 % of DRAM; latency, with 13 warps an SM.
-template <int RT>
-__global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
-  using C = LoraCfg<RT>;
-  constexpr int R = C::R, NT = RT * 2, PER = kTile / kShrinkTokens, LD = C::LDK, CHUNKS = kShrinkK / 8;
+// u of 32 or 64 tokens of one adapter: tokens are the mma's rows, ranks its columns.  x and A come through a ring
+// of 128-element stages; two warps take half the tokens each over each quarter of a stage.  Rows are not padded: odd rows
+// have the halves of each 128 bytes swapped, so that two neighbouring rows of 4 lanes, 16 bytes each, meet all banks once
+// (two CTAs an SM fit; against padded rows 3000 tokens take 35.1 us instead of 37.8).  Where there are fewer tiles than
+// places, a cluster of CTAs shares a tile's K (each a run of stages) and each finishes its share of the tokens.
+// 8192 tokens, K = 4096, r = 64: 33 us (10 by bytes); latency, with 16 warps an SM.
+template <int RT, int MT>
+struct ShrinkCfg {
+  static constexpr int R = RT * 16, TOKENS = 32 * MT;    // of a CTA
+  static constexpr int STAGE = (TOKENS + R) * kShrinkK * 2;
+  static constexpr int SMEM = kShrinkStages * STAGE;
+  static_assert(SMEM >= 4 * TOKENS * R * 4, "the four shares of u");
+};
+
+template <int RT, int MT>
+__global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) shrink_kernel(const __grid_constant__ LoraArgs p, const LoraRows w) {
+  using C = ShrinkCfg<RT, MT>;
+  constexpr int R = C::R, NT = RT * 2, TOKENS = C::TOKENS, PER = kTile / TOKENS, LD = kShrinkK, CHUNKS = kShrinkK / 8;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int m0 = (warp & 1) * 16, share = warp >> 1;     // of kShrinkK: 32 elements, two mma's
+  const int m0 = (warp & 1) * 16 * MT, share = warp >> 1;     // of kShrinkK: 32 elements, two mma's
   const int me = (int)cluster_ctarank(), ncta = cluster_nctas();
   griddep_launch();
   griddep_wait();
@@ -466,14 +472,14 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
   const int klo = nk * me / ncta, khi = nk * (me + 1) / ncta;
   for (int item = blockIdx.x / ncta; item < total; item += gridDim.x / ncta) {
     const PlanTile tile = w.tiles[item / PER];
-    const int tr = (item / PER - tile.first) * kTile + item % PER * kShrinkTokens;   // first token within the adapter
+    const int tr = (item / PER - tile.first) * kTile + item % PER * TOKENS;   // first token within the adapter
     if (tile.index >= p.n || tr >= tile.rows) continue;
     const int row0 = tile.row0 + tr;
     const int rank = lora_rank(p, tile.index);
     const __half* A = p.a + tile.index * p.a_stride;
     // this thread's pieces of a stage: 16 threads a row, 16 rows a pass
-    const int pc = tid % CHUNKS * 8, pr = tid / CHUNKS;
-    constexpr int XP = kShrinkTokens / (kLoraThreads / CHUNKS), AP = (R + kLoraThreads / CHUNKS - 1) / (kLoraThreads / CHUNKS);
+    const int pr = tid / CHUNKS, pc = tid % CHUNKS * 8, put = pc ^ (pr & 1) * 32;
+    constexpr int XP = TOKENS / (kLoraThreads / CHUNKS), AP = (R + kLoraThreads / CHUNKS - 1) / (kLoraThreads / CHUNKS);
     const __half* xp[XP];
 #pragma unroll
     for (int e = 0; e < XP; ++e) {
@@ -482,18 +488,18 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
     }
     auto ask = [&](int ks) {
       if (ks < khi) {
-        __half* const st = reinterpret_cast<__half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
+        __half* const st = reinterpret_cast<__half*>(smem + ks % kShrinkStages * C::STAGE);
         const int k = ks * kShrinkK + pc;
 #pragma unroll
         for (int e = 0; e < XP; ++e) {
           const bool in = xp[e] && k < p.K;
-          cp_async_16(st + (e * (kLoraThreads / CHUNKS) + pr) * LD + pc, in ? xp[e] + k : p.x, in);
+          cp_async_16(st + (e * (kLoraThreads / CHUNKS) + pr) * LD + put, in ? xp[e] + k : p.x, in);
         }
 #pragma unroll
         for (int e = 0; e < AP; ++e) {
           const int row = e * (kLoraThreads / CHUNKS) + pr;
           const bool in = row < rank && k < p.K;
-          if (row < R) cp_async_16(st + (kShrinkTokens + row) * LD + pc, in ? A + row * p.lda + k : p.a, in);
+          if (row < R) cp_async_16(st + (TOKENS + row) * LD + put, in ? A + row * p.lda + k : p.a, in);
         }
       }
       cp_async_commit();
@@ -501,42 +507,56 @@ __global__ void __launch_bounds__(kLoraThreads) shrink_kernel(const __grid_const
     __syncthreads();                                     // the previous item's shared memory is read
 #pragma unroll
     for (int s = 0; s < kShrinkStages - 1; ++s) ask(klo + s);
-    float acc[NT][4] = {};
+    const int get = (share * 32 + 8 * q) ^ (g & 1) * 32;
+    float acc[MT][NT][4] = {};
     for (int ks = klo; ks < khi; ++ks) {
       cp_async_wait<kShrinkStages - 2>();
       __syncthreads();                                   // stage ks is here, stage ks - 1 free
       ask(ks + kShrinkStages - 1);
-      const __half* const st = reinterpret_cast<const __half*>(smem + ks % kShrinkStages * C::SHRINK_STAGE);
-      const __half* const xs = st + (m0 + g) * LD + share * 32 + 8 * q;
-      const __half* const as = st + (kShrinkTokens + g) * LD + share * 32 + 8 * q;
-      const uint4 x0 = *reinterpret_cast<const uint4*>(xs), x1 = *reinterpret_cast<const uint4*>(xs + 8 * LD);
+      const __half* const st = reinterpret_cast<const __half*>(smem + ks % kShrinkStages * C::STAGE);
+      const __half* const xs = st + (m0 + g) * LD + get;
+      const __half* const as = st + (TOKENS + g) * LD + get;
+      uint4 x[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        x[m][0] = *reinterpret_cast<const uint4*>(xs + m * 16 * LD);
+        x[m][1] = *reinterpret_cast<const uint4*>(xs + (m * 16 + 8) * LD);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; nt += 2) {
         if (nt * 8 >= rank) break;
         const uint4 a0 = *reinterpret_cast<const uint4*>(as + nt * 8 * LD), a1 = *reinterpret_cast<const uint4*>(as + (nt + 1) * 8 * LD);
-        mma_16816(acc[nt], x0.x, x1.x, x0.y, x1.y, a0.x, a0.y);
-        mma_16816(acc[nt + 1], x0.x, x1.x, x0.y, x1.y, a1.x, a1.y);
-        mma_16816(acc[nt], x0.z, x1.z, x0.w, x1.w, a0.z, a0.w);
-        mma_16816(acc[nt + 1], x0.z, x1.z, x0.w, x1.w, a1.z, a1.w);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_16816(acc[m][nt], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a0.x, a0.y);
+          mma_16816(acc[m][nt + 1], x[m][0].x, x[m][1].x, x[m][0].y, x[m][1].y, a1.x, a1.y);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          mma_16816(acc[m][nt], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a0.z, a0.w);
+          mma_16816(acc[m][nt + 1], x[m][0].z, x[m][1].z, x[m][0].w, x[m][1].w, a1.z, a1.w);
+        }
       }
     }
     cp_async_wait<0>();
     __syncthreads();
-    float* const part = reinterpret_cast<float*>(smem);  // [quarter of K][32 tokens][R]
+    float* const part = reinterpret_cast<float*>(smem);  // [quarter of K][tokens][R]
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      float* at = part + (share * kShrinkTokens + m0 + g) * R + nt * 8 + 2 * q;
-      *reinterpret_cast<float2*>(at) = make_float2(acc[nt][0], acc[nt][1]);
-      *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[nt][2], acc[nt][3]);
-    }
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float* at = part + (share * TOKENS + m0 + m * 16 + g) * R + nt * 8 + 2 * q;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[m][nt][0], acc[m][nt][1]);
+        *reinterpret_cast<float2*>(at + 8 * R) = make_float2(acc[m][nt][2], acc[m][nt][3]);
+      }
     __syncthreads();
-    for (int e = tid; e < kShrinkTokens * R; e += kLoraThreads)
-      part[e] += part[e + kShrinkTokens * R] + part[e + 2 * kShrinkTokens * R] + part[e + 3 * kShrinkTokens * R];
+    for (int e = tid; e < TOKENS * R; e += kLoraThreads)
+      part[e] += part[e + TOKENS * R] + part[e + 2 * TOKENS * R] + part[e + 3 * TOKENS * R];
     if (ncta > 1) cluster_sync();                        // every CTA's sums are there
     else __syncthreads();
     const float scale = p.scales ? p.scales[tile.index] : 1.f;
-    const int thi = kShrinkTokens * (me + 1) / ncta;
-    for (int t = kShrinkTokens * me / ncta + warp; t < thi; t += kLoraThreads / 32) {
+    const int thi = TOKENS * (me + 1) / ncta;
+    for (int t = TOKENS * me / ncta + warp; t < thi; t += kLoraThreads / 32) {
       float u[R / 32];
       float m = 0.f;
 #pragma unroll
@@ -823,6 +843,7 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   using C = LoraCfg<RT>;
   static bool attr_set[64] = {};
   static bool wide[64] = {};             // clusters of 16 fit
+  constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
@@ -849,7 +870,10 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
       cfg.gridDim = dim3(16);
       cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(16);
       wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT, true>, &cfg) == cudaSuccess && fit > 0;
-      e = cudaFuncSetAttribute(shrink_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SHRINK_SMEM);
+      e = cudaFuncSetAttribute(shrink_kernel<RT, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, ShrinkCfg<RT, 1>::SMEM);
+    }
+    if (e == cudaSuccess) {
+      e = cudaFuncSetAttribute(shrink_kernel<RT, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, ShrinkCfg<RT, kWide>::SMEM);
     }
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(expand_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
@@ -873,23 +897,26 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   if (rc) return rc;
   const LoraRows rows = {plan.head, plan.tiles, plan.slot, reinterpret_cast<__half*>(ws + m.hi),
                          reinterpret_cast<__half*>(ws + m.lo), reinterpret_cast<float*>(ws + m.down)};
-  // CTAs per tile: as many as the SMs have room for, each with at least two stages (K = 1024, 300 tokens: 6.7 us
-  // with four, 5.7 with two, 5.4 with one, and no difference to a whole call between two and one).  K = 4096, r = 64, us
-  // with one CTA and with as many as this: 300 tokens 23.0 and 8.2, 1024 tokens 25.9 and 13.2, 2048 tokens 28.1 and 20.0.
-  const int64_t items = (p.T + kShrinkTokens - 1) / kShrinkTokens;
+  // 64 tokens a CTA read A half as often, which pays once they fill the SMs (K = 4096, us a call, 32 and 64 tokens: 2048
+  // tokens 32.6 and 33.2, 3000 33.0 and 32.0, 16384 103.3 and 92.7).  CTAs per tile: as many as fill the slots, each
+  // with at least two stages (300 tokens, K = 1024, the product: 6.7 us with four, 5.7 with two).  One CTA a tile and as many
+  // as this, the product alone at K = 4096, r = 64: 300 tokens 23.0 and 7.4, 1024 tokens 25.9 and 14.4, 8192 37.7 and 32.9.
+  const bool twice = kWide > 1 && p.T >= 2560;
+  const int tokens = twice ? 32 * kWide : 32;
+  const int64_t items = (p.T + tokens - 1) / tokens;
   int share = 1;
-  while (share < 8 && items * share * 2 <= sm_count() && p.K > (share * 2 * 2 - 1) * kShrinkK) share *= 2;
+  while (share < 8 && items * share * 2 <= sm_count() * kSlots && p.K > (share * 2 * 2 - 1) * kShrinkK) share *= 2;
   {
     cudaLaunchAttribute both[2] = {attr[0], attr[0]};
     both[0].val.clusterDim.x = (unsigned)share;
     both[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     both[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(m.max_tiles * (kTile / kShrinkTokens), std::max(1, sm_count() * 2 / share)) * share));
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(m.max_tiles * (kTile / tokens), std::max(1, sm_count() * 2 / share)) * share));
     cfg.blockDim = dim3(kLoraThreads);
-    cfg.dynamicSmemBytes = C::SHRINK_SMEM;
+    cfg.dynamicSmemBytes = twice ? ShrinkCfg<RT, kWide>::SMEM : ShrinkCfg<RT, 1>::SMEM;
     cfg.attrs = both;
     cfg.numAttrs = 2;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, shrink_kernel<RT>, p, rows);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, twice ? shrink_kernel<RT, kWide> : shrink_kernel<RT, 1>, p, rows);
     if (e != cudaSuccess) return cuda_fail(e, "cudaLaunchKernelEx(shrink)");
   }
   const int64_t steps = (p.N + kExpandCols - 1) / kExpandCols;

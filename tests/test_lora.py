@@ -272,3 +272,13 @@ def test_lora_a_token_that_is_not_finite_stays_alone(pkg, cuda, T, bad):
     got = pkg.lora_add(*a)
     keep = torch.arange(T, device=cuda) != 2
     assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N,r,n,run", [
+    (2559, 520, 72, 64, 5, 70), (2560, 520, 72, 64, 5, 70), (2600, 1032, 40, 32, 40, 3), (2700, 264, 33, 128, 3, 200),
+    (4100, 8, 64, 16, 2, 1000), (9500, 520, 24, 64, 3, 500),
+])
+def test_lora_both_sides_of_the_rules(pkg, oracle, cuda, T, K, N, r, n, run):
+    p = Problem(T, K, N, r, n, run)
+    p.check(oracle, pkg.lora_add(*p.args()))
