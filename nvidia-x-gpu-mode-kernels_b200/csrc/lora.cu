@@ -17,9 +17,9 @@
 //
 // Few tokens (decode_kernel): one launch.  A cluster of CTAs takes up to 8 tokens of one adapter: each CTA
 // sums its share of K for all ranks, the partial u's are exchanged through distributed shared memory and each CTA
-// writes its share of N.  B is prefetched into L2 at the start, so both matrices stream at once.  K = 4096,
-// N = 14336: one token of rank 16 7 us, 64 tokens of 32 adapters of rank 64 25 us at 32 % of DRAM (43 MB, 7 us by
-// bytes): with 13 warps an SM the latency of its loads bounds it.
+// writes its share of N, whose first two steps of B are under way during the exchange.  K = 4096, N = 14336: one token
+// of rank 16 7 us, 64 tokens of 32 adapters of rank 64 20 us (43 MB, 7 by bytes): with 13 warps an SM the latency of its
+// loads bounds it.  Prefetching B into L2 from the start took 24 us, asking for one step behind the exchange 21.
 //
 // Many tokens: the plan (plan.cuh) orders them by adapter; shrink_kernel computes u, expand_kernel adds u . B^T.
 #include <cuda_fp16.h>
@@ -228,14 +228,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
     const int rank = lora_rank(p, i);
     const __half* A = p.a + i * p.a_stride;
     const __half* B = p.b + i * p.b_stride;
-    {
-      // B's rows of this CTA, on their way into L2 while A streams
-      const int n0 = glo * 32, n1 = min(p.N, ghi * 32);
-      const char* lo_b = reinterpret_cast<const char*>(B + n0 * p.ldb);
-      const int64_t bytes = n1 > n0 ? ((int64_t)(n1 - 1 - n0) * p.ldb + rank) * 2 : 0;
-      for (int64_t o = (int64_t)tid * 128; o < bytes; o += (int64_t)blockDim.x * 128)
-        asm volatile("prefetch.global.L2 [%0];" :: "l"(lo_b + o));
-    }
     const int j = lane >> 2, mytok = tok[j];             // this lane's token and columns in the end
     struct Step {
       uint4 b[RS][4], base;
@@ -295,6 +287,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
         *reinterpret_cast<float2*>(&part[warp][m * 16 + g + 8][2 * q]) = make_float2(acc[m][2], acc[m][3]);
       }
     }
+    if (kAhead) {                                        // in flight over the exchange
+      ask(glo + warp, one);
+      ask(glo + warp + kDecodeWarps, two);
+    }
     __syncthreads();
     // this CTA's share goes to every CTA of the cluster, its own included, once all of them have arrived
     cluster_wait();
@@ -305,7 +301,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
       const uint32_t there = smem_u32(shares + me * R * 8 + e);
       for (int c = 0; c < ncta; ++c) st_cluster_f32(mapa(there, c), s);
     }
-    if (kAhead) ask(glo + warp, one);                    // in flight over the exchange
     cluster_sync();
     // every CTA adds all shares in the same order: the same u everywhere
     {
@@ -388,10 +383,10 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
     };
     if (kAhead) {
       for (int gr = glo + warp; gr < ghi; gr += 2 * kDecodeWarps) {
-        ask(gr + kDecodeWarps, two);
         add(gr, one);
         ask(gr + 2 * kDecodeWarps, one);
         add(gr + kDecodeWarps, two);
+        ask(gr + 3 * kDecodeWarps, two);
       }
     } else {
       for (int gr = glo + warp; gr < ghi; gr += kDecodeWarps) {
