@@ -24,6 +24,7 @@
 // Many tokens: the plan (plan.cuh) orders them by adapter; shrink_kernel computes u, expand_kernel adds u . B^T.
 #include <cuda_fp16.h>
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <type_traits>
 #include "common.h"
@@ -833,12 +834,23 @@ int lora_check(int64_t T, int64_t r, int64_t n) {
   return NVFP4_OK;
 }
 
+// CTAs a cluster for few tokens: 8 read an item's matrices sooner, but where more items than clusters are to be expected
+// smaller clusters take them in fewer rounds.  The items are in GPU memory; `T` tokens that choose among n adapters at
+// random take n (1 - (1 - 1/n)^T) of them, in eights.  us with 8, 4 and 2 (K = N = 4096): 48 tokens of 48 adapters of rank 32
+// 7.6, 8.8, 12.3; 100 of 100 of rank 16 15.0, 10.9, 14.8; 256 of 4 of rank 64 14.5, 14.4, 19.5; 256 of 200 65.8, 42.1, 38.2;
+// with 8, 2 and 1: 256 of 1000 of rank 16 64.4, 33.1, 31.1.
+int decode_cluster(int T, int n, int slots) {
+  const double used = n * (1 - std::pow(1 - 1.0 / n, T));
+  const double items = used * std::max(1.0, (T / used + 3.5) / 8);
+  return items <= slots / 8 ? 8 : items <= slots / 4 ? 4 : items <= slots / 2 ? 2 : 1;
+}
+
 template <int RT>
 int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t stream) {
   using C = LoraCfg<RT>;
   static bool attr_set[64] = {};
   static bool wide[64] = {};             // clusters of 16 fit
-  constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product
+  constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product and of decode_kernel
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
@@ -878,7 +890,7 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
     attr_set[dev] = true;
   }
   if (p.T <= kDecodeTokens) {
-    const int ncta = p.T <= 4 && wide[dev] ? 16 : 8;
+    const int ncta = p.T <= 4 && wide[dev] ? 16 : decode_cluster(p.T, p.n, sm_count() * kSlots);
     attr[0].val.clusterDim.x = (unsigned)ncta;
     cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(ncta);
     cfg.gridDim = dim3((unsigned)(std::min(p.T, std::max(1, sm_count() * 2 / ncta)) * ncta));

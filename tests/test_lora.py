@@ -282,3 +282,16 @@ def test_lora_a_token_that_is_not_finite_stays_alone(pkg, cuda, T, bad):
 def test_lora_both_sides_of_the_rules(pkg, oracle, cuda, T, K, N, r, n, run):
     p = Problem(T, K, N, r, n, run)
     p.check(oracle, pkg.lora_add(*p.args()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("T,K,N,r,n", [      # the clusters' sizes for few tokens: 16, 8, 4, 2, 1
+    (4, 200, 72, 64, 9), (48, 136, 72, 32, 48), (100, 64, 200, 16, 100), (180, 264, 33, 32, 180), (256, 72, 40, 16, 1000),
+    (18, 136, 72, 128, 40), (40, 136, 72, 128, 60), (100, 72, 33, 128, 100), (200, 136, 72, 128, 200), (256, 40, 8, 112, 1),
+])
+def test_lora_clusters_of_every_size(pkg, oracle, cuda, T, K, N, r, n, in_place):
+    p = Problem(T, K, N, r, n)
+    a = p.args()
+    out = None if in_place else torch.full((T, N), float("nan"), dtype=torch.float16, device=cuda)
+    p.check(oracle, pkg.lora_add(*a, out=out))
