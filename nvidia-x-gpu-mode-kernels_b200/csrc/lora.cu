@@ -18,7 +18,7 @@
 // Few tokens (decode_kernel): one launch.  A cluster of CTAs takes up to 8 tokens of one adapter: each CTA
 // sums its share of K for all ranks, the partial u's are exchanged through distributed shared memory and each CTA
 // writes its share of N, whose first two steps of B are under way during the exchange.  K = 4096, N = 14336: one token
-// of rank 16 7 us, 64 tokens of 32 adapters of rank 64 20 us (43 MB, 7 by bytes): with 13 warps an SM the latency of its
+// of rank 16 5.3 us, 64 tokens of 32 adapters of rank 64 21 us (43 MB, 7 by bytes): with 13 warps an SM the latency of its
 // loads bounds it.  Prefetching B into L2 from the start took 24 us, asking for one step behind the exchange 21.
 //
 // Many tokens: the plan (plan.cuh) orders them by adapter; shrink_kernel computes u, expand_kernel adds u . B^T.
@@ -140,6 +140,11 @@ struct DecodeCfg {
   static constexpr int smem(int ncta) { return (POOL + ncta * R * 8) * 4; }
 };
 
+// Into how many parts an item's columns may go: every warp of a cluster has a step of 32 columns.
+__host__ __device__ constexpr int decode_parts(int N, int ncta) {
+  return ((N + 31) / 32 + ncta * kDecodeWarps - 1) / (ncta * kDecodeWarps);
+}
+
 // The two halves of a cluster barrier.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -187,10 +192,15 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
   if (leads) items[at + __popc(leaders & ((1u << lane) - 1))] = tid;
   __syncthreads();
   const int groups = (p.N + 31) / 32;                    // 32 columns per warp and step
-  const int glo = groups * me / ncta, ghi = groups * (me + 1) / ncta;
+  // Where clusters outnumber items, several share an item's columns, and each computes u (K = 4096, N = 14336: one token
+  // of rank 16 6.5 -> 5.3 us, 16 of 16 adapters of rank 64 13.6 -> 12.1, 64 of one among 300 of rank 16 12.5 -> 8.1).  All
+  // clusters run at once: the launch has no more than fit.
+  const int clusters = (int)gridDim.x / ncta;
+  const int parts = max(1, min(clusters / max(nitems, 1), decode_parts(p.N, ncta)));
 
-  for (int item = (int)(blockIdx.x / ncta); item < nitems; item += (int)(gridDim.x / ncta)) {
-    const int t0 = items[item], i = key[t0];
+  for (int work = (int)blockIdx.x / ncta; work < nitems * parts; work += clusters) {
+    const int t0 = items[work / parts], i = key[t0], share = work % parts * ncta + me;
+    const int glo = groups * share / (parts * ncta), ghi = groups * (share + 1) / (parts * ncta);
     if (warp == 0) {                                     // the eight's tokens; the previous item's readers have left
       if (lane < 8) tok[lane] = -1;
       __syncwarp();
@@ -836,28 +846,31 @@ int lora_check(int64_t T, int64_t r, int64_t n) {
 
 // CTAs a cluster for few tokens: 8 read an item's matrices sooner, but where more items than clusters are to be expected
 // smaller clusters take them in fewer rounds.  The items are in GPU memory; `T` tokens that choose among n adapters at
-// random take n (1 - (1 - 1/n)^T) of them, in eights.  us with 8, 4 and 2 (K = N = 4096): 48 tokens of 48 adapters of rank 32
-// 7.6, 8.8, 12.3; 100 of 100 of rank 16 15.0, 10.9, 14.8; 256 of 4 of rank 64 14.5, 14.4, 19.5; 256 of 200 65.8, 42.1, 38.2;
-// with 8, 2 and 1: 256 of 1000 of rank 16 64.4, 33.1, 31.1.
-int decode_cluster(int T, int n, int slots) {
+// random take n (1 - (1 - 1/n)^T) of them, in eights.  fit: clusters of 1, 2, 4, 8 that run at once.  Returns the size's log2.
+// us with 8, 4, 2 and 1 (K = N = 4096): 16 tokens of 300 adapters of rank 16 6.6, 7.0, 8.2, 10.6; 100 of 100 of rank 16 12.7, 9.7, 12.7,
+// 17.0; 256 of 200 of rank 64 52.8, 40.0, 37.4, 48.8; 256 of 256 (1024 x 1024) 24.8, 16.1, 13.2, 11.2.  A batch of one adapter
+// among many would rather have 8 (200 tokens, 300 adapters of rank 64: 12.0, where this takes 2 and 16.6).
+int decode_cluster(int T, int n, const int (&fit)[4]) {
   const double used = n * (1 - std::pow(1 - 1.0 / n, T));
   const double items = used * std::max(1.0, (T / used + 3.5) / 8);
-  return items <= slots / 8 ? 8 : items <= slots / 4 ? 4 : items <= slots / 2 ? 2 : 1;
+  int size = 3;
+  while (size > 0 && items > fit[size]) --size;
+  return size;
 }
 
 template <int RT>
 int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t stream) {
   using C = LoraCfg<RT>;
   static bool attr_set[64] = {};
-  static bool wide[64] = {};             // clusters of 16 fit
-  constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product and of decode_kernel
+  static int fits[64][4];                // clusters of 1, 2, 4, 8 for few tokens that run at once
+  constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 16;
+  attr[0].val.clusterDim.x = 1;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
   cfg.blockDim = dim3(kDecodeWarps * 32);
@@ -865,23 +878,22 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   if (!attr_set[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(8));
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(8));
+    for (int size = 0; size < 4 && e == cudaSuccess; ++size) {
+      int with = 0, without = 0;
+      attr[0].val.clusterDim.x = 1u << size;
+      cfg.gridDim = dim3(1u << size);
+      cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(1 << size);
+      e = cudaOccupancyMaxActiveClusters(&with, decode_kernel<RT, true>, &cfg);
+      if (e == cudaSuccess) e = cudaOccupancyMaxActiveClusters(&without, decode_kernel<RT, false>, &cfg);
+      fits[dev][size] = std::max(1, std::min(with, without));
+    }
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(16));
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(16));
-    if (e == cudaSuccess) {
-      int fit = 0;
-      cfg.gridDim = dim3(16);
-      cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(16);
-      wide[dev] = cudaOccupancyMaxActiveClusters(&fit, decode_kernel<RT, true>, &cfg) == cudaSuccess && fit > 0;
       e = cudaFuncSetAttribute(shrink_kernel<RT, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, ShrinkCfg<RT, 1>::SMEM);
-    }
-    if (e == cudaSuccess) {
+    if (e == cudaSuccess)
       e = cudaFuncSetAttribute(shrink_kernel<RT, kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, ShrinkCfg<RT, kWide>::SMEM);
-    }
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(expand_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
     if (e == cudaSuccess)
@@ -890,10 +902,12 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
     attr_set[dev] = true;
   }
   if (p.T <= kDecodeTokens) {
-    const int ncta = p.T <= 4 && wide[dev] ? 16 : decode_cluster(p.T, p.n, sm_count() * kSlots);
+    const int size = decode_cluster(p.T, p.n, fits[dev]);
+    const int ncta = 1 << size;
     attr[0].val.clusterDim.x = (unsigned)ncta;
     cfg.dynamicSmemBytes = DecodeCfg<RT>::smem(ncta);
-    cfg.gridDim = dim3((unsigned)(std::min(p.T, std::max(1, sm_count() * 2 / ncta)) * ncta));
+    const int64_t most = (int64_t)p.T * decode_parts(p.N, ncta);
+    cfg.gridDim = dim3((unsigned)(std::min<int64_t>(most, fits[dev][size]) * ncta));
     cudaError_t e = cudaLaunchKernelEx(&cfg, p.vec ? decode_kernel<RT, true> : decode_kernel<RT, false>, p);
     return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaLaunchKernelEx(decode)");
   }

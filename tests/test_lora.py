@@ -295,3 +295,17 @@ def test_lora_clusters_of_every_size(pkg, oracle, cuda, T, K, N, r, n, in_place)
     a = p.args()
     out = None if in_place else torch.full((T, N), float("nan"), dtype=torch.float16, device=cuda)
     p.check(oracle, pkg.lora_add(*a, out=out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,K,N,r,n,run", [     # fewer items than clusters: several share one's columns
+    (1, 64, 9000, 16, 2, 1), (1, 200, 8195, 128, 1, 1), (9, 72, 5000, 64, 2, 9), (30, 136, 4104, 32, 200, 30),
+    (200, 72, 4099, 16, 900, 200), (256, 40, 2200, 128, 300, 256), (64, 64, 2048, 64, 3, 20),
+])
+def test_lora_clusters_that_share_an_item(pkg, oracle, cuda, T, K, N, r, n, run):
+    p = Problem(T, K, N, r, n, run)
+    p.adapters[0] = 0
+    for in_place in (False, True):
+        a = p.args()
+        out = None if in_place else torch.full((T, N), float("nan"), dtype=torch.float16, device=cuda)
+        p.check(oracle, pkg.lora_add(*a, out=out))
