@@ -454,7 +454,7 @@ struct LoraCfg {
 // have the halves of each 128 bytes swapped, so that two neighbouring rows of 4 lanes, 16 bytes each, meet all banks once
 // (two CTAs an SM fit; against padded rows 3000 tokens take 35.1 us instead of 37.8).  Where there are fewer tiles than
 // places, a cluster of CTAs shares a tile's K (each a run of stages) and each finishes its share of the tokens.
-// 8192 tokens, K = 4096, r = 64: 33 us (10 by bytes); latency, with 16 warps an SM.
+// 8192 tokens, K = 4096, r = 64: 30 us (10 by bytes); latency, with 13 warps an SM.
 template <int RT, int MT>
 struct ShrinkCfg {
   static constexpr int R = RT * 16, TOKENS = 32 * MT;    // of a CTA
@@ -597,7 +597,7 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) shrink_kernel(c
 // out += u . B^T for 128 tokens of one adapter and a run of columns, 64 at a time: a warp takes 16 tokens, whose u
 // stays in its registers.  B comes through a ring in shared memory that all warps read; base through a ring of
 // which each lane reads back just what it asked for itself.
-// 8192 tokens, N = 14336, r = 64: 120 us at 47 % of DRAM.  11 instructions for 32 outputs at 16 warps an SM bound it
+// 8192 tokens, N = 14336, r = 64: 114 us at 50 % of DRAM.  9 instructions for 32 outputs at 15 warps an SM bound it
 // (registers: three CTAs an SM spill, 164 -> 230 us, four 267, before the sums started from base).
 // The 8 columns of mma tile j of four stand for columns 8 (c / 2) + 2 j + c % 2 of 32, so that the four tiles
 // give a lane 8 consecutive columns of a token.
