@@ -239,9 +239,11 @@ __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float
       const unsigned e = i * 32 + lane;
       U v = key[i] < below || (key[i] == below && e > after) ? key[i] : 0;
       unsigned w = e;
+      // strictly larger goes first and moves all that follow down by one: equal ones stay in index order
+      bool up = false;
 #pragma unroll
-      for (int d = 0; d < DEPTH; ++d) {  // strictly larger goes first: equal ones stay in index order
-        const bool up = v > top[d];
+      for (int d = 0; d < DEPTH; ++d) {
+        up = up || v > top[d];
         const U tv = top[d];
         const unsigned tw = at[d];
         top[d] = up ? v : tv;

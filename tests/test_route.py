@@ -213,3 +213,42 @@ def test_route_refuses_outputs_that_are_no_tensors(pkg, cuda):
         pkg.route_experts(x, 2, weights=[0.0] * 8)
     with pytest.raises(ValueError, match="ids"):
         pkg.route_experts(x, 2, ids=[0] * 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["plain", "bias", "groups", "unscaled"])
+@pytest.mark.parametrize("E,k", [(96, 5), (128, 8), (256, 8), (250, 32), (500, 12), (1024, 9)])
+def test_route_equal_logits_of_one_lane(pkg, oracle, cuda, E, k, kind, dtype, score):
+    """Equal logits 32 experts apart, which one lane of a warp ranks, with larger ones behind, between and before them:
+    ties go to the lowest index."""
+    g = torch.Generator().manual_seed(E + k)
+    T = 60
+    x = torch.randint(0, 5, (T, E), generator=g).float() / 2     # many ties everywhere
+    x[0] = -4
+    x[0, [3, 35]], x[0, 67] = 1.0, 2.0                           # two equal ones, then a larger one
+    x[1] = torch.randn(E, generator=g) - 4
+    x[1, 1::32] = 1.0
+    x[1, E - 31:E:32] = 2.0
+    x[2:20] = torch.randn((18, E), generator=g) - 4              # ties in a few lanes alone
+    for t in range(2, 20):
+        lane = int(torch.randint(0, 32, (1,), generator=g))
+        x[t, lane::32] = torch.randint(1, 4, (len(x[t, lane::32]),), generator=g).float()
+    kw = dict(score=score)
+    bias = torch.zeros(E, device=cuda) if kind == "bias" else None
+    if kind == "groups":
+        kw.update(groups=2, top_groups=1) if E % 2 == 0 else None
+    if kind == "unscaled":
+        kw.update(renormalize=False)
+    _check(pkg, oracle, x.to(dtype).to(cuda), k, bias, **kw)
+
+
+@pytest.mark.gpu
+def test_route_ties_in_many_rows(pkg, oracle, cuda):
+    """bfloat16 logits of a long prompt, of few different values: every row's ids."""
+    x = (torch.randn((12000, 256), generator=torch.Generator().manual_seed(11)) * 2).to(torch.bfloat16)
+    x[::2] = (x[::2].float() * 2).round().div(2).to(torch.bfloat16)
+    _, ids = pkg.route_experts(x.to(cuda), 8)
+    want = x.float().sort(dim=1, descending=True, stable=True).indices[:, :8]
+    assert torch.equal(ids.cpu().long(), want)
