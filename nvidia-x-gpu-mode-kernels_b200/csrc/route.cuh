@@ -14,7 +14,8 @@
 // decides (the last group in against the first one out, and every neighbouring pair of the k + 1 best)
 // must differ by more than the 32-bit evaluation can be off, otherwise the warp repeats the row in 64
 // bits (256 experts with a bias, normal logits: 0.4 to 0.5 % of the rows with sigmoid, 1 % with softmax).
-// Comparisons of logits alone are exact.
+// Comparisons of logits alone are exact.  The same holds for a row whose chosen scores fall below the normal numbers of
+// 32 bits although its weights do not (`faint`).
 //
 // Three forms of the 32-bit pass:
 //   quick_row    rows without surprises: the lowest bits of a value carry its place, batches of rows;
@@ -112,8 +113,16 @@ __device__ __forceinline__ bool too_near(float hi, float lo) {
   return !(hi - lo > 4e-6f * fmaxf(1.0f, fmaxf(fabsf(hi), fabsf(lo))));
 }
 
+// Whether a chosen score s has too few digits in 32 bits: it lies below the normal numbers (0 among them), and the
+// weight made of it, scale / total times as large, is more than the 64 times that leave it below 1e-36 anyway.  So it is for sigmoids
+// of logits that are all below -88, and for softmaxes whose bias prefers experts far below the row's maximum.
+__device__ __forceinline__ bool faint(float s, float scale, float total) {
+  return s < FLT_MIN && !(fabsf(scale) <= 64.f * total);
+}
+
 // One row in R arithmetic.  x: this lane's logits (expert i * 32 + lane), -inf where off.  Returns whether
-// a comparison was too near to be trusted (R = float only); lane j then holds slot j's id and weight.
+// a comparison was too near to be trusted, or a chosen score too small (R = float only); else lane j holds slot j's id and
+// weight.
 template <typename R, int VPL, bool SOFTMAX, bool BIAS, bool GROUPS>
 __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float (&bias)[VPL],
                           int lane, int& id, float& weight) {
@@ -295,10 +304,9 @@ __device__ bool route_row(const RouteArgs& p, const float (&x)[VPL], const float
       w = score(lx);
     }
   }
-  if (p.renorm) {
-    const R total = warp_sum(w);
-    w = total > 0 ? w / total : (R)0;
-  }
+  const R total = p.renorm ? warp_sum(w) : (R)1;
+  if (kScreen && __any_sync(kAll, id >= 0 && faint((float)w, p.scale, (float)total))) return true;
+  if (p.renorm) w = total > 0 ? w / total : (R)0;
   weight = (float)(w * (R)p.scale);
   return false;
 }
@@ -393,7 +401,7 @@ __device__ __forceinline__ float reciprocal_approx(float v) {
 // (-inf: off), and the lowest bits of a choice replaced by its place in the lane, so that a lane's choices
 // differ and carry their index.  That moves a choice by less than VPL units of 2^-23 relative.  Two forms of it:
 // quick_row for rows without surprises, careful_row for all.
-enum RowState { kDone, kOdd, kNear };   // kOdd: not for quick_row; kNear: a comparison is too near, 64 bits must decide
+enum RowState { kDone, kOdd, kNear };   // kOdd: not for quick_row; kNear: a comparison is too near or a score too small, 64 bits must decide
 
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -537,10 +545,9 @@ __device__ __noinline__ RowState careful_row(const RouteArgs& p, int64_t t, int 
     const float x = logit_at(p, t, id);
     w = SOFTMAX ? expf(x - m) : 1.f / (1.f + expf(-x));
   }
-  if (p.renorm) {
-    const float total = warp_sum(w);
-    w = total > 0.f ? w / total : 0.f;
-  }
+  const float total = p.renorm ? warp_sum(w) : 1.f;
+  if (__any_sync(kAll, on && faint(w, p.scale, total))) return kNear;
+  if (p.renorm) w = total > 0.f ? w / total : 0.f;
   store_row(p, t, lane, id, w * p.scale);
   return kDone;
 }
@@ -763,18 +770,20 @@ __global__ void __launch_bounds__(256, VPL <= 8 ? 4 : VPL == 16 ? 2 : 1) route_k
       const float2 slot = on ? slots[lane] : make_float2(0.f, 0.f);
       const float mine = slot.x;
       const float up = __shfl_up_sync(kAll, mine, 1);
-      const bool bad = on && ((j > 0 && near_choices<VPL>(up, mine)) ||
-                              (j == p.k - 1 && left_out > -INFINITY && near_choices<VPL>(mine, left_out)));
-      const unsigned bad_lanes = __ballot_sync(kAll, bad);
+      bool bad = on && ((j > 0 && near_choices<VPL>(up, mine)) ||
+                        (j == p.k - 1 && left_out > -INFINITY && near_choices<VPL>(mine, left_out)));
       const int id = (int)(__float_as_int(slot.y) * VPL + (kPlace - (__float_as_uint(mine) & kPlace)));
       const float x = on ? logit_at(p, t0 + b, id) : 0.f;
       if (SOFTMAX && !BIAS && !GROUPS) m = __shfl_sync(kAll, x, b << shift);      // the best of all
       float w = !on ? 0.f : SOFTMAX ? expf(x - m) : 1.f / (1.f + expf(-x));
+      float total = 1.f;
       if (p.renorm) {
-        float total = w;
+        total = w;
         for (int o = width / 2; o; o >>= 1) total += __shfl_xor_sync(kAll, total, o);
-        w = total > 0.f ? w / total : 0.f;
       }
+      bad = bad || (on && faint(w, p.scale, total));
+      if (p.renorm) w = total > 0.f ? w / total : 0.f;
+      const unsigned bad_lanes = __ballot_sync(kAll, bad);
       const unsigned first_row = width == 32 ? kAll : (1u << width) - 1;
       if (on && !(bad_lanes & (first_row << (b << shift)))) {
         p.ids[(t0 + b) * p.k + j] = id;

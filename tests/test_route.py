@@ -252,3 +252,68 @@ def test_route_ties_in_many_rows(pkg, oracle, cuda):
     _, ids = pkg.route_experts(x.to(cuda), 8)
     want = x.float().sort(dim=1, descending=True, stable=True).indices[:, :8]
     assert torch.equal(ids.cpu().long(), want)
+
+
+# Scores that 32 bits cannot hold although the weights made of them are ordinary numbers.  Tolerance: an exponential of
+# an argument up to 88 away is off by at most (88 + 2) * 2^-24 where 32 bits still do, the sum and the quotients as above:
+# (90 + 37 + 8) * 2^-24 < 8.1e-6.  A weight of less than 64 times the smallest normal number (7.6e-37) may be lost.
+FAINT_RTOL, FAINT_ATOL = 8.1e-6, 7.6e-37
+
+
+def _check_weights(oracle, got, logits, k, bias=None, rows=None, **kw):
+    w, ids = (t.cpu() for t in got)
+    rows = torch.arange(len(logits)) if rows is None else rows
+    rw, ri = oracle.route(logits.cpu()[rows], k, bias, **kw)
+    np.testing.assert_array_equal(ids[rows].numpy(), ri)
+    np.testing.assert_allclose(w[rows].numpy().astype(np.float64), rw, rtol=FAINT_RTOL, atol=FAINT_ATOL)
+    return rw
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k,groups,top_groups", [(8, 2, 1, 1), (60, 5, 1, 1), (256, 8, 1, 1), (256, 8, 8, 4), (96, 3, 4, 1), (400, 4, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("T", [41, 9700])
+def test_route_sigmoids_below_32_bits(pkg, oracle, cuda, T, with_bias, dtype, E, k, groups, top_groups):
+    """Rows of logits around -80 to -700: every score is tiny, their ratios are not.  Few rows and enough for a warp to
+    take several at once."""
+    g = torch.Generator().manual_seed(T + E)
+    x = (torch.randn((T, E), generator=g) * 3 - torch.linspace(80, 690, T)[torch.randperm(T, generator=g)].unsqueeze(1)).to(dtype)
+    x[::7] += 690                                                # ordinary rows among them
+    x[3::7, 1:] -= 5                                             # one expert far above the others
+    bias = torch.randn(E, generator=g).to(cuda) if with_bias else None
+    got = pkg.route_experts(x.to(cuda), k, bias=bias, score="sigmoid", num_groups=groups, top_groups=top_groups, scale=2.5)
+    rows = torch.arange(0, T, 1 if T < 100 else 23)
+    rw = _check_weights(oracle, got, x, k, bias, rows, score="sigmoid", groups=groups, top_groups=top_groups, scale=2.5)
+    np.testing.assert_allclose(rw.sum(axis=1), 2.5)              # no row was lost in 64 bits
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("E,k,groups,top_groups", [(8, 2, 1, 1), (60, 5, 1, 1), (256, 8, 1, 1), (256, 8, 8, 4), (96, 3, 4, 1), (400, 4, 1, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T", [41, 9700])
+def test_route_bias_prefers_experts_far_below(pkg, oracle, cuda, T, dtype, E, k, groups, top_groups):
+    """A softmax whose bias keeps the larger half of the logits out: the chosen scores are e^-80 to e^-600 of the
+    largest."""
+    g = torch.Generator().manual_seed(T + E + 1)
+    x = torch.randn((T, E), generator=g)
+    x[:, :E // 2] += torch.linspace(80, 600, T)[torch.randperm(T, generator=g)].unsqueeze(1)
+    x[::7, :E // 2] = 0
+    x = x.to(dtype)
+    bias = torch.randn(E, generator=g)
+    bias[:E // 2] -= 20
+    got = pkg.route_experts(x.to(cuda), k, bias=bias.to(cuda), num_groups=groups, top_groups=top_groups)
+    rows = torch.arange(0, T, 1 if T < 100 else 23)
+    rw = _check_weights(oracle, got, x, k, bias, rows, groups=groups, top_groups=top_groups)
+    np.testing.assert_allclose(rw.sum(axis=1), 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("with_bias", [False, True])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("scale", [1.0, 1e30])
+def test_route_weights_that_a_scale_brings_back(pkg, oracle, cuda, scale, renormalize, with_bias):
+    x = torch.randn((50, 24), generator=torch.Generator().manual_seed(3)) - torch.linspace(0, 160, 50).unsqueeze(1)
+    bias = torch.randn(24, generator=torch.Generator().manual_seed(4)).to(cuda) if with_bias else None
+    got = pkg.route_experts(x.to(cuda), 6, bias=bias, score="sigmoid", renormalize=renormalize, scale=scale)
+    _check_weights(oracle, got, x, 6, bias, score="sigmoid", renormalize=renormalize, scale=scale)
