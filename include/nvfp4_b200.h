@@ -281,8 +281,9 @@ NVFP4_API int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, cons
 /*
  * Low-rank adapters of many requests, added to a shared projection's output:
  *   out[t] = fp16( base[t] + scales[i] * ((x[t] . A_i^T) . B_i^T) ),  i = adapters[t]
- * in fp32 (the inner product enters the outer one with at least 22 bits), one
- * rounding at the end.  A token whose index is not in [0, n) keeps base.
+ * in fp32, one rounding at the end.  Each entry of the inner product enters the
+ * outer one with 22 bits, or off by at most 2^-39 of the token's largest entry.
+ * A token whose index is not in [0, n) keeps base.
  *   base, out [T, N] fp16 (row strides ld_base, ldo elements; out may be base
  *   (in place); otherwise it overlaps neither base nor x);
  *   x [T, K] fp16; a: n matrices [r, K], b: n matrices [N, r], fp16, with row

@@ -8,8 +8,9 @@
 //
 // The products run on mma.sync (fp16 operands, fp32 accumulators): with ranks of 16 to 128 there is too
 // little arithmetic per byte for tensor memory and its round trips to pay.  u = x . A^T enters the second
-// product as two fp16 halves, u = 2^-p (hi + lo), with a 2^p per token that keeps them in fp16's range: 22 bits of
-// the token's largest |u| survive, and the sum stays in fp32.
+// product as two fp16 halves, u = 2^-p (hi + lo), with a 2^p per token that brings its largest |u| to [2^14, 2^15): each u
+// keeps 22 bits, or is off by at most 2^-39 of the largest, where lo reaches the end of fp16's range.  The sum stays in
+// fp32.
 //
 // The k index of an mma is summed over, so its 16 slots may stand for any 16 elements as long as both operands
 // agree.  Two mma's take 32 elements, slots {2q, 2q+1, 2q+8, 2q+9} of lane q of 4 standing for elements 8q..8q+3 in
@@ -64,15 +65,23 @@ __device__ __forceinline__ int lora_rank(const LoraArgs& p, int i) {
   return p.ranks ? max(0, min(p.ranks[i], p.r)) : p.r;
 }
 
-// A power of two under which two halves hold 22 bits of every u up to magnitude m, and its inverse: 1 where m is
-// in [2^-2, 2^15), so that most tokens need no scaling, else what brings m to [2^14, 2^15).  At most 2^110: base
-// times it stays finite.
+// The power of two that brings magnitude m to [2^14, 2^15), and its inverse.  Without it where m is in fp16's range
+// already, lo would end at 2^-25 however small m: entries of 2^-20 beside one of 2^-2 would keep 6 bits.  At most 2^110.
 __device__ __forceinline__ void half_scale(float m, float& up, float& down) {
   int e = (int)((__float_as_uint(m) >> 23) & 255) - 127;
-  if (m == 0.f || e == 128 || (e >= -2 && e < 14)) e = 14;   // nothing to bring up, infinite already, or fine
+  if (m == 0.f || e == 128) e = 14;                          // nothing to bring up, or infinite already
   const int q = min(14 - e, 110);
   up = __uint_as_float((uint32_t)(q + 127) << 23);
   down = __uint_as_float((uint32_t)(127 - q) << 23);
+}
+
+// (a0 * m + c0, a1 * m + c1)
+__device__ __forceinline__ float2 fma_pair(float a0, float a1, float m, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 a, m, c;\n mov.b64 a, {%2, %3};\n mov.b64 m, {%4, %4};\n mov.b64 c, {%5, %6};\n fma.rn.f32x2 a, a, m, c;\n"
+      " mov.b64 {%0, %1}, a;\n}\n"
+      : "=f"(r.x), "=f"(r.y) : "f"(a0), "f"(a1), "f"(m), "f"(c.x), "f"(c.y));
+  return r;
 }
 
 __device__ __forceinline__ void split_halves(float v, __half& hi, __half& lo) {
@@ -598,7 +607,8 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) shrink_kernel(c
 // stays in its registers.  B comes through a ring in shared memory that all warps read; base through a ring of
 // which each lane reads back just what it asked for itself.
 // 8192 tokens, N = 14336, r = 64: 114 us at 50 % of DRAM.  9 instructions for 32 outputs at 15 warps an SM bound it
-// (registers: three CTAs an SM spill, 164 -> 230 us, four 267, before the sums started from base).
+// (registers: three CTAs an SM spill, 164 -> 230 us, four 267, in an earlier form).  Base is read before the products
+// where registers allow (r = 64: 141.6 us a call against 151.0 with it read after them, r = 128: 305.5 and 270.6).
 // The 8 columns of mma tile j of four stand for columns 8 (c / 2) + 2 j + c % 2 of 32, so that the four tiles
 // give a lane 8 consecutive columns of a token.
 template <int RT, bool VEC>
@@ -607,6 +617,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
   using C = LoraCfg<RT>;
   constexpr int R = C::R, LD = C::LDR, RS = RT / 2, CHUNKS = R / 8;
   constexpr int BROWS = kLoraThreads / CHUNKS;           // rows of B that the CTA copies in one go
+  constexpr bool kBaseFirst = RT <= 4;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   uint8_t* const bases = smem + kExpandStages * C::EXPAND_B + warp * 2048 + lane * 16;
@@ -652,7 +663,6 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
         u[1][s] = reinterpret_cast<const uint4*>(w.lo)[from];
       }
     }
-    const bool unit = __all_sync(0xffffffffu, down[0] == 1.f && down[1] == 1.f);
     int ring_in = 0, ahead = 0;                          // next ring to fill, its distance from lo in steps
     auto ask = [&]() {
       if (lo + ahead < hi) {
@@ -701,30 +711,15 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
                 plain[t] = tk >= 0 && n0 + lane < p.N ? p.base[tk * p.ld_base + n0 + lane] : __float2half_rn(0.f);
               }
             }
-            // VEC: the sums start from base (times 2^p)
-            float acc[4][4] = {};
+            // -0 leaves base's own zeros as they are where nothing is added
+            const float zero = rank > 0 ? 0.f : -0.f;
+            float acc[4][4];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e >> 2][e & 3] = zero;
+            uint4 bv[2];                                   // VEC: base of 8 columns of each token
+            auto read_base = [&](int h) { bv[h] = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512); };
+            if (VEC && kBaseFirst) read_base(0), read_base(1);
             const bool whole = FULL || col + 8 <= p.N;
-            if (VEC) {
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint4 v = *reinterpret_cast<const uint4*>(bases + ring * C::EXPAND_BASE + (half * 2 + h) * 512);
-                const uint32_t b[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  float2 f = __half22float2(*reinterpret_cast<const __half2*>(&b[j]));
-                  if (!whole) f = make_float2(col + 2 * j < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j]) : 0.f,
-                                              col + 2 * j + 1 < p.N && tok[h] >= 0 ? __half2float(src[h][off + 2 * j + 1]) : 0.f);
-                  acc[j][2 * h] = f.x;
-                  acc[j][2 * h + 1] = f.y;
-                }
-              }
-              if (!unit) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[j][e] *= 1.f / down[e >> 1];     // a power of two: exact
-              }
-            }
 #pragma unroll
             for (int s = 0; s < RS; ++s) {
               if (s * 32 >= rank) break;
@@ -745,27 +740,25 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
               }
             }
             if (VEC) {
-              if (!unit) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) acc[j][e] *= down[e >> 1];
-              }
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 if (tok[h] < 0) continue;
                 if (whole) {
+                  if (!kBaseFirst) read_base(h);
+                  const uint32_t from[4] = {bv[h].x, bv[h].y, bv[h].z, bv[h].w};
                   uint32_t o[4];
 #pragma unroll
                   for (int j = 0; j < 4; ++j) {
-                    const __half2 r = __floats2half2_rn(acc[j][2 * h], acc[j][2 * h + 1]);
+                    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&from[j]));
+                    const __half2 r = __float22half2_rn(fma_pair(acc[j][2 * h], acc[j][2 * h + 1], down[h], f));
                     o[j] = *reinterpret_cast<const uint32_t*>(&r);
                   }
                   *reinterpret_cast<uint4*>(dst[h] + off) = make_uint4(o[0], o[1], o[2], o[3]);
                 } else {
 #pragma unroll
                   for (int e = 0; e < 8; ++e)
-                    if (col + e < p.N) dst[h][off + e] = __float2half_rn(acc[e >> 1][2 * h + (e & 1)]);
+                    if (col + e < p.N)
+                      dst[h][off + e] = __float2half_rn(fmaf(acc[e >> 1][2 * h + (e & 1)], down[h], __half2float(src[h][off + e])));
                 }
               }
             } else {

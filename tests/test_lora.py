@@ -309,3 +309,51 @@ def test_lora_clusters_that_share_an_item(pkg, oracle, cuda, T, K, N, r, n, run)
         a = p.args()
         out = None if in_place else torch.full((T, N), float("nan"), dtype=torch.float16, device=cuda)
         p.check(oracle, pkg.lora_add(*a, out=out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [6, 300, 2600])
+@pytest.mark.parametrize("N", [72, 33])
+@pytest.mark.parametrize("r", [16, 64, 128])
+@pytest.mark.parametrize("top", [0.3, 300.0])
+def test_lora_entries_of_very_different_size(pkg, oracle, cuda, T, N, r, top):
+    """A token's inner products from `top` down to 2^-19 of it, each alone in an output column that brings it back.
+    An entry keeps 22 bits, or is off by at most 2^-39 of the token's largest; to that come the sum over K in 32 bits (4
+    steps of 16 and 24 joined parts, two roundings each), that of the mma's, and fp16's rounding of the result."""
+    K, n = 64, 2
+    g = torch.Generator().manual_seed(T + N + r)
+    size = torch.exp2(-19 * torch.arange(r) / (r - 1))
+    x = torch.randn((T, K), generator=g).to(torch.float16)
+    a = (torch.randn((n, r, K), generator=g) * (top / K ** 0.5 * size).unsqueeze(1)).to(torch.float16)
+    b = torch.zeros((n, N, r))
+    alone = torch.arange(N) * (r - 1) // (N - 1)
+    b[:, torch.arange(N), alone] = (1 / size[alone]).clamp(max=3e4)
+    b = b.to(torch.float16)
+    base = torch.zeros((T, N), dtype=torch.float16)
+    ad = torch.randint(0, n, (T,), generator=g).to(torch.int32)
+    got = pkg.lora_add(*(t.to(cuda) for t in (base, x, a, b, ad))).cpu().double()
+    a64, b64, x64 = a.double()[ad.long()], b.double()[ad.long()], x.double()
+    u, ua = torch.einsum("trk,tk->tr", a64, x64), torch.einsum("trk,tk->tr", a64.abs(), x64.abs())
+    want = torch.einsum("tnr,tr->tn", b64, u)
+    eu = (4 + 24) * 2.0 ** -23 * ua + 2.0 ** -22 * u.abs() + 2.0 ** -39 * u.abs().amax(dim=1, keepdim=True)
+    tol = torch.einsum("tnr,tr->tn", b64.abs(), eu + (2 * r / 16 + 8) * 2.0 ** -23 * u.abs())
+    tol = tol + (want.abs() + tol) * 2.0 ** -11 + 2.0 ** -25
+    assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [300, 2600])
+@pytest.mark.parametrize("N,r", [(64, 16), (72, 64), (33, 64), (40, 128), (35, 128)])
+@pytest.mark.parametrize("size", [1e-6, 2e3])
+def test_lora_far_ranges_of_many_tokens(pkg, oracle, cuda, T, N, r, size):
+    """Inner products far below and above fp16's range where two products follow one another, tokens of very different
+    size among the rows of one tile, rows of any alignment."""
+    K, n = 264, 3
+    p = Problem(T, K, N, r, n, run=7, mixed=False)
+    g = torch.Generator().manual_seed(3)
+    per_token = torch.exp2(-torch.randint(0, 12, (T, 1), generator=g).float())
+    p.x = (torch.randn((T, K), generator=g) * max(size, 1) * per_token).to(torch.float16)
+    p.a = (torch.randn((n, r, K), generator=g) * size).to(torch.float16)
+    p.b = (torch.randn((n, N, r), generator=g) * (1e-6 if size > 1 else 1e4)).to(torch.float16)
+    p.scales = torch.full((n,), 1e-2 if size > 1 else 1.0)
+    p.check(oracle, pkg.lora_add(*p.args()))
