@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
         for (int e = tid; e < 8 * chunks; e += blockDim.x) {
           const int t = tok[e / chunks], c = c0 + e % chunks * 8;
           if (t < 0) continue;
-          const float zero[8] = {};
-          add_eight(p, t, c, zero, 0.f, c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.base + t * p.ld_base + c) : make_uint4(0, 0, 0, 0));
+          const float none[8] = {-0.f, -0.f, -0.f, -0.f, -0.f, -0.f, -0.f, -0.f};   // leaves base's own zeros as they are
+          add_eight(p, t, c, none, 1.f, c + 8 <= p.N ? *reinterpret_cast<const uint4*>(p.base + t * p.ld_base + c) : make_uint4(0, 0, 0, 0));
         }
       } else {
 #pragma unroll 8
@@ -360,7 +360,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, RT <= 4 ? 2 : 1) decode_ker
     auto add = [&](int gr, Step& v) {
       if (gr >= ghi) return;
       const int n0 = gr * 32, c = n0 + (lane & 3) * 8;
-      float acc[2][4] = {};
+      const float zero = rank > 0 ? 0.f : -0.f;
+      float acc[2][4] = {{zero, zero, zero, zero}, {zero, zero, zero, zero}};
 #pragma unroll
       for (int s = 0; s < RS; ++s) {
         if (s * 32 >= rank) break;

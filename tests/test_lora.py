@@ -357,3 +357,20 @@ def test_lora_far_ranges_of_many_tokens(pkg, oracle, cuda, T, N, r, size):
     p.b = (torch.randn((n, N, r), generator=g) * (1e-6 if size > 1 else 1e4)).to(torch.float16)
     p.scales = torch.full((n,), 1e-2 if size > 1 else 1.0)
     p.check(oracle, pkg.lora_add(*p.args()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [20, 300])
+@pytest.mark.parametrize("N", [72, 33])
+def test_lora_rows_without_an_adapter_keep_every_bit(pkg, cuda, T, N):
+    """Zeros of both signs, infinities and subnormals of base, where nothing is added: no adapter, or one of rank 0."""
+    p = Problem(T, 64, N, 32, 2, mixed=False)
+    p.adapters[:] = torch.tensor([-1, 0]).repeat(T)[:T]
+    p.ranks = torch.zeros(2, dtype=torch.int32)
+    p.base[:, ::3] = -0.0
+    p.base[:, 1::5] = float("-inf")
+    p.base[:, 2::7] = 6e-8
+    a = p.args()
+    out = torch.full_like(a[0], 7.0)
+    pkg.lora_add(*a, out=out)
+    assert torch.equal(out.view(torch.int16), a[0].view(torch.int16))
