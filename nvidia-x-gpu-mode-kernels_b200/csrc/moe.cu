@@ -145,9 +145,9 @@ __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __rest
 
 // out[t] = sum of its slots' rows of y, in slot order (and of the parts of each); eight columns a thread.
 // 4096 tokens of 4096 columns in 2 slots each: it ends 38 us after the down product, 4.4 TB/s of y (fp32) and out.
-__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ y, int parts, int64_t part_stride,
-                                                      const int* __restrict__ rows, int64_t T, int k, int D,
-                                                      __half* __restrict__ out, int64_t ldo, int vec) {
+// No __restrict__: y is still being written when this kernel starts, so it is not read-only for the kernel's lifetime.
+__global__ void __launch_bounds__(256) combine_kernel(const float* y, int parts, int64_t part_stride, const int* rows,
+                                                      int64_t T, int k, int D, __half* out, int64_t ldo, int vec) {
   griddep_launch();
   griddep_wait();
   const int per = D / 8;
