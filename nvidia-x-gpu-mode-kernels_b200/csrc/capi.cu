@@ -16,11 +16,10 @@ thread_local char g_msg[512] = "";
 // One word per device (a __device__ variable exists once per device context).
 __device__ uint32_t g_error_word;
 
-constexpr int kMaxDevices = 64;
 // Per-device addresses, published with release stores and read with acquire
 // loads outside the lock (double-checked initialisation).
 std::atomic<uint32_t*> g_err_ptr[kMaxDevices] = {};
-int g_sms[kMaxDevices] = {};
+std::atomic<int> g_sms[kMaxDevices] = {};
 std::mutex g_mu;
 
 __global__ void selftest_wait_kernel(uint32_t* err, uint64_t budget_ns, uint32_t* done) {
@@ -62,28 +61,28 @@ int sm_count() {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return 148;
-  if (!g_sms[dev]) {
-    int n = 0;
+  int n = g_sms[dev].load(std::memory_order_relaxed);     // the value alone: whoever finds 0 asks for the same one
+  if (!n) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    g_sms[dev] = n;
+    g_sms[dev].store(n, std::memory_order_relaxed);
   }
-  return g_sms[dev];
+  return n;
 }
 
 namespace {
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+std::atomic<PFN_cuTensorMapEncodeTiled_v12000> g_encode{nullptr};
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  if (g_encode) return g_encode;
+  if (auto found = g_encode.load(std::memory_order_acquire)) return found;
   std::lock_guard<std::mutex> lk(g_mu);
-  if (!g_encode) {
+  if (!g_encode.load(std::memory_order_relaxed)) {
     void* fn = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &q) ==
             cudaSuccess && q == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+      g_encode.store(reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn), std::memory_order_release);
   }
-  return g_encode;
+  return g_encode.load(std::memory_order_relaxed);
 }
 }  // namespace
 

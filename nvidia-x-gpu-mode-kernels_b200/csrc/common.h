@@ -6,6 +6,7 @@
 #include <cstdarg>
 #include <cuda_runtime.h>
 #include "../../include/nvfp4_b200.h"
+#include "once.h"
 
 namespace nvfp4 {
 

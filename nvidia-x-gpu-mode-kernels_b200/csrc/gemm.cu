@@ -48,14 +48,14 @@ namespace {
 
 template <class C, int MAXG>
 int launch_gemm(const GemmParams<MAXG>& P, cudaStream_t stream) {
-  static bool attr_set[64] = {};
+  static OncePerDevice once;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 64 && !attr_set[dev]) {
+  const int rc = once.run(dev, [] {
     cudaError_t e = cudaFuncSetAttribute(gemm_kernel<C, MAXG>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(gemm)");
-    attr_set[dev] = true;
-  }
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaFuncSetAttribute(gemm)");
+  });
+  if (rc) return rc;
   int grid = sm_count();
   if (P.total_tiles < grid) grid = P.total_tiles;
   if (grid < 1) return NVFP4_OK;
@@ -65,11 +65,11 @@ int launch_gemm(const GemmParams<MAXG>& P, cudaStream_t stream) {
 
 template <class C, int MAXG>
 int launch_pair(const GemmParams<MAXG>& P, cudaStream_t stream) {
-  static bool attr_set[64] = {};
-  static int max_pairs[64] = {};
+  static OncePerDevice once;
+  static int max_pairs[kMaxDevices] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
+  if (dev < 0 || dev >= kMaxDevices) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   auto kern = pair_kernel<C, MAXG>;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -82,7 +82,7 @@ int launch_pair(const GemmParams<MAXG>& P, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (!attr_set[dev]) {
+  const int rc = once.run(dev, [&]() -> int {
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(pair gemm)");
     cfg.gridDim = dim3(2 * (sm_count() / 2));
@@ -90,8 +90,9 @@ int launch_pair(const GemmParams<MAXG>& P, cudaStream_t stream) {
     e = cudaOccupancyMaxActiveClusters(&n, kern, &cfg);
     if (e != cudaSuccess || n < 1) return fail(NVFP4_ERR_UNSUPPORTED, "no CTA pairs fit on this device");
     max_pairs[dev] = n;
-    attr_set[dev] = true;
-  }
+    return NVFP4_OK;
+  });
+  if (rc) return rc;
   int pairs = max_pairs[dev];
   if (P.total_tiles < pairs) pairs = P.total_tiles;
   if (pairs < 1) return NVFP4_OK;
@@ -388,14 +389,14 @@ extern "C" int nvfp4_mma_peak_pattern(int iters, int pattern, void* stream) {
   uint32_t* err = device_error_word();
   if (!err) return fail(NVFP4_ERR_CUDA, "nvfp4_mma_peak: cannot resolve the device error word");
   constexpr int kSmem = 49152 + 64 + 1024;
-  static bool attr_set[64] = {};
+  static OncePerDevice once;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 64 && !attr_set[dev]) {
+  const int rc = once.run(dev, [] {
     cudaError_t e = cudaFuncSetAttribute(mma_peak_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(mma_peak)");
-    attr_set[dev] = true;
-  }
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaFuncSetAttribute(mma_peak)");
+  });
+  if (rc) return rc;
   mma_peak_kernel<<<sm_count(), 128, kSmem, static_cast<cudaStream_t>(stream)>>>(iters, pattern, err);
   return check_launch("mma_peak_kernel");
 }

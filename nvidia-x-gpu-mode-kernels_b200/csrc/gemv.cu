@@ -498,16 +498,16 @@ int launch_tma(const GemvArgs& p, cudaStream_t stream, int64_t* grid_out) {
     *grid_out = grid_of<C>(p);
     return NVFP4_OK;
   }
-  static bool attr_set[64] = {};
+  static OncePerDevice once;
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 64 && !attr_set[dev]) {
+  int rc = once.run(dev, [] {
     cudaError_t e = cudaFuncSetAttribute(gemv_tma_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(gemv)");
-    attr_set[dev] = true;
-  }
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaFuncSetAttribute(gemv)");
+  });
+  if (rc) return rc;
   GemvMaps maps;
-  int rc = cached_maps<C>(p, maps);
+  rc = cached_maps<C>(p, maps);
   if (rc) return rc;
   const int64_t grid = grid_of<C>(p);
   cudaLaunchConfig_t cfg = {};

@@ -855,12 +855,12 @@ int decode_cluster(int T, int n, const int (&fit)[4]) {
 template <int RT>
 int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t stream) {
   using C = LoraCfg<RT>;
-  static bool attr_set[64] = {};
-  static int fits[64][4];                // clusters of 1, 2, 4, 8 for few tokens that run at once
+  static OncePerDevice once;
+  static int fits[kMaxDevices][4];       // clusters of 1, 2, 4, 8 for few tokens that run at once
   constexpr int kWide = RT <= 4 ? 2 : 1, kSlots = RT <= 4 ? 2 : 1;   // m tiles a warp, CTAs an SM, of the first product
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
+  if (dev < 0 || dev >= kMaxDevices) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -871,7 +871,7 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (!attr_set[dev]) {
+  int rc = once.run(dev, [&] {
     cudaError_t e = cudaFuncSetAttribute(decode_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(8));
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(decode_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, DecodeCfg<RT>::smem(8));
@@ -892,9 +892,9 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
       e = cudaFuncSetAttribute(expand_kernel<RT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(expand_kernel<RT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::EXPAND_SMEM);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(low-rank products)");
-    attr_set[dev] = true;
-  }
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaFuncSetAttribute(low-rank products)");
+  });
+  if (rc) return rc;
   if (p.T <= kDecodeTokens) {
     const int size = decode_cluster(p.T, p.n, fits[dev]);
     const int ncta = 1 << size;
@@ -908,7 +908,7 @@ int lora_run(const LoraArgs& p, const LoraLayout& m, uint8_t* ws, cudaStream_t s
   const Plan plan = {reinterpret_cast<int*>(ws), reinterpret_cast<PlanTile*>(ws + m.tiles),
                      reinterpret_cast<int*>(ws + m.row), reinterpret_cast<int*>(ws + m.slot)};
   // tokens without an adapter become adapter n's, which only copies; in place they are left out
-  int rc = launch_plan(p.adapters, p.T, p.n, p.in_place ? -1 : p.n, kTile, kTile, plan, stream);
+  rc = launch_plan(p.adapters, p.T, p.n, p.in_place ? -1 : p.n, kTile, kTile, plan, stream);
   if (rc) return rc;
   const LoraRows rows = {plan.head, plan.tiles, plan.slot, reinterpret_cast<__half*>(ws + m.hi),
                          reinterpret_cast<__half*>(ws + m.lo), reinterpret_cast<float*>(ws + m.down)};

@@ -324,13 +324,11 @@ int expert_params(const MoeCall& c, ExpertParams& P) {
   P.part_stride = m.rows * c.D;
   P.err = c.err;
   if (m.max_tiles * P.wtiles * m.parts > INT32_MAX / 2) return fail(NVFP4_ERR_INVALID, "nvfp4_moe_mlp: too many tiles");
-  static bool attr_set[64] = {};
-  if (!attr_set[c.dev]) {
+  static OncePerDevice once;
+  return once.run(c.dev, [] {
     cudaError_t e = cudaFuncSetAttribute(expert_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-    if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(expert product)");
-    attr_set[c.dev] = true;
-  }
-  return NVFP4_OK;
+    return e == cudaSuccess ? NVFP4_OK : cuda_fail(e, "cudaFuncSetAttribute(expert product)");
+  });
 }
 
 template <class C>
@@ -407,7 +405,7 @@ extern "C" int nvfp4_moe_mlp(const void* x, int64_t ldx, const int32_t* ids, con
       (rc = check_weights("down", w_down, sf_down, E, F, ld_down, es_down, sfe_down)))
     return rc;
   cudaGetDevice(&c.dev);
-  if (c.dev < 0 || c.dev >= 64) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
+  if (c.dev < 0 || c.dev >= kMaxDevices) return fail(NVFP4_ERR_UNSUPPORTED, "device index out of range");
   c.err = device_error_word();
   if (!c.err) return fail(NVFP4_ERR_CUDA, "nvfp4_moe_mlp: cannot resolve the device error word");
   using Up = ExpertCfg<false, true, 128, 1, 4>;
