@@ -267,8 +267,9 @@ NVFP4_API int nvfp4_route_experts(const void* logits, int dtype, int64_t T, int6
  *   Gate and up share their strides.
  * D and F are multiples of 64; E <= 1024, k <= 32, T * k <= 2^24; T may be 0.
  * The counts per expert stay on the GPU.  `workspace` is device memory of at
- * least nvfp4_moe_workspace() bytes, 256-byte aligned, with undefined contents,
- * in use until the call's work on `stream` ends.  No counterpart in the
+ * least nvfp4_moe_workspace() bytes (asked for with the same device current),
+ * 256-byte aligned, with undefined contents, in use until the call's work on
+ * `stream` ends.  No counterpart in the
  * reference.
  */
 NVFP4_API int nvfp4_moe_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t F, int64_t* bytes);

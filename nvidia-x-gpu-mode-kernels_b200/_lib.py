@@ -107,6 +107,21 @@ def call(name: str, index: int, *args) -> None:
         check(status)
 
 
+def query(name: str, index: int, *args) -> int:
+    """The int64 that an entry point without a stream writes to its last
+    argument, with device `index` current, as a call's workspace may depend on it."""
+    f = getattr(_lib or lib(), name)
+    value = ctypes.c_int64(0)
+    if index == torch.cuda.current_device():
+        status = f(*args, ctypes.byref(value))
+    else:
+        with torch.cuda.device(index):
+            status = f(*args, ctypes.byref(value))
+    if status != 0:
+        check(status)
+    return value.value
+
+
 def check(status: int) -> None:
     if status != 0:
         msg = lib().nvfp4_last_error().decode(errors="replace")

@@ -16,8 +16,6 @@ workspace comes from torch's allocator, on the current stream.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
@@ -88,11 +86,10 @@ def moe_mlp(x, ids, weights, w_gate, w_up, w_down, scale_gate, scale_up, scale_d
     elif not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or out.shape != (T, D) \
             or out.stride(1) != 1 or out.get_device() != index:
         raise ValueError(f"out must be a float16 [{T}, {D}] tensor with unit column stride on the device of x")
-    need = ctypes.c_int64(0)
-    _lib.check(_lib.lib().nvfp4_moe_workspace(T, k, E, D, F, ctypes.byref(need)))
-    ws = x.new_empty(need.value, dtype=torch.uint8)
+    need = _lib.query("nvfp4_moe_workspace", index, T, k, E, D, F)
+    ws = x.new_empty(need, dtype=torch.uint8)
     _lib.call("nvfp4_moe_mlp", index, x.data_ptr(), s_x[0], ids.data_ptr(), weights.data_ptr(), T, k, E, D, F,
               w_gate.data_ptr(), w_up.data_ptr(), sg.data_ptr(), su.data_ptr(), s_in[1], s_in[0], sfe,
               w_down.data_ptr(), sd.data_ptr(), s_down[1], s_down[0], sd.stride(0), out.data_ptr(), out.stride(0),
-              ws.data_ptr(), need.value)
+              ws.data_ptr(), need)
     return out
