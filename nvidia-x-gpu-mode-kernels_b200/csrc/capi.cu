@@ -105,14 +105,15 @@ struct TmapKeyHash {
     return (size_t)h;
   }
 };
-std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> g_tmap_cache;
+std::unordered_map<TmapKey, CUtensorMap, TmapKeyHash> g_tmap_cache[2];   // by TmapOf
 std::mutex g_tmap_mu;
 constexpr size_t kTmapCacheMax = 4096;
 }  // namespace
 
 int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const void* base,
                 const uint64_t* dims, const uint64_t* strides_bytes, const uint32_t* box,
-                CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo) {
+                CUtensorMapSwizzle swizzle, CUtensorMapL2promotion promo, TmapOf of) {
+  auto& cache = g_tmap_cache[of == TmapOf::kWorkspace];
   TmapKey key;
   std::memset(&key, 0, sizeof(key));
   key.base = base;
@@ -127,8 +128,8 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const voi
   }
   {
     std::lock_guard<std::mutex> lk(g_tmap_mu);
-    auto it = g_tmap_cache.find(key);
-    if (it != g_tmap_cache.end()) {
+    auto it = cache.find(key);
+    if (it != cache.end()) {
       *map = it->second;
       return NVFP4_OK;
     }
@@ -149,8 +150,8 @@ int encode_tmap(CUtensorMap* map, CUtensorMapDataType dtype, int rank, const voi
     return fail(NVFP4_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d): rank %d dims[0]=%llu box[0]=%u", (int)r,
                 rank, (unsigned long long)dims[0], box[0]);
   std::lock_guard<std::mutex> lk(g_tmap_mu);
-  if (g_tmap_cache.size() >= kTmapCacheMax) g_tmap_cache.clear();
-  g_tmap_cache.emplace(key, *map);
+  if (cache.size() >= kTmapCacheMax) cache.clear();
+  cache.emplace(key, *map);
   return NVFP4_OK;
 }
 

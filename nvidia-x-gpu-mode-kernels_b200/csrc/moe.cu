@@ -269,13 +269,15 @@ int token_maps(ExpertParams& P, const void* codes, const void* sf, int64_t rows,
   const uint64_t dims[2] = {(uint64_t)(K / 2), (uint64_t)rows};
   const uint64_t str[1] = {(uint64_t)(K / 2)};
   const uint32_t box[2] = {KSTEP_BYTES, (uint32_t)box_rows};
-  int rc = encode_tmap(&P.tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+  int rc = encode_tmap(&P.tt, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, codes, dims, str, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, TmapOf::kWorkspace);
   if (rc) return rc;
   const uint64_t nk64 = (uint64_t)(K / 64);
   const uint64_t sdims[3] = {128, nk64, (uint64_t)(rows / 128)};
   const uint64_t sstr[2] = {512, nk64 * 512};
   const uint32_t sbox[3] = {128, (uint32_t)kps, 1};
-  return encode_tmap(&P.tst, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, sf, sdims, sstr, sbox, CU_TENSOR_MAP_SWIZZLE_NONE);
+  return encode_tmap(&P.tst, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, sf, sdims, sstr, sbox, CU_TENSOR_MAP_SWIZZLE_NONE,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, TmapOf::kWorkspace);
 }
 
 struct MoeCall {

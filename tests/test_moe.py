@@ -315,3 +315,18 @@ def test_moe_both_sides_of_the_rules(pkg, oracle, cuda, T, k, E, D, F):
     torch.cuda.synchronize()
     assert pkg._lib.device_errors() == 0
     p.check(oracle, out)
+
+
+@pytest.mark.gpu
+def test_moe_more_token_counts_than_maps_are_kept(pkg, oracle, cuda):
+    """1100 token counts: four tensor maps of its workspace each, more than are kept at a time."""
+    p = Problem(pkg, 1100, 1, 2, 64, 64)
+    x, ids, w, *rest = p.args()
+    want = pkg.moe_mlp(x, ids, w, *rest)
+    p.check(oracle, want)
+    for T in range(1, 1101):
+        got = pkg.moe_mlp(x[:T], ids[:T], w[:T], *rest)
+        if T % 50 == 0:
+            assert torch.equal(got, pkg.moe_mlp(x[:T], ids[:T], w[:T], *rest))
+    assert torch.equal(got, want)
+    assert pkg._lib.device_errors() == 0
