@@ -13,6 +13,8 @@ weights, each token's own low-rank term, from the activations before their quant
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
@@ -61,9 +63,10 @@ def lora_add(base, x, a, b, adapters, scales=None, ranks=None, out=None):
     ad = _vector("adapters", adapters, T, torch.int32, index)
     sc = None if scales is None else _vector("scales", scales, n, torch.float32, index)
     rk = None if ranks is None else _vector("ranks", ranks, n, torch.int32, index)
-    need = _lib.query("nvfp4_lora_workspace", index, T, r, n)
-    ws = base.new_empty(need, dtype=torch.uint8) if need else None
+    need = ctypes.c_int64(0)
+    _lib.check(_lib.lib().nvfp4_lora_workspace(T, r, n, ctypes.byref(need)))
+    ws = base.new_empty(need.value, dtype=torch.uint8) if need.value else None
     _lib.call("nvfp4_lora_add", index, base.data_ptr(), s_base[0], x.data_ptr(), s_x[0], a.data_ptr(), s_a[1], s_a[0],
               b.data_ptr(), s_b[1], s_b[0], ad, sc, rk, T, K, N, r, n, out.data_ptr(), s_out[0],
-              None if ws is None else ws.data_ptr(), need)
+              None if ws is None else ws.data_ptr(), need.value)
     return out
