@@ -122,6 +122,13 @@ def query(name: str, index: int, *args) -> int:
     return value.value
 
 
+def no_gradient(name: str, t: torch.Tensor) -> None:
+    """Refuses an output that autograd follows: the library writes to it
+    behind autograd's back, and the gradients through it would be wrong."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient: the operators are for inference, call them under torch.no_grad()")
+
+
 def check(status: int) -> None:
     if status != 0:
         msg = lib().nvfp4_last_error().decode(errors="replace")

@@ -9,7 +9,8 @@ weights, each token's own low-rank term, from the activations before their quant
   largest rank, padded to a multiple of 16 (up to 128); ``ranks`` int32 ``[n]`` says how much of it each adapter uses,
   what lies beyond may hold anything;
 * ``adapters`` int32 ``[T]`` on the GPU: an index outside ``[0, n)``, such as -1, is a token without an adapter;
-* ``out`` is ``base`` (in place) unless given; it may not overlap ``x``.
+* ``out`` is ``base`` (in place) unless given; it may not overlap ``x``, nor require a gradient outside of
+  ``torch.no_grad()``: there is no backward pass.
 """
 from __future__ import annotations
 
@@ -60,6 +61,7 @@ def lora_add(base, x, a, b, adapters, scales=None, ranks=None, out=None):
         s_out = _half("out", out, 2, index)
         if out.shape != base.shape:
             raise ValueError(f"out has shape {tuple(out.shape)}, expected {tuple(base.shape)}")
+    _lib.no_gradient("out (base, in place)", out)
     ad = _vector("adapters", adapters, T, torch.int32, index)
     sc = None if scales is None else _vector("scales", scales, n, torch.float32, index)
     rk = None if ranks is None else _vector("ranks", ranks, n, torch.int32, index)

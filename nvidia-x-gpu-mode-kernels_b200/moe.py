@@ -86,6 +86,8 @@ def moe_mlp(x, ids, weights, w_gate, w_up, w_down, scale_gate, scale_up, scale_d
     elif not isinstance(out, torch.Tensor) or out.dtype != torch.float16 or out.shape != (T, D) \
             or out.stride(1) != 1 or out.get_device() != index:
         raise ValueError(f"out must be a float16 [{T}, {D}] tensor with unit column stride on the device of x")
+    else:
+        _lib.no_gradient("out", out)
     need = _lib.query("nvfp4_moe_workspace", index, T, k, E, D, F)
     ws = x.new_empty(need, dtype=torch.uint8)
     _lib.call("nvfp4_moe_mlp", index, x.data_ptr(), s_x[0], ids.data_ptr(), weights.data_ptr(), T, k, E, D, F,

@@ -47,6 +47,8 @@ def route_experts(logits: torch.Tensor, top_k: int, bias: torch.Tensor | None = 
     elif not isinstance(weights, torch.Tensor) or weights.dtype != torch.float32 or weights.shape != (T, top_k) \
             or weights.get_device() != index or not weights.is_contiguous():
         raise ValueError(f"weights must be a contiguous float32 tensor [{T}, {top_k}] on the device of logits")
+    else:
+        _lib.no_gradient("weights", weights)
     if ids is None:
         ids = logits.new_empty((T, top_k), dtype=torch.int32)
     elif not isinstance(ids, torch.Tensor) or ids.dtype != torch.int32 or ids.shape != (T, top_k) \
