@@ -737,8 +737,15 @@ __global__ void __launch_bounds__(256, VPL <= 8 ? 4 : VPL == 16 ? 2 : 1) route_k
   float bias[VPL];
   // softmax weights as they are want an accurate sum over all experts, which the keyed pass has
   const bool keyed = !BIAS || (SOFTMAX && !p.renorm);
-  // 16-bit logits that rank by themselves are equal too often (5.0 us with the short form first, 4.5 without, at 4097 x 60)
-  bool odd = (GROUPS && p.group_lanes == 0) || (SOFTMAX && !p.renorm) || (!BIAS && p.dtype != 0);
+  // 16-bit logits that rank by themselves are often equal, and a row is then tried in vain: it counts where a warp has no
+  // other row, and for bfloat16 the more of the best there are.  us with the short form first and without it:
+  //   one row a warp    4097 x 60 fp16 5.1 and 4.4, bf16 5.2 and 4.6; 64 x 256 5.5 and 4.4, 5.6 and 4.5
+  //   fp16, batches     32768 x 256, k = 8 22.9 and 33.7, k = 16 36.6 and 41.7; x 60, k = 4 13.9 and 21.8; 9500 x 256 10.6 and 13.8
+  //   bf16, k = 4       32768 x 256 24.6 and 33.4, x 60 16.9 and 23.7; 12000 x 256 13.4 and 13.9, x 128 11.3 and 11.1
+  //   bf16, k = 6, 8    32768 x 256 35.1 and 34.3, x 32 17.6 and 19.6; 12000 x 60 11.9 and 10.3, x 128 14.8 and 13.1
+  //   bf16, 8 groups    32768 x 256, k = 8 67.1 and 82.8, k = 12 95.4 and 81.6; 12000 x 256, k = 8 33.3 and 39.2
+  const bool ties = !BIAS && p.dtype != 0 && (p.batch == 1 || (p.dtype == 2 && p.k > (GROUPS ? 8 : 4)));
+  bool odd = ties || (GROUPS && p.group_lanes == 0) || (SOFTMAX && !p.renorm);
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     bias[i] = BIAS && lane * VPL + i < p.E ? p.bias[lane * VPL + i] : 0.f;

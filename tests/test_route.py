@@ -317,3 +317,18 @@ def test_route_weights_that_a_scale_brings_back(pkg, oracle, cuda, scale, renorm
     bias = torch.randn(24, generator=torch.Generator().manual_seed(4)).to(cuda) if with_bias else None
     got = pkg.route_experts(x.to(cuda), 6, bias=bias, score="sigmoid", renormalize=renormalize, scale=scale)
     _check_weights(oracle, got, x, 6, bias, score="sigmoid", renormalize=renormalize, scale=scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("T,E,k,groups,top_groups", [
+    (9471, 64, 4, 1, 1), (9472, 64, 4, 1, 1), (9473, 200, 5, 1, 1), (12000, 200, 4, 1, 1), (9600, 256, 8, 8, 4), (9600, 256, 9, 8, 4)])
+def test_route_both_sides_of_the_rule_on_ties(pkg, oracle, cuda, T, E, k, groups, top_groups, dtype, score):
+    x = (torch.randn((T, E), generator=torch.Generator().manual_seed(T + k)) * 2).to(dtype)
+    x[::2] = (x[::2].float() * 4).round().div(4).to(dtype)       # half of the rows with many ties
+    w, ids = pkg.route_experts(x.to(cuda), k, score=score, num_groups=groups, top_groups=top_groups)
+    rows = torch.cat([torch.arange(0, T, 31), torch.tensor([T - 1])])
+    rw, ri = oracle.route(x[rows], k, score=score, groups=groups, top_groups=top_groups)
+    np.testing.assert_array_equal(ids.cpu()[rows].numpy(), ri)
+    np.testing.assert_allclose(w.cpu()[rows].numpy().astype(np.float64), rw, rtol=RTOL, atol=ATOL)
