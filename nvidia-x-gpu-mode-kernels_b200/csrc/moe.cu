@@ -70,10 +70,12 @@ __global__ void __launch_bounds__(256) scatter_kernel(const int* rows, ScatterAr
 
 // Plan and scatter in one launch, for few slots: every CTA (one per token) counts all of them for itself and
 // finds the rows of its own token's, a warp a slot: its expert's first row plus the number of equal ids before
-// it.  CTA 0 lists the tiles.  Against the two kernels one after the other: 2.7 us less a call for one token, 1.4 at
-// 512 slots; every CTA counts all slots, so many tokens of many slots are slower
-// (2000 tokens of one slot: 64 us instead of 55): up to 2048 slots for up to 384 tokens (333 of 4: 43.2 and 44.2).
-constexpr int kFusedSlots = 2048, kFewSlots = 1024, kFewTokens = 384;
+// it.  CTA 0 lists the tiles.  Every CTA counts all slots, which pays while the CTAs run at once.  Calls, us, so and with
+// the two kernels one after the other (64 experts of 2048 x 1024): 1 token of 8 slots 20.1 and 21.4, 256 of 8 64.7 and
+// 66.1, 384 of 5 62.5 and 63.2, 512 of 2 56.7 and 57.8, 512 of 4 63.7 and 64.3; 682 of 3 64.3 and 63.9, 1024 of 1 59.7 and
+// 56.8, 1000 of 2 68.3 and 64.8, 2000 of 1 75.6 and 66.7.  Few tokens of many slots are as fast either way (64 of 32:
+// 75.1 and 74.6).
+constexpr int kFusedSlots = 2048, kFewTokens = 512;
 
 __global__ void __launch_bounds__(256) plan_scatter_kernel(const int32_t* __restrict__ ids, int n, int experts, int align,
                                                            int tile, Plan p, ScatterArgs a) {
@@ -351,7 +353,7 @@ int moe_run(const MoeCall& c) {
   const ScatterArgs a = {c.x, c.ldx, c.T, (int)c.k, (int)c.D, c.weights, c.ws + m.xq, c.ws + m.xs,
                          reinterpret_cast<float*>(c.ws + m.row_weight)};
   const int64_t n = c.T * c.k;
-  if (n <= kFewSlots || (n <= kFusedSlots && c.T <= kFewTokens)) {
+  if (n <= kFusedSlots && c.T <= kFewTokens) {
     plan_scatter_kernel<<<(unsigned)c.T, 256, 0, c.stream>>>(c.ids, (int)n, (int)c.E, m.tile, m.tile, plan, a);
     if ((rc = check_launch("plan_scatter_kernel"))) return rc;
   } else {

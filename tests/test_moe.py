@@ -330,3 +330,16 @@ def test_moe_more_token_counts_than_maps_are_kept(pkg, oracle, cuda):
             assert torch.equal(got, pkg.moe_mlp(x[:T], ids[:T], w[:T], *rest))
     assert torch.equal(got, want)
     assert pkg._lib.device_errors() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k,E,D,F", [
+    (512, 4, 8, 128, 128), (512, 5, 8, 128, 128), (513, 1, 8, 128, 128), (513, 3, 8, 64, 128), (64, 32, 64, 64, 64),
+    (1024, 1, 40, 64, 128),
+])
+def test_moe_both_sides_of_the_rule_on_the_plans_launch(pkg, oracle, cuda, T, k, E, D, F):
+    p = Problem(pkg, T, k, E, D, F)
+    out = pkg.moe_mlp(*p.args())
+    torch.cuda.synchronize()
+    assert pkg._lib.device_errors() == 0
+    p.check(oracle, out)
