@@ -122,6 +122,25 @@ __device__ __forceinline__ void expert_mma(uint32_t tmem, uint64_t dt, uint64_t 
   }
 }
 
+// silu(g) * u.  An h that lies beside the border of two 4-bit codes is decided by its last digits: the approximations
+// that an fp16 result can do with (off by 2^-20 at g = -16) put outputs up to 5 times as far from the definition as 32-bit
+// functions do.  e^-g = 2^t * e^d with t = -g log2(e) as rounded and d = -g - t ln(2), which a fused step gets without
+// cancellation; |d| < 2^-18, so e^d is 1 + d.  The quotient gets one step of its residual.  Off by at most 12 units of
+// 2^-24: 4 of ex2.approx, 4 of ln(2) at |t| = 115, one each of the product, 1 + e, the quotient and the product with u.
+// Calls, us, with the approximations, with this and with CUDA's exponential and quotient: 4096 tokens of 2 of 8 experts
+// of 4096 x 14336 874, 884 and 942; 333 of 4 of 16 of 1984 x 1344 45.2, 45.2 and 54.7; 64 of 8 of 64 112.7, 112.9 and 115.0.
+__device__ __forceinline__ float silu_mul_32(float g, float u) {
+  const float a = fmaxf(g, -80.f);         // below, |g|, |u| < 2^20 (6 * 448)^2 leave nothing that a scale of 2^-9 holds
+  const float t = a * -1.4426950408889634f;
+  float p, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(t));
+  const float d = fmaf(t, -0.6931471805599453f, -a);
+  const float n = 1.f + fmaf(p, d, p);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(n));
+  const float q = g * r;
+  return fmaf(fmaf(-q, n, g), r, q) * u;
+}
+
 // Through L2: the down product's early reads come before its griddep_wait.
 __device__ __forceinline__ PlanTile load_tile(const PlanTile* p) {
   const int4 a = __ldcg(reinterpret_cast<const int4*>(p));
@@ -376,7 +395,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
         tc::wait_ld();
         release();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) buf[j * 36 + lane] = silu_mul(__uint_as_float(g[j]), __uint_as_float(u[j]));
+        for (int j = 0; j < 16; ++j) buf[j * 36 + lane] = silu_mul_32(__uint_as_float(g[j]), __uint_as_float(u[j]));
         __syncwarp();
         float v[16];
 #pragma unroll
@@ -426,7 +445,7 @@ __global__ void __launch_bounds__(C::THREADS, 1) expert_kernel(const __grid_cons
           for (int b = 0; b < 2; ++b) {
             float h[16];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) h[j] = silu_mul(__uint_as_float(v[16 * b + j]), __uint_as_float(u[16 * b + j]));
+            for (int j = 0; j < 16; ++j) h[j] = silu_mul_32(__uint_as_float(v[16 * b + j]), __uint_as_float(u[16 * b + j]));
             uint32_t packed[2];
             scales |= quant_floats(h, packed) << (8 * b);
             codes[2 * b] = packed[0];

@@ -343,3 +343,76 @@ def test_moe_both_sides_of_the_rule_on_the_plans_launch(pkg, oracle, cuda, T, k,
     torch.cuda.synchronize()
     assert pkg._lib.device_errors() == 0
     p.check(oracle, out)
+
+
+def _digits(v, scales):
+    """v = sum_b scales[b] * (sum of 15 e2m1 values): the codes [len(scales), 15], coarsest scale first."""
+    grid = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+    out = np.zeros((len(scales), 15), np.int64)
+    for b, s in enumerate(scales):
+        m = np.clip(np.round(v / s * 2) / 2, -84, 84)        # a multiple of 0.5
+        v -= m * s
+        left = abs(m)
+        for j in range(15):
+            c = int(np.searchsorted(grid, left, side="right")) - 1
+            out[b, j] = c | (8 if m < 0 and c else 0)
+            left -= grid[c]
+        assert left == 0
+    assert v == 0
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("copies", [1, 40])
+def test_moe_values_beside_the_borders_of_codes(pkg, cuda, copies):
+    """Gate and up products that are exact in 32 bits and whose silu(g) * u lies between 12.4 and 13.8 units of 2^-24 from
+    the border of two codes, a little more than the error that SiLU in 32 bits may have: h must get the code of the exact
+    value.  The down product is the identity, so the output is h as quantised.  Both forms (16 tokens, 640 tokens of 16
+    experts)."""
+    E, D = 16, 128
+    unit, scale = 2.0 ** -24, 2.0 ** -9                       # of h's blocks
+    scales = [2.0 ** 8, 2.0 ** 1, 2.0 ** -6, 2.0 ** -9]
+    silu = lambda g: g / (1 + np.exp(-g))
+    # g where g * log2(e) rounds far down, so that an exponential of the rounded product is off the most
+    g = -np.arange(17 * 1024, 20 * 1024) / 1024.0
+    t = (g.astype(np.float32) * np.float32(-1.4426950408889634)).astype(np.float64)
+    g = g[np.argsort((t - g * -1.4426950408889634))][:E * 120]
+    pairs, want = np.zeros((E, D, 2)), np.zeros((E, D))
+    borders, values = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5]), np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+    at = beside = 0
+    for e in range(E):
+        for c in range(D):
+            if c % 16 == 0:                                   # its amax fixes the block's scale
+                pairs[e, c] = -12.0, np.round(6 * scale / silu(-12.0) * 1024) / 1024
+            else:
+                reach = borders[(borders * scale / -silu(g[at]) < 21000)]
+                u = reach[-1] * scale / silu(g[at])           # negative: h is positive
+                near = (np.floor(u * (1 - 13.1 * unit) * 1024) + np.arange(-9, 10)) / 1024
+                off = 1 - near / u
+                fit = near[(off > 12.4 * unit) & (off < 13.8 * unit)]
+                beside += len(fit) > 0
+                pairs[e, c] = g[at], fit[0] if len(fit) else np.round(u * 0.97 * 1024) / 1024   # u's grid is too coarse there
+                at += 1
+            v = silu(pairs[e, c, 0]) * pairs[e, c, 1] / scale
+            want[e, c] = values[np.searchsorted(borders, v)] * scale
+    assert beside > 1000
+    codes = np.zeros((2, E, D, D), np.int64)
+    for m in range(2):
+        for e in range(E):
+            for c in range(D):
+                d = _digits(pairs[e, c, m], scales)
+                for b in range(4):
+                    codes[m, e, c, 16 * b + 1:16 * b + 16] = d[b]
+    pack = lambda c: torch.from_numpy((c[..., 0::2] | c[..., 1::2] << 4).astype(np.uint8)).to(cuda)
+    e4m3 = lambda v: torch.tensor(v, dtype=torch.float32).to(torch.float8_e4m3fn).view(torch.uint8)
+    sf = e4m3(scales + [1.0] * 4).repeat(E, D, 1).to(cuda)
+    eye = torch.zeros((E, D, D), dtype=torch.int64)
+    eye[:, torch.arange(D), torch.arange(D)] = 2              # 1.0
+    x = torch.ones((E * copies, D), dtype=torch.float16, device=cuda)
+    x[:, ::16] = 6.0                                          # a scale of 1; the weights there are 0
+    ids = torch.arange(E, dtype=torch.int32, device=cuda).repeat(copies).unsqueeze(1).contiguous()
+    one = torch.full((E, D, D // 16), 0x38, dtype=torch.uint8, device=cuda)
+    out = pkg.moe_mlp(x, ids, torch.ones((E * copies, 1), device=cuda), pack(codes[0]), pack(codes[1]), pack(eye.numpy()),
+                      sf, sf, one)
+    got = out.cpu().double().numpy().reshape(copies, E, D)
+    assert (got == want).all(), f"{(got != want).sum()} of {got.size} codes"
