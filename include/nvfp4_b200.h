@@ -241,7 +241,9 @@ NVFP4_API int nvfp4_quantize(const void* x, int64_t M, int64_t K, int64_t ldx, v
  *   renorm is non-zero, times scale.
  * An expert whose logit or bias is -inf or NaN is off: it has score 0, and a
  * slot that no expert fills gets id -1 and weight 0.  +inf counts as the
- * largest float.  The ids are those of 64-bit arithmetic; weights are float32.
+ * largest float.  The ids are those of 64-bit arithmetic (choices that differ in
+ * its last digit only may come in either order); weights are float32, scores
+ * that 64 bits cannot hold (about e^-745) count as 0 in them.
  * 1 <= E <= 1024, k <= min(32, E), groups <= 32 and divides E; T may be 0.
  * weights and ids are contiguous [T, k].  No counterpart in the reference.
  */

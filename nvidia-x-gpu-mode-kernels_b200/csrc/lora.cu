@@ -3,14 +3,13 @@
 //   out[t] = fp16( base[t] + scale_i * ((x[t] . A_i^T) . B_i^T) ),   i = adapters[t]
 //
 // A_i [r, K], B_i [N, r] (fp16), of which adapter i uses its first ranks[i] rows / columns.  Tokens without
-// an adapter (an index outside [0, n)) keep base.  Bytes bound both forms: x, base and out once, and the
-// matrices of the adapters in use.
+// an adapter (an index outside [0, n)) keep base.  The floor of both forms is their bytes: x, base and out once,
+// and the matrices of the adapters in use.
 //
-// The products run on mma.sync (fp16 operands, fp32 accumulators): with ranks of 16 to 128 there is too
-// little arithmetic per byte for tensor memory and its round trips to pay.  u = x . A^T enters the second
-// product as two fp16 halves, u = 2^-p (hi + lo), with a 2^p per token that brings its largest |u| to [2^14, 2^15): each u
-// keeps 22 bits, or is off by at most 2^-39 of the largest, where lo reaches the end of fp16's range.  The sum stays in
-// fp32.
+// The products run on mma.sync (fp16 operands, fp32 accumulators): with ranks of 16 to 128 there is little arithmetic
+// per byte for tensor memory's round trips.  u = x . A^T enters the second product as two fp16 halves, u = 2^-p (hi + lo),
+// with a 2^p per token that brings its largest |u| to [2^14, 2^15): each u keeps 22 bits, or is off by at most 2^-39 of the
+// largest, where lo reaches the end of fp16's range.  The sum stays in fp32.
 //
 // The k index of an mma is summed over, so its 16 slots may stand for any 16 elements as long as both operands
 // agree.  Two mma's take 32 elements, slots {2q, 2q+1, 2q+8, 2q+9} of lane q of 4 standing for elements 8q..8q+3 in
@@ -607,7 +606,8 @@ __global__ void __launch_bounds__(kLoraThreads, RT <= 4 ? 2 : 1) shrink_kernel(c
 // out += u . B^T for 128 tokens of one adapter and a run of columns, 64 at a time: a warp takes 16 tokens, whose u
 // stays in its registers.  B comes through a ring in shared memory that all warps read; base through a ring of
 // which each lane reads back just what it asked for itself.
-// 8192 tokens, N = 14336, r = 64: 114 us at 50 % of DRAM.  9 instructions for 32 outputs at 15 warps an SM bound it
+// 8192 tokens, N = 14336, r = 64: 112 us at 51 % of DRAM.  11 instructions for 32 outputs at 15 warps an SM bound it, not
+// bytes (tensor memory, which would free the accumulators' registers, has not been tried)
 // (registers: three CTAs an SM spill, 164 -> 230 us, four 267, in an earlier form).  Base is read before the products
 // where registers allow (r = 64: 141.6 us a call against 151.0 with it read after them, r = 128: 305.5 and 270.6).
 // The 8 columns of mma tile j of four stand for columns 8 (c / 2) + 2 j + c % 2 of 32, so that the four tiles
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2)
       if (live) {
         const __half* const bs = bget + ring * (C::EXPAND_B / 2);
         auto columns = [&](auto full) {
-          // all 64 columns exist: without the code for the last ones 141.7 -> 137.2 us a call (8192 tokens, r = 64)
+          // all 64 columns exist: without the code for the last ones 3 % less a call (8192 tokens, r = 64)
           constexpr bool FULL = decltype(full)::value;
 #pragma unroll
           for (int half = 0; half < 2; ++half) {

@@ -37,7 +37,7 @@
 // a stage, 5 slots; before the one MMA for both): 935 us a call against 954, the
 // gate and up product alone slower (516 against 481).  Prefetching weights into
 // L2: no gain.  Under minutes of such work the power
-// limit takes its share, too (782 us a call before it sets in, 908 after).
+// limit takes its share, too (772 us a call before it sets in, 909 after).
 #pragma once
 #include "plan.cuh"
 #include "quant.cuh"

@@ -24,9 +24,9 @@
 //                with its lowest index; also the 64-bit pass, over double.
 //
 // The bytes (a row read once) are 5 us at 32768 x 256; what bounds the kernel is the issue of comparisons and
-// selections: 568 instructions a row of 256 experts with a bias in 8 groups, two of three cycles issue one (37 us).
-// Keys for every row took 88 us, comparing floats 58, the short form for rows without surprises 48, weights and
-// stores of several rows together and groups as runs of lanes 37.  top_k = 8 of a softmax without a bias: 19 us.
+// selections: 575 instructions a row of 256 experts with a bias in 8 groups, two of three cycles issue one (41 us in a
+// graph).  Keys for every row took 88 us, comparing floats 58, the short form for rows without surprises 48; weights and
+// stores of several rows together and groups as runs of lanes followed.  top_k = 8 of a softmax without a bias: 17 us.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
